@@ -9,6 +9,7 @@
 #include <stdlib.h>
 
 #include "../../include/lycoris_amd.h"
+#include "errors.h"
 #include "conv_kernels.h"
 #include "dense_kernels.h"
 #include "ia3_kernels.h"
@@ -34,22 +35,6 @@
 using namespace lyc;
 
 namespace {
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-int check_launch(const char* what) {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(LYC_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
-  return LYC_OK;
-}
-
 inline long cdiv(long a, long b) { return (a + b - 1) / b; }
 inline long round_up(long a, long b) { return cdiv(a, b) * b; }
 
