@@ -54,7 +54,7 @@ enum { LYC_F32_ROWS = 0x100, LYC_DEFER_WGRAD = 0x200,
 #define LYC_KCONV_ROW_TILE(mi) (((mi) & 0xf) << 12)
 enum { LYC_OK = 0, LYC_ERR_ARG = 1, LYC_ERR_UNSUPPORTED = 2, LYC_ERR_LAUNCH = 3 };
 
-#define LYC_ABI_VERSION 13
+#define LYC_ABI_VERSION 14
 int lyc_abi_version(void);
 const char* lyc_last_error(void);
 
@@ -463,6 +463,37 @@ int lyc_col2im_rows(const void* dcols, void* dx_rows, int64_t B, int64_t C, int6
                     int pw, int dh, int dw, int dtype, void* stream);
 int lyc_nchw_to_rows(const void* t, void* rows, int64_t B, int64_t C, int64_t P, int dtype, void* stream);
 int lyc_rows_to_nchw(const void* rows, void* t, int64_t B, int64_t C, int64_t P, int dtype, void* stream);
+
+/* ---- frozen layers held in 8 bits ---------------------------------------------------------------------
+ * The frozen nn.Linear under an adapter (the `org_forward(x)` of every lycoris/modules forward) with its weight kept as integers:
+ *   w[n, k] ~= sw[n] wq[n, k],  sw[n] = max_k |w[n, k]| / 127,  wq = round-half-even(127 w / max|w|)   (lyc_int8_quantize on its rows)
+ * and its input quantised the same way, one scale a row, on every call.  A row that holds an infinity or a NaN gets scale NaN.
+ * Rows of 8-bit operands: 16-byte aligned base, pitch a multiple of 16.  K <= 2^17 (the int32 sums cannot overflow).
+ * `bias`: [N], fp32 when bias_f32, else `dtype`; `base`: [M, N] in `dtype` (an adapter's output), either may be NULL.
+ * `ws`: device scratch of the *_workspace_bytes(...) bytes (-1: bad arguments), 16-byte aligned, no need to clear.        */
+int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int64_t K, int dtype, void* stream);
+/* y = (sa[m] sb[n]) sum_k aq[m, k] bq[n, k] + bias[n] + base[m, n].  aq's rows hold ZEROS from K up to the next multiple of 16. */
+int lyc_int8_matmul(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32,
+                    const void* base, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+int64_t lyc_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int backward);
+int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* y, void* ws,
+                        int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+/* dx = g (sw wq): the gradient is not quantised; the weight is expanded to the activation type (32 bits: three bf16 products) */
+int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const float* sw, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int dtype,
+                        void* stream);
+
+/* ---- gated projection of a feed-forward block ------------------------------------------------------------
+ *   p = x w^T + bias + base  [M, 2 F];   h = value * act(gate)  [M, F]
+ * value and gate are the halves of p's columns (value first, or gate first with gate_first).  w [2 F, I] in `dtype`, contiguous, or 8-bit
+ * rows of pitch ldw with scales sw (then x is quantised as above).  `pre` (training): receives p rounded to `dtype`, which bwd reads.
+ * bwd, each output optional: dbase = dp [M, 2 F], dx = dp w, dw = dp^T x (not with an 8-bit weight), dbias = sum_m dp.          */
+enum { LYC_ACT_GELU = 0, LYC_ACT_GELU_TANH = 1, LYC_ACT_SILU = 2 };
+enum { LYC_GATED_INT8 = 1, LYC_GATED_BACKWARD = 2, LYC_GATED_DBASE = 4, LYC_GATED_DX = 8, LYC_GATED_DW = 16, LYC_GATED_DBIAS = 32 };
+int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dtype, int flags);
+int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* h, void* pre,
+                         void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream);
+int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const void* w, int64_t ldw, const float* sw, void* dbase, void* dx, void* dw,
+                         void* dbias, void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,7 @@ from __future__ import annotations
 __version__ = "0.1.0"
 
 from . import functional, modules, ops  # noqa: F401
-from .modules import IA3Module, LoConModule, LohaModule, LokrModule  # noqa: F401
+from .modules import GatedLinear, IA3Module, Int8Linear, LoConModule, LohaModule, LokrModule, quantize_frozen  # noqa: F401
 
 NATIVE_ALGOS = {"lora": LoConModule, "locon": LoConModule, "loha": LohaModule, "lokr": LokrModule, "ia3": IA3Module}
 _installed = {}

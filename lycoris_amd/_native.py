@@ -13,7 +13,7 @@ import torch
 
 _LIB_NAME = "liblycoris_amd.so"
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), _LIB_NAME)
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 LYC_F32, LYC_F16, LYC_BF16 = 0, 1, 2
 _DTYPE_CODE = {torch.float32: LYC_F32, torch.float16: LYC_F16, torch.bfloat16: LYC_BF16}
@@ -70,6 +70,12 @@ SIGNATURES = {
     "lyc_lokr_linear_bwd_group_sum": [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _vp],
     "lyc_nchw_to_rows": [_vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_rows_to_nchw": [_vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "lyc_int8_quantize": [_vp, _i64, _vp, _i64, _fp, _i64, _i64, _i32, _vp],
+    "lyc_int8_matmul": [_vp, _i64, _fp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "lyc_int8_linear_fwd": [_vp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "lyc_int8_linear_bwd": [_vp, _vp, _i64, _fp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "lyc_gated_linear_fwd": [_vp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+    "lyc_gated_linear_bwd": [_vp, _vp, _vp, _vp, _i64, _fp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
 }
 # entry points that return something other than a status code
 VALUE_SIGNATURES = {
@@ -85,6 +91,8 @@ VALUE_SIGNATURES = {
     "lyc_lokr_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32], ctypes.c_int),  # 1 / 0, not an error code
     "lyc_locon_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32], ctypes.c_int),
     "lyc_loha_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32], ctypes.c_int),
+    "lyc_int8_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
+    "lyc_gated_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
     "lyc_loha_plane_cacheable": ([_fp, _fp, _fp, _fp, _i32, _i32, _i32, _i32], ctypes.c_int),
 }
 

@@ -93,3 +93,77 @@ def lokr_conv2d(x, w1, w2, alpha, stride, padding, dilation):
 def loha_conv2d(x, w1a, w1b, w2a, w2b, alpha, shape, stride, padding, dilation):
     dw = (_hada(w1a, w1b.reshape(w1b.shape[0], -1), w2a, w2b.reshape(w2b.shape[0], -1)) * alpha).reshape(tuple(shape))
     return F.conv2d(x, dw.to(x.dtype), None, tuple(stride), tuple(padding), tuple(dilation))
+
+
+def int8_quantize(x):
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"int8_quantize: x must have rows, got {tuple(x.shape)}")
+    amax = x.abs().amax(-1, keepdim=True).double()
+    ok = torch.isfinite(amax)
+    q = torch.round(127.0 * x.double() / torch.where(ok & (amax > 0), amax, torch.ones_like(amax)))
+    q = torch.where(ok, q, torch.zeros_like(q)).to(torch.int8)
+    return q, torch.where(ok, amax.float() / 127.0, torch.full_like(amax, float("nan")).float())[..., 0]
+
+
+def int8_matmul(aq, a_scale, bq, b_scale, bias, dtype):
+    _check_w8(bq, "int8_matmul")
+    if aq.shape[-1] != bq.shape[1]:
+        raise RuntimeError(f"int8_matmul: a has rows of {aq.shape[-1]}, b of {bq.shape[1]}")
+    y = (aq.double() @ bq.double().t()).float() * a_scale.reshape(*aq.shape[:-1], 1) * b_scale.reshape(-1)
+    return (y if bias is None else y + bias.float()).to(dtype)
+
+
+def _check_w8(wq, what):
+    if wq.dim() != 2 or wq.dtype != torch.int8 or 0 in wq.shape:
+        raise RuntimeError(f"{what}: the 8-bit operand must be a non-empty int8 matrix, got {tuple(wq.shape)} {wq.dtype}")
+
+
+def _check_base(base, x, n):
+    if base is not None and tuple(base.shape) != (*x.shape[:-1], n):
+        raise RuntimeError(f"base must be {(*x.shape[:-1], n)}, got {tuple(base.shape)}")
+
+
+def _held_product(x, wq, w_scale, what):
+    """the 8-bit product in 32 bits (64 for float64 x), with the straight-through derivative: forward of the quantised product, backward of
+    x times the weight as it is held"""
+    _check_w8(wq, what)
+    if x.shape[-1] != wq.shape[1]:
+        raise RuntimeError(f"{what}: x has {x.shape[-1]} features, the weight {wq.shape[1]}")
+    ct = torch.promote_types(x.dtype, torch.float32)
+    straight = x.to(ct) @ (wq.to(ct) * w_scale.to(ct).reshape(-1, 1)).t()
+    q, s = int8_quantize(x.detach())
+    y = (q.double() @ wq.double().t()).to(ct) * s.to(ct)[..., None] * w_scale.to(ct).reshape(-1)
+    return straight + (y - straight).detach()
+
+
+def int8_linear(x, wq, w_scale, bias=None, base=None):
+    if w_scale.requires_grad or (bias is not None and bias.requires_grad):
+        raise RuntimeError("int8_linear: the layer is frozen, its scale and bias cannot require a gradient")
+    y = _held_product(x, wq, w_scale, "int8_linear")
+    _check_base(base, x, wq.shape[0])
+    for t in (bias, base):
+        y = y if t is None else y + t.to(y.dtype)
+    return y.to(x.dtype)
+
+
+def gated_linear(x, weight, bias=None, base=None, act="gelu", gate_first=False, weight_scale=None):
+    if weight.dim() != 2 or weight.shape[0] % 2 or 0 in weight.shape:
+        raise RuntimeError(f"gated_linear: the weight must be [2 F, I], got {tuple(weight.shape)}")
+    if weight_scale is not None:
+        if weight_scale.requires_grad:
+            raise RuntimeError("gated_linear: an 8-bit weight is frozen, its scale cannot require a gradient")
+        p = _held_product(x, weight, weight_scale, "gated_linear")
+    else:
+        if weight.dtype != x.dtype:
+            raise RuntimeError(f"gated_linear: the weight is {weight.dtype}, the activation {x.dtype}; an int8 weight needs its scale")
+        if x.shape[-1] != weight.shape[1]:
+            raise RuntimeError(f"gated_linear: x has {x.shape[-1]} features, the weight {weight.shape[1]}")
+        ct = torch.promote_types(x.dtype, torch.float32)
+        p = x.to(ct) @ weight.to(ct).t()
+    _check_base(base, x, weight.shape[0])
+    for t in (bias, base):
+        p = p if t is None else p + t.to(p.dtype)
+    first, second = p.chunk(2, -1)
+    value, gate = (second, first) if gate_first else (first, second)
+    a = F.silu(gate) if act == "silu" else F.gelu(gate, approximate="tanh" if act == "gelu_tanh" else "none")
+    return (value * a).to(x.dtype)

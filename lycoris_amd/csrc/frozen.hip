@@ -1,0 +1,414 @@
+// frozen.hip -- C ABI of the 8-bit frozen layer and the gated projection (include/lycoris_amd.h).  gfx950 only.
+#include <hip/hip_runtime.h>
+
+#include <atomic>
+
+#include "../../include/lycoris_amd.h"
+#include "errors.h"
+#include "frozen_rows.h"
+
+using namespace lyc;
+
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+
+#define FZ_DTYPE(dtype_, ...)                                        \
+  switch (dtype_) {                                                  \
+    case LYC_BF16: { using T = __bf16; __VA_ARGS__; } break;         \
+    case LYC_F16: { using T = _Float16; __VA_ARGS__; } break;        \
+    case LYC_F32: { using T = float; __VA_ARGS__; } break;           \
+    default: return fail(LYC_ERR_ARG, "unknown dtype %d", dtype_);   \
+  }
+
+// a workspace handed out piece by piece; with a null base it only counts
+struct Carve {
+  char* base;
+  int64_t used = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    used = up(used, 256);
+    T* r = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += n * (int64_t)sizeof(T);
+    return r;
+  }
+};
+
+int check_dims(const char* who, int64_t M, int64_t N, int64_t K, int dtype) {
+  if (dtype != LYC_F32 && dtype != LYC_F16 && dtype != LYC_BF16) return fail(LYC_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+  if (M < 0 || N < 1 || K < 1) return fail(LYC_ERR_ARG, "%s: bad dims M=%ld N=%ld K=%ld", who, (long)M, (long)N, (long)K);
+  if (M > (1 << 30) || N > (1 << 20) || K > (1 << 17))
+    return fail(LYC_ERR_UNSUPPORTED, "%s: M=%ld N=%ld K=%ld exceed 2^30 rows, 2^20 outputs or 2^17 inputs", who, (long)M, (long)N, (long)K);
+  return LYC_OK;
+}
+#define FZ_TRY(expr)                  \
+  do {                                \
+    const int rc_ = (expr);           \
+    if (rc_ != LYC_OK) return rc_;    \
+  } while (0)
+
+int need16(const char* who, const char* what, const void* p, bool optional = false) {
+  if (!p) return optional ? LYC_OK : fail(LYC_ERR_ARG, "%s: null pointer (%s)", who, what);
+  return fz_al16(p) ? LYC_OK : fail(LYC_ERR_ARG, "%s: %s must be 16-byte aligned", who, what);
+}
+
+// dynamic LDS above 64 KiB is allowed per kernel AND device
+template <typename Kern>
+int allow_lds(Kern kern, int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return fail(LYC_ERR_LAUNCH, "hipGetDevice failed");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return LYC_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return fail(LYC_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return LYC_OK;
+}
+
+template <typename K, int BM, int BNO>
+int launch_tile(const FzProb& p, const FzEpi& ep, int64_t NO, hipStream_t st) {
+  const G16DMap mp = gemm16d_map((int)cdiv(p.M, BM), (int)cdiv(NO, BNO), p.M, p.N);
+  FZ_TRY(allow_lds(&fz_gemm_kernel<K>, K::LDS));
+  hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * mp.tm_per * mp.tn_per)), dim3(K::NW * 64), K::LDS, st, p, ep);
+  return check_launch("fz_gemm");
+}
+template <typename E, typename TO, bool A_KS, bool B_KS, int EPI>
+int launch_gemm(const FzProb& p, const FzEpi& ep, hipStream_t st) {
+  constexpr bool G = EPI == FZ_GATED;
+  return launch_tile<FzKernel<E, TO, 128, 128, 2, 2, 2, A_KS, B_KS, EPI>, 128, G ? 64 : 128>(p, ep, G ? ep.F : p.N, st);
+}
+
+template <typename T>
+int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int K, hipStream_t st) {
+  const int vec = fz_al16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0 && K % 8 == 0;
+  const int64_t c = ldq / 8;  // chunks of 8 a row
+  auto go = [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+    hipLaunchKernelGGL((fz_quant_kernel<T, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
+  };
+  using std::integral_constant;
+  if (c <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (c <= 128) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (c <= 256) go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (c <= 512) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (c <= 1024) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else hipLaunchKernelGGL((fz_quant_long_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
+  return check_launch("int8_quantize");
+}
+
+int grid_of(int64_t chunks) { return (int)(cdiv(chunks, 256) < 16384 ? cdiv(chunks, 256) : 16384); }
+
+// x [rows, cols] contiguous -> NP planes of [rows, up(cols, 8)]
+template <typename TI, typename TO, int NP>
+int launch_stage(const TI* x, const float* col, TO* out, int64_t rows, int64_t cols, hipStream_t st) {
+  const int64_t ldo = up(cols, 8);
+  const int vec = fz_al16(x) && cols % 8 == 0;
+  hipLaunchKernelGGL((fz_stage_kernel<TI, TO, NP>), dim3(grid_of(rows * ldo / 8)), dim3(256), 0, st, x, col, out, ldo, rows, (int)cols, vec);
+  return check_launch("stage");
+}
+template <typename T>
+int launch_plane(const int8_t* q, int64_t ldq, const float* sw, T* out, float* alpha, int64_t O, int64_t I, int scaled, hipStream_t st) {
+  const int rows = std::is_same<T, _Float16>::value ? 16 : 4;  // fp16: every workgroup reads all scales first
+  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, sw, out, up(I, 8), alpha, (int)O, (int)I, rows, scaled);
+  return check_launch("weight plane");
+}
+
+// One operand of a product in the type the matrix cores take: the tensor itself, its staged copy, or its three bf16 planes.
+template <typename T>
+struct Operand {
+  using E = typename std::conditional<sizeof(T) == 4, __bf16, T>::type;
+  const void* p = nullptr;
+  int64_t ld = 0, plane = 0;  // bytes
+  void* room = nullptr;
+  int64_t rows, cols;
+  bool own;
+  Operand(Carve& ws, int64_t rows_, int64_t cols_, bool wanted) : rows(rows_), cols(cols_), own(sizeof(T) == 4 || cols_ % 8 != 0) {
+    if (wanted && own) room = ws.take<E>((sizeof(T) == 4 ? 3 : 1) * rows * up(cols, 8));
+  }
+  int fill(const T* x, const float* col, hipStream_t st) {
+    if (!own) {
+      p = x;
+      ld = cols * (int64_t)sizeof(T);
+      return LYC_OK;
+    }
+    p = room;
+    ld = up(cols, 8) * 2;
+    plane = rows * ld;
+    return launch_stage<T, E, sizeof(T) == 4 ? 3 : 1>(x, col, static_cast<E*>(room), rows, cols, st);
+  }
+};
+// segments: 16-bit 1; fp32 x fp32 6; fp32 x exact bf16 (an 8-bit weight's integers) 3.  The small terms come first.
+void segments(FzProb& p, int n) {
+  p.nseg = n;
+  p.pa = n == 6 ? 0x010120u : n == 3 ? 0x012u : 0u;
+  p.pb = n == 6 ? 0x001102u : 0u;
+}
+
+FzProb prob(const void* A, int64_t lda, int64_t a_plane, const void* B, int64_t ldb, int64_t b_plane, int64_t M, int64_t N, int64_t K, int es) {
+  FzProb p{};
+  p.A = A; p.B = B; p.lda = lda; p.ldb = ldb; p.a_plane = a_plane; p.b_plane = b_plane;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  p.kb = (int)up(K * es, 16);
+  p.nseg = 1;
+  return p;
+}
+
+int matmul8(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32, const void* base,
+            void* y, int64_t M, int64_t N, int64_t K, int dtype, hipStream_t st) {
+  FzProb p = prob(aq, lda, 0, bq, ldb, 0, M, N, K, 1);
+  FzEpi ep{};
+  ep.out = y; ep.sa = sa; ep.sw = sb; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base;
+  FZ_DTYPE(dtype, return (launch_gemm<int8_t, T, false, false, FZ_LINEAR>(p, ep, st)));
+  return LYC_OK;
+}
+
+int check_q(const char* who, const char* what, const void* q, int64_t ld, int64_t K) {
+  FZ_TRY(need16(who, what, q));
+  if (ld < K || ld % 16 || ld > (1 << 22)) return fail(LYC_ERR_ARG, "%s: the row pitch of %s must be a multiple of 16, at least K and at most 2^22 (%ld)", who, what, (long)ld);
+  return LYC_OK;
+}
+
+// ---- dx of a frozen 8-bit layer: g [M, N] times (sw wq) [N, K] -------------------------------------------------------------------------
+template <typename T>
+int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve ws, int64_t* bytes, int64_t M, int64_t N, int64_t K, hipStream_t st) {
+  using E = typename Operand<T>::E;
+  E* plane = ws.take<E>(N * up(K, 8));
+  float* alpha = ws.take<float>(1);
+  Operand<T> a(ws, M, N, true);
+  if (bytes) {
+    *bytes = ws.used;
+    return LYC_OK;
+  }
+  constexpr bool F32 = sizeof(T) == 4;
+  FZ_TRY(launch_plane<E>(wq, ldw, sw, plane, alpha, N, K, !F32, st));
+  FZ_TRY(a.fill(g, F32 ? sw : nullptr, st));
+  FzProb p = prob(a.p, a.ld, a.plane, plane, up(K, 8) * 2, 0, M, K, N, 2);
+  segments(p, F32 ? 3 : 1);
+  FzEpi ep{};
+  ep.out = dx;
+  ep.alpha = std::is_same<T, _Float16>::value ? alpha : nullptr;
+  return launch_gemm<E, T, false, true, FZ_PLAIN>(p, ep, st);
+}
+
+// ---- gated projection ---------------------------------------------------------------------------------------------------------------------
+struct Gated {
+  const void* w;
+  int64_t ldw;
+  const float* sw;
+  int64_t M, I, F;
+  int act, gate_first;
+};
+
+template <typename T>
+int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const T* base, T* h, T* pre, Carve ws, int64_t* bytes, hipStream_t st) {
+  using E = typename Operand<T>::E;
+  FzEpi ep{};
+  ep.out = h; ep.pre = pre; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base; ep.sw = q.sw; ep.act = q.act; ep.gate_first = q.gate_first; ep.F = (int)q.F;
+  if (q.sw) {
+    const int64_t ldq = up(q.I, 16);
+    int8_t* xq = ws.take<int8_t>(q.M * ldq);
+    float* sa = ws.take<float>(q.M);
+    if (bytes) {
+      *bytes = ws.used;
+      return LYC_OK;
+    }
+    FZ_TRY(launch_quant<T>(x, q.I, xq, ldq, sa, q.M, (int)q.I, st));
+    ep.sa = sa;
+    FzProb p = prob(xq, ldq, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
+    return launch_gemm<int8_t, T, false, false, FZ_GATED>(p, ep, st);
+  }
+  Operand<T> a(ws, q.M, q.I, true), b(ws, 2 * q.F, q.I, true);
+  if (bytes) {
+    *bytes = ws.used;
+    return LYC_OK;
+  }
+  FZ_TRY(a.fill(x, nullptr, st));
+  FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
+  FzProb p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, 2 * q.F, q.I, 2);
+  segments(p, sizeof(T) == 4 ? 6 : 1);
+  return launch_gemm<E, T, false, false, FZ_GATED>(p, ep, st);
+}
+
+template <typename T>
+int gated_bwd(const Gated& q, const T* g, const T* pre, const T* x, T* dp, T* dx, T* dw, T* dbias, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
+  using E = typename Operand<T>::E;
+  constexpr bool F32 = sizeof(T) == 4;
+  const bool held = flags & LYC_GATED_INT8;
+  const int64_t N = 2 * q.F, parts = cdiv(q.M, FZ_SUM_ROWS);
+  if (!(flags & LYC_GATED_DBASE)) dp = ws.take<T>(q.M * N);
+  const bool want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
+  Operand<T> a(ws, q.M, N, want_dx || want_dw);  // dp as the products' operand (K-contiguous for dx, K-strided for dw)
+  Operand<T> b(ws, N, q.I, want_dx && !held), xo(ws, q.M, q.I, want_dw);
+  E* plane = want_dx && held ? ws.take<E>(N * up(q.I, 8)) : nullptr;
+  float* alpha = ws.take<float>(1);
+  float* part = flags & LYC_GATED_DBIAS ? ws.take<float>(parts * N) : nullptr;
+  if (bytes) {
+    *bytes = ws.used;
+    return LYC_OK;
+  }
+  const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp);
+  hipLaunchKernelGGL((fz_dgate_kernel<T>), dim3(grid_of(q.M * cdiv(q.F, 8))), dim3(256), 0, st, g, pre, dp, q.M, (int)q.F, q.act, q.gate_first, vec);
+  FZ_TRY(check_launch("gated backward"));
+  if (want_dx || want_dw) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));
+  if (want_dx) {
+    FzEpi ep{};
+    ep.out = dx;
+    FzProb p;
+    if (held) {
+      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, q.sw, plane, alpha, N, q.I, !F32, st));
+      p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
+      ep.alpha = std::is_same<T, _Float16>::value ? alpha : nullptr;
+    } else {
+      FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
+      p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, q.I, N, 2);
+    }
+    segments(p, F32 ? (held ? 3 : 6) : 1);
+    FZ_TRY((launch_gemm<E, T, false, true, FZ_PLAIN>(p, ep, st)));
+  }
+  if (want_dw) {
+    FZ_TRY(xo.fill(x, nullptr, st));
+    FzProb p = prob(a.p, a.ld, a.plane, xo.p, xo.ld, xo.plane, N, q.I, q.M, 2);
+    segments(p, F32 ? 6 : 1);
+    FzEpi ep{};
+    ep.out = dw;
+    FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(p, ep, st)));
+  }
+  if (part) {
+    hipLaunchKernelGGL((fz_colsum_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)parts), dim3(256), 0, st, dp, part, q.M, (int)N);
+    hipLaunchKernelGGL((fz_colsum_join_kernel<T>), dim3((unsigned)cdiv(N, 256)), dim3(256), 0, st, part, dbias, (int)parts, (int)N);
+    FZ_TRY(check_launch("column sums"));
+  }
+  return LYC_OK;
+}
+
+int check_gated(const char* who, const Gated& q, bool held, int dtype) {
+  if (q.F > (1 << 19)) return fail(LYC_ERR_UNSUPPORTED, "%s: F=%ld exceeds 2^19", who, (long)q.F);
+  FZ_TRY(check_dims(who, q.M, q.F < 1 ? 0 : 2 * q.F, q.I, dtype));
+  if (q.act < 0 || q.act > 2) return fail(LYC_ERR_ARG, "%s: unknown activation %d", who, q.act);
+  if ((q.F + 512) * (held ? q.ldw : up(q.I, 8) * 2) >= ((int64_t)1 << 31)) return fail(LYC_ERR_UNSUPPORTED, "%s: half a weight of 2 GiB or more", who);
+  return LYC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int64_t K, int dtype, void* stream) {
+  FZ_TRY(check_dims("int8_quantize", M, 1, K, dtype));
+  if (M == 0) return LYC_OK;
+  if (!x || !scale) return fail(LYC_ERR_ARG, "int8_quantize: null pointer");
+  if (ldx < K) return fail(LYC_ERR_ARG, "int8_quantize: the row pitch of x is %ld, below K=%ld", (long)ldx, (long)K);
+  FZ_TRY(check_q("int8_quantize", "q", q, ldq, K));
+  FZ_DTYPE(dtype, return launch_quant<T>(static_cast<const T*>(x), ldx, q, ldq, scale, M, (int)K, static_cast<hipStream_t>(stream)));
+  return LYC_OK;
+}
+
+int lyc_int8_matmul(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32,
+                    const void* base, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
+  FZ_TRY(check_dims("int8_matmul", M, N, K, dtype));
+  if (M == 0) return LYC_OK;
+  if (!sa || !sb || !y) return fail(LYC_ERR_ARG, "int8_matmul: null pointer");
+  FZ_TRY(check_q("int8_matmul", "a", aq, lda, K));
+  FZ_TRY(check_q("int8_matmul", "b", bq, ldb, K));
+  return matmul8(aq, lda, sa, bq, ldb, sb, bias, bias_f32, base, y, M, N, K, dtype, static_cast<hipStream_t>(stream));
+}
+
+int64_t lyc_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int backward) {
+  if (check_dims("int8_linear", M, N, K, dtype) != LYC_OK) return -1;
+  Carve ws{nullptr};
+  if (!backward) {
+    ws.take<int8_t>(M * up(K, 16));
+    ws.take<float>(M);
+    return ws.used;
+  }
+  int64_t n = 0;
+  FZ_DTYPE(dtype, (void)dx8<T>(nullptr, nullptr, 0, nullptr, nullptr, ws, &n, M, N, K, nullptr));
+  return n;
+}
+
+int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* y, void* ws,
+                        int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
+  const char* who = "int8_linear_fwd";
+  FZ_TRY(check_dims(who, M, N, K, dtype));
+  if (M == 0) return LYC_OK;
+  if (!x || !sw || !y) return fail(LYC_ERR_ARG, "%s: null pointer", who);
+  FZ_TRY(need16(who, "workspace", ws));
+  FZ_TRY(check_q(who, "wq", wq, ldw, K));
+  Carve c{static_cast<char*>(ws)};
+  const int64_t ldq = up(K, 16);
+  int8_t* xq = c.take<int8_t>(M * ldq);
+  float* sa = c.take<float>(M);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  FZ_DTYPE(dtype, FZ_TRY(launch_quant<T>(static_cast<const T*>(x), K, xq, ldq, sa, M, (int)K, st)));
+  return matmul8(xq, ldq, sa, wq, ldw, sw, bias, bias_f32, base, y, M, N, K, dtype, st);
+}
+
+int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const float* sw, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int dtype,
+                        void* stream) {
+  const char* who = "int8_linear_bwd";
+  FZ_TRY(check_dims(who, M, N, K, dtype));
+  if (M == 0) return LYC_OK;
+  if (!sw || !dx) return fail(LYC_ERR_ARG, "%s: null pointer", who);
+  FZ_TRY(need16(who, "g", g));
+  FZ_TRY(need16(who, "workspace", ws));
+  FZ_TRY(check_q(who, "wq", wq, ldw, K));
+  FZ_DTYPE(dtype, return dx8<T>(static_cast<const T*>(g), wq, ldw, sw, static_cast<T*>(dx), Carve{static_cast<char*>(ws)}, nullptr, M, N, K,
+                                static_cast<hipStream_t>(stream)));
+  return LYC_OK;
+}
+
+int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dtype, int flags) {
+  Gated q{nullptr, 16, nullptr, M, I, F, 0, 0};
+  if (check_gated("gated_linear", q, true, dtype) != LYC_OK) return -1;
+  int64_t n = 0;
+  const float one = 1.f;
+  Carve ws{nullptr};
+  if (flags & LYC_GATED_BACKWARD) {
+    FZ_DTYPE(dtype, (void)gated_bwd<T>(q, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, flags, ws, &n, nullptr));
+  } else {
+    q.sw = flags & LYC_GATED_INT8 ? &one : nullptr;
+    FZ_DTYPE(dtype, (void)gated_fwd<T>(q, nullptr, nullptr, 0, nullptr, nullptr, nullptr, ws, &n, nullptr));
+  }
+  return n;
+}
+
+int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* h, void* pre,
+                         void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream) {
+  const char* who = "gated_linear_fwd";
+  const Gated q{w, ldw, sw, M, I, F, act, gate_first};
+  FZ_TRY(check_gated(who, q, sw != nullptr, dtype));
+  if (M == 0) return LYC_OK;
+  if (!h) return fail(LYC_ERR_ARG, "%s: null pointer", who);
+  FZ_TRY(need16(who, "x", x));
+  FZ_TRY(need16(who, "workspace", ws, lyc_gated_linear_workspace_bytes(M, I, F, dtype, sw ? LYC_GATED_INT8 : 0) == 0));
+  if (sw) FZ_TRY(check_q(who, "w", w, ldw, I));
+  else FZ_TRY(need16(who, "w", w));
+  FZ_DTYPE(dtype, return gated_fwd<T>(q, static_cast<const T*>(x), bias, bias_f32, static_cast<const T*>(base), static_cast<T*>(h), static_cast<T*>(pre),
+                                      Carve{static_cast<char*>(ws)}, nullptr, static_cast<hipStream_t>(stream)));
+  return LYC_OK;
+}
+
+int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const void* w, int64_t ldw, const float* sw, void* dbase, void* dx, void* dw,
+                         void* dbias, void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream) {
+  const char* who = "gated_linear_bwd";
+  const Gated q{w, ldw, sw, M, I, F, act, gate_first};
+  FZ_TRY(check_gated(who, q, sw != nullptr, dtype));
+  if (dw && sw) return fail(LYC_ERR_UNSUPPORTED, "%s: an 8-bit weight is frozen", who);
+  if (M == 0) return LYC_OK;
+  if (!g || !pre) return fail(LYC_ERR_ARG, "%s: null pointer", who);
+  if (dx && sw) FZ_TRY(check_q(who, "w", w, ldw, I));
+  else if (dx) FZ_TRY(need16(who, "w", w));
+  if (dw) FZ_TRY(need16(who, "x", x));
+  FZ_TRY(need16(who, "dbase", dbase, true));
+  FZ_TRY(need16(who, "workspace", ws));
+  const int flags = LYC_GATED_BACKWARD | (sw ? LYC_GATED_INT8 : 0) | (dbase ? LYC_GATED_DBASE : 0) | (dx ? LYC_GATED_DX : 0) | (dw ? LYC_GATED_DW : 0) |
+                    (dbias ? LYC_GATED_DBIAS : 0);
+  FZ_DTYPE(dtype, return gated_bwd<T>(q, static_cast<const T*>(g), static_cast<const T*>(pre), static_cast<const T*>(x), static_cast<T*>(dbase),
+                                      static_cast<T*>(dx), static_cast<T*>(dw), static_cast<T*>(dbias), flags, Carve{static_cast<char*>(ws)}, nullptr,
+                                      static_cast<hipStream_t>(stream)));
+  return LYC_OK;
+}
+
+}  // extern "C"

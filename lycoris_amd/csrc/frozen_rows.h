@@ -1,0 +1,227 @@
+// frozen_rows.h -- the row kernels around the products of frozen_gemm.h: quantisation, weight planes, operand staging, the gated
+// backward's elementwise pass, column sums.  All of them are bound by HBM (or, for one row, by the launch).
+#pragma once
+#include "frozen_gemm.h"
+
+namespace lyc {
+
+// 8 elements of a row from column k on (beyond K: 0); `vec`: 16-byte loads are aligned and K % 8 == 0
+template <typename T>
+__device__ __forceinline__ void fz_row8(const T* row, int k, int K, bool vec, float (&v)[8]) {
+  fz_load8<T>(row, k, k, K, vec && k < K, v);
+}
+
+// ---- rows to 8-bit integers: scale = max|x| / 127, q = round-half-even(127 x / max|x|) ----------------------------------------------
+// 127 x is exact in fp32 for 16-bit inputs, and the correctly rounded quotient of two such numbers is a half exactly when the true
+// quotient is (they are at least 2^-20 apart otherwise): fp32 decides every element as exact arithmetic would.  fp32 inputs take the same
+// quotient in fp64 for the same reason.  The maximum is taken over the BIT PATTERNS of |x|, which order like the values and put infinity
+// and NaN on top: a row that holds one gets scale NaN and q = 0, so its outputs are NaN rather than silently finite.
+template <typename T>
+__device__ __forceinline__ int fz_quant(float x, float amax) {
+  if constexpr (sizeof(T) == 4) return (int)rint(127.0 * (double)x / (double)amax);
+  else return (int)rintf(127.f * x / amax);
+}
+__device__ __forceinline__ float fz_amax_of(unsigned bits, float* scale) {
+  if (bits >= 0x7f800000u) {
+    *scale = __uint_as_float(0x7fc00000u);
+    return 0.f;
+  }
+  const float a = __uint_as_float(bits);
+  *scale = a / 127.f;
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ u32x2 fz_pack_q(const float (&v)[8], float amax) {
+  u32x2 o = {0u, 0u};
+  if (amax > 0.f) {
+    const float down = amax > 1e36f ? 0x1p-16f : 1.f;  // 127 x stays finite; what this flushes rounds to 0 anyway
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e >> 2] |= ((unsigned)fz_quant<T>(v[e] * down, amax * down) & 0xffu) << (8 * (e & 3));
+  }
+  return o;
+}
+
+// TPR threads a row, each holding NV chunks of 8 elements in registers: x is read once.  Columns K .. ldq are written as zeros.
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(256) void fz_quant_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
+                                                       int64_t M, int K, int vec) {
+  __shared__ unsigned red[4];
+  const int t = threadIdx.x % TPR;
+  const int64_t m = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  float v[NV][8];
+  unsigned bits = 0;
+  if (m < M) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      fz_row8<T>(x + m * ldx, (i * TPR + t) * 8, K, vec, v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[i][e]) & 0x7fffffffu);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = bits;
+    __syncthreads();
+    bits = max(max(red[0], red[1]), max(red[2], red[3]));
+  }
+  if (m >= M) return;
+  float sc;
+  const float amax = fz_amax_of(bits, &sc);
+  if (t == 0) scale[m] = sc;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t k = (int64_t)(i * TPR + t) * 8;
+    if (k < ldq) *reinterpret_cast<u32x2*>(q + m * ldq + k) = fz_pack_q<T>(v[i], amax);
+  }
+}
+// rows too long for the registers of a workgroup: two passes, the second out of the caches
+template <typename T>
+__global__ __launch_bounds__(256) void fz_quant_long_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
+                                                            int64_t M, int K, int vec) {
+  __shared__ unsigned red[4];
+  const int64_t m = blockIdx.x;
+  const T* row = x + m * ldx;
+  unsigned bits = 0;
+  float v[8];
+  for (int k = threadIdx.x * 8; k < K; k += 2048) {
+    fz_row8<T>(row, k, K, vec, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[e]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = bits;
+  __syncthreads();
+  bits = max(max(red[0], red[1]), max(red[2], red[3]));
+  float sc;
+  const float amax = fz_amax_of(bits, &sc);
+  if (threadIdx.x == 0) scale[m] = sc;
+  for (int64_t k = threadIdx.x * 8; k < ldq; k += 2048) {
+    fz_row8<T>(row, (int)k, K, vec, v);
+    *reinterpret_cast<u32x2*>(q + m * ldq + k) = fz_pack_q<T>(v, amax);
+  }
+}
+
+// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): out[o, i] = sw[o] q[o, i] f, one rounding ---------------------
+// f = 1 in bf16.  fp16 has 5 exponent bits and the scales of a weight may lie anywhere: f = 2^e brings the largest entry to [2^13, 2^14),
+// and the product's alpha (`alpha[0] = 2^-e`) takes it out again; every workgroup finds the same e from the scales.  scaled = 0: the
+// integers themselves (exact in bf16; the fp32 product folds sw into the other operand).
+template <typename T>
+__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ sw, T* __restrict__ out, int64_t ldo,
+                                                       float* __restrict__ alpha, int O, int I, int rows_per_wg, int scaled) {
+  __shared__ float red[4];
+  float f = 1.f;
+  if constexpr (std::is_same<T, _Float16>::value) {
+    float mx = 0.f;
+    for (int o = threadIdx.x; o < O; o += 256) {
+      const float a = fabsf(sw[o]);
+      if (a <= 3.4e38f) mx = fmaxf(mx, a);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int e = mx > 1e-30f && mx < 1e30f ? 6 - ilogbf(mx) : 0;  // 127 mx < 2^(ilogb + 8)
+    f = ldexpf(1.f, e);
+    if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = ldexpf(1.f, -e);
+  }
+  const int chunks = (int)(ldo >> 3);
+  for (int r = 0; r < rows_per_wg; ++r) {
+    const int o = blockIdx.x * rows_per_wg + r;
+    if (o >= O) return;
+    const float s = scaled ? sw[o] * f : 1.f;
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      T t[8];
+      if (8 * c + 8 <= I) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(q + (int64_t)o * ldq + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)(s * (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)(8 * c + e < I ? s * (float)q[(int64_t)o * ldq + 8 * c + e] : 0.f);
+      }
+      *reinterpret_cast<u32x4*>(out + (int64_t)o * ldo + 8 * c) = *reinterpret_cast<u32x4*>(t);
+    }
+  }
+}
+
+// ---- staging: a row matrix into 16-byte aligned rows of 16-bit elements, NP planes -----------------------------------------------------
+// NP = 1: a copy (rows whose length or base is not a multiple of 16 bytes).  NP = 3, fp32: x = h + m + l in bf16, each the rounding of
+// what the ones before left; `col` scales the columns first.  Columns cols .. ldo are zeros.
+template <typename TI, typename TO, int NP>
+__global__ __launch_bounds__(256) void fz_stage_kernel(const TI* __restrict__ x, const float* __restrict__ col, TO* __restrict__ out, int64_t ldo, int64_t rows,
+                                                       int cols, int vec) {
+  const int64_t chunks = ldo >> 3, n = rows * chunks, plane = rows * ldo;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int k = (int)(i - r * chunks) * 8;
+    float v[8];
+    fz_row8<TI>(x + r * cols, k, cols, vec, v);
+    if (col) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= k + e < cols ? col[k + e] : 0.f;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      TO t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t[e] = (TO)v[e];
+        const float h = (float)t[e];
+        v[e] = fabsf(h) <= 3.4e38f ? v[e] - h : 0.f;
+      }
+      *reinterpret_cast<u32x4*>(out + p * plane + r * ldo + k) = *reinterpret_cast<u32x4*>(t);
+    }
+  }
+}
+
+// ---- gated backward, elementwise: dp = (g act(gate), g value act'(gate)) in the order of p's halves -----------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const T* __restrict__ pre, T* __restrict__ dp, int64_t M, int F, int act,
+                                                       int gate_first, int vec) {
+  const int chunks = (F + 7) >> 3;
+  const int64_t n = M * chunks;
+  const int vo = gate_first ? F : 0, go = gate_first ? 0 : F;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / chunks;
+    const int k = (int)(i - m * chunks) * 8;
+    const bool full = vec && k + 8 <= F;
+    float gv[8], v[8], t[8], dv[8], dt[8];
+    fz_load8<T>(g, m * F + k, k, F, full, gv);
+    fz_load8<T>(pre, m * 2 * F + vo + k, k, F, full, v);
+    fz_load8<T>(pre, m * 2 * F + go + k, k, F, full, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float a, da;
+      fz_act_grad(act, t[e], a, da);
+      dv[e] = gv[e] * a;
+      dt[e] = gv[e] * v[e] * da;
+    }
+    fz_store8<T>(dp, m * 2 * F + vo + k, k, F, full, dv);
+    fz_store8<T>(dp, m * 2 * F + go + k, k, F, full, dt);
+  }
+}
+
+// ---- column sums of [M, N] in two passes (fixed order: the same bits every time): partials of FZ_SUM_ROWS rows, then their sum ---------
+constexpr int FZ_SUM_ROWS = 256;
+template <typename T>
+__global__ __launch_bounds__(256) void fz_colsum_kernel(const T* __restrict__ x, float* __restrict__ part, int64_t M, int N) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  const int64_t m0 = (int64_t)blockIdx.y * FZ_SUM_ROWS, m1 = m0 + FZ_SUM_ROWS < M ? m0 + FZ_SUM_ROWS : M;
+  float s = 0.f;
+  for (int64_t m = m0; m < m1; ++m) s += (float)x[m * N + n];
+  part[(int64_t)blockIdx.y * N + n] = s;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void fz_colsum_join_kernel(const float* __restrict__ part, T* __restrict__ out, int parts, int N) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float s = 0.f;
+  for (int r = 0; r < parts; ++r) s += part[(int64_t)r * N + n];
+  out[n] = (T)s;
+}
+
+}  // namespace lyc

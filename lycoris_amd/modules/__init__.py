@@ -2,6 +2,7 @@
 import torch
 
 from .base import LycorisBaseModule
+from .frozen import GatedLinear, Int8Linear, quantize_frozen
 from .ia3 import IA3Module
 from .locon import LoConModule
 from .loha import LohaModule

@@ -515,9 +515,15 @@ class LycorisBaseModule(nn.Module, metaclass=_TwinMeta):
         p = next(self.parameters())
         return p.device, p.dtype
 
+    def _require_writable_weight(self, what):
+        if isinstance(getattr(type(self.org_module[0]), "weight", None), property):  # Int8Linear: `weight` is an expansion, not storage
+            raise _unsupported(f"{what} into a {type(self.org_module[0]).__name__} ({self.lora_name}): its 8-bit weight cannot take the sum; "
+                               "merge into the unquantised layer, then quantise")
+
     def merge_to(self, multiplier=1.0):
         if self.not_supported:
             return
+        self._require_writable_weight("merge_to")
         if self._native_ws() and not getattr(self, "wd", False) and self.org_weight.is_contiguous():
             from .. import ops
             with torch.no_grad():  # W += dW * mult in place, dW tiles rebuilt on chip (no [O, I] temporary)
@@ -539,6 +545,7 @@ class LycorisBaseModule(nn.Module, metaclass=_TwinMeta):
     def onfly_merge(self, multiplier=1.0):
         if self.not_supported:
             return
+        self._require_writable_weight("onfly_merge")
         dev, dt = self._own_device_dtype()
         self.to(self.org_weight)
         layer = self.org_module[0]
@@ -570,6 +577,13 @@ class LycorisBaseModule(nn.Module, metaclass=_TwinMeta):
     # ---- hot path (implemented by the algorithms) -------------------------------------------------------------
     def bypass_forward_diff(self, x, scale=1):
         raise NotImplementedError
+
+    def additive(self):
+        """is forward(x) exactly org_forward(x) + bypass_forward_diff(x, multiplier) now, on an nn.Linear?  (what a caller may rely on that
+        forms the sum itself: modules/frozen.py GatedLinear)"""
+        return (self.module_type == "linear" and not self.not_supported and self._ws_algo is not None
+                and not (getattr(self, "wd", False) and not self.bypass_mode)
+                and not (self.training and (self.module_dropout or self.rank_dropout or (self.bypass_mode and self.dropout))))
 
     def bypass_forward(self, x, scale=1):
         return self.org_forward(x) + self.bypass_forward_diff(x, scale=scale)

@@ -876,6 +876,74 @@ def chan_affine(a, w, bias=None, s0=0.0, mult=1.0, chan_dim=-1):
     return _ChanAffine.apply(_amp(a), w, bias, s0, mult, chan_dim)
 
 
+# ---------------------------------------------------------------------------------------------------------------
+# frozen layers held in 8 bits, and the gated projection of a feed-forward block (csrc/frozen.hip, csrc/frozen_ops.cpp)
+# ---------------------------------------------------------------------------------------------------------------
+_FROZEN_OPS = {}
+ACTIVATIONS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}  # LYC_ACT_*
+
+
+def _frozen_op(name):
+    """the C++ op, whatever ops.set_dispatch() says: these operators have no Python statement"""
+    if name not in _FROZEN_OPS:
+        N.load_torch_ops()
+        _FROZEN_OPS[name] = getattr(torch.ops.lycoris_amd, name).default
+    return _FROZEN_OPS[name]
+
+
+def int8_quantize(x):
+    """x [..., K] -> (q int8 [..., K], scale fp32 [...]): rows to 8-bit integers, scale = max|x| / 127 of the row, q = 127 x / max|x| rounded
+    half to even (exactly: no element is off by a step).  Rows of activations are tokens, rows of a weight [N, K] its output channels.
+
+    q lies in rows of a 128-byte pitch, as int8_linear / int8_matmul read it without a copy.  A row of zeros has scale 0; a row that holds
+    an infinity or a NaN has scale NaN (and q = 0), so that its products are NaN.  Not differentiable: the result carries no gradient."""
+    x = x.detach()
+    return _host.int8_quantize(x) if not x.is_cuda else _frozen_op("int8_quantize")(x)
+
+
+def int8_matmul(aq, a_scale, bq, b_scale, bias=None, dtype=torch.bfloat16):
+    """(a_scale[m] b_scale[n]) sum_k aq[m, k] bq[n, k] + bias[n] in `dtype`: the product of two quantised row matrices, aq [..., K] and
+    bq [N, K] (int8_quantize), int32 sums.  For projections that share one quantised input; not differentiable (int8_linear is)."""
+    if not aq.is_cuda:
+        return _host.int8_matmul(aq, a_scale, bq, b_scale, bias, dtype)
+    return _frozen_op("int8_matmul")(aq, a_scale.detach(), bq, b_scale.detach(), None if bias is None else bias.detach(), dtype)
+
+
+def int8_linear(x, wq, w_scale, bias=None, base=None):
+    """A frozen nn.Linear held in 8 bits: x [..., K] is quantised row by row, multiplied with wq [N, K] (int8) and scaled by both scales,
+    plus bias [N] and `base` [..., N] (an adapter's output, same dtype as x), in one epilogue.
+
+    Differentiable in x and base.  The gradient is not quantised: dx = g (w_scale wq), the derivative of the layer with its weight as it is
+    held, with the rounding of x passed straight through.  The weight, its scale and the bias are frozen (a bias or scale that requires a
+    gradient is refused).  K is limited to 2^17."""
+    x = _amp(x)
+    if base is not None and base.dtype != x.dtype:
+        base = base.to(x.dtype)
+    if not x.is_cuda:
+        return _host.int8_linear(x, wq, w_scale, bias, base)
+    return _frozen_op("int8_linear")(x, wq, w_scale, bias, base)
+
+
+def gated_linear(x, weight, bias=None, base=None, act="gelu", gate_first=False, weight_scale=None):
+    """value * act(gate) of the two halves of p = x weight^T + bias + base, in one kernel: x [..., I], weight [2 F, I], bias [2 F],
+    base [..., 2 F] (the output of an adapter on this projection) -> [..., F].  act: "gelu" (erf), "gelu_tanh" or "silu"; the value half
+    comes first (diffusion feed-forwards) unless `gate_first` (stacked gate / up projections).
+
+    weight in x's dtype, trainable or frozen, or int8 with `weight_scale` [2 F] (int8_quantize of its rows): x is then quantised row by row
+    as in int8_linear.  Differentiable in x, base, bias and an unquantised weight; the backward pass reads p, kept rounded to x's dtype, and
+    an 8-bit weight's gradient dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products (24 bits)."""
+    if act not in ACTIVATIONS:
+        raise ValueError(f"gated_linear: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    x = _amp(x)
+    if weight_scale is None and weight.dtype != x.dtype and weight.is_floating_point() and torch.is_autocast_enabled(x.device.type):
+        weight = weight.to(x.dtype)
+    if base is not None and base.dtype != x.dtype:
+        base = base.to(x.dtype)
+    if not x.is_cuda:
+        return _host.gated_linear(x, weight, bias, base, act, gate_first, weight_scale)
+    return _frozen_op("gated_linear")(x, weight, weight_scale, bias, base, ACTIVATIONS[act], bool(gate_first))
+
+
 _ROWS_ALGO = {"_LokrCore": 0, "_LoconCore": 1, "_LohaCore": 2}  # csrc/torch_ops.cpp ALGO_*
 
 
