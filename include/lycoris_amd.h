@@ -485,7 +485,8 @@ int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const floa
 /* ---- gated projection of a feed-forward block ------------------------------------------------------------
  *   p = x w^T + bias + base  [M, 2 F];   h = value * act(gate)  [M, F]
  * value and gate are the halves of p's columns (value first, or gate first with gate_first).  w [2 F, I] in `dtype`, contiguous, or 8-bit
- * rows of pitch ldw with scales sw (then x is quantised as above).  `pre` (training): receives p rounded to `dtype`, which bwd reads.
+ * rows of pitch ldw with scales sw (then x is quantised as above).  `pre` (training, 16-byte aligned): receives p for
+ * bwd: fp32 in 32 bits; else 24 bits of each value, 3 * M * 2 F bytes.
  * bwd, each output optional: dbase = dp [M, 2 F], dx = dp w, dw = dp^T x (not with an 8-bit weight), dbias = sum_m dp.          */
 enum { LYC_ACT_GELU = 0, LYC_ACT_GELU_TANH = 1, LYC_ACT_SILU = 2 };
 enum { LYC_GATED_INT8 = 1, LYC_GATED_BACKWARD = 2, LYC_GATED_DBASE = 4, LYC_GATED_DX = 8, LYC_GATED_DW = 16, LYC_GATED_DBIAS = 32 };

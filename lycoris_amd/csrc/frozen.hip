@@ -5,7 +5,7 @@
 
 #include "../../include/lycoris_amd.h"
 #include "errors.h"
-#include "frozen_rows.h"
+#include "frozen_skinny.h"
 
 using namespace lyc;
 
@@ -68,17 +68,90 @@ int allow_lds(Kern kern, int bytes) {
 }
 
 template <typename K, int BM, int BNO>
-int launch_tile(const FzProb& p, const FzEpi& ep, int64_t NO, hipStream_t st) {
-  const G16DMap mp = gemm16d_map((int)cdiv(p.M, BM), (int)cdiv(NO, BNO), p.M, p.N);
+int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
+  const G16DMap mp = gemm16d_map((int)cdiv(p.M, BM), (int)cdiv(K::GATED ? ep.F : p.N, BNO), p.M, p.N);
   FZ_TRY(allow_lds(&fz_gemm_kernel<K>, K::LDS));
   hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * mp.tm_per * mp.tn_per)), dim3(K::NW * 64), K::LDS, st, p, ep);
   return check_launch("fz_gemm");
 }
+
+// Which tiles for a product of M x NO outputs and `steps` 64-byte steps of K: 256 x 256 (one workgroup a CU), 128 x 128 (two) or 64 x 64
+// (three) -- and, where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those tiles over the rows that fill whole
+// rounds and 128 x 128 ones over the rest.  The rule compares estimates in microseconds: a round costs what a step costs times the steps,
+// plus what a tile's beginning and end leave exposed.
+struct TileCost {
+  double step, tile;
+};
+constexpr TileCost T256{0.66, 6.0}, T128_2{0.44, 3.0}, T128_1{0.28, 4.0}, T64_3{0.36, 2.5}, T64_2{0.26, 2.5}, T64_1{0.18, 3.0};
+double round_cost(TileCost c, double steps) { return c.step * steps + c.tile; }
+double cost256(int64_t tiles, double steps) { return (double)cdiv(tiles, 256) * round_cost(T256, steps); }
+double cost128(int64_t tiles, double steps) {
+  const int64_t r = tiles % 512;
+  return (double)(tiles / 512) * round_cost(T128_2, steps) + (r == 0 ? 0.0 : round_cost(r <= 256 ? T128_1 : T128_2, steps));
+}
+double cost64(int64_t tiles, double steps) {
+  const int64_t r = tiles % 768;
+  return (double)(tiles / 768) * round_cost(T64_3, steps) + (r == 0 ? 0.0 : round_cost(r <= 256 ? T64_1 : r <= 512 ? T64_2 : T64_3, steps));
+}
+
 template <typename E, typename TO, bool A_KS, bool B_KS, int EPI>
 int launch_gemm(const FzProb& p, const FzEpi& ep, hipStream_t st) {
   constexpr bool G = EPI == FZ_GATED;
-  return launch_tile<FzKernel<E, TO, 128, 128, 2, 2, 2, A_KS, B_KS, EPI>, 128, G ? 64 : 128>(p, ep, G ? ep.F : p.N, st);
+  constexpr int O = G ? 2 : 1;  // B rows an output column takes
+  using K256 = FzKernel<E, TO, 256, 256, 2, 4, 5, A_KS, B_KS, EPI>;
+  using K128 = FzKernel<E, TO, 128, 128, 4, 2, 5, A_KS, B_KS, EPI>;
+  using K64 = FzKernel<E, TO, 64, 64 * O, 2, 2, 6, A_KS, B_KS, EPI>;
+  const int64_t M = p.M, NO = G ? ep.F : p.N;
+  const double steps = (double)cdiv((int64_t)p.K * FE<E>::SIZE, 64) * p.nseg;
+  const int64_t tn256 = cdiv(NO, 256 / O), tn128 = cdiv(NO, 128 / O);
+  const int64_t tm256 = cdiv(M, 256), whole = tm256 * tn256 / 256 * 256 / tn256;  // row tiles that fill whole rounds
+  const double c256 = cost256(tm256 * tn256, steps), c128 = cost128(cdiv(M, 128) * tn128, steps);
+  const double c64 = cost64(cdiv(M, 64) * cdiv(NO, 64), steps * (G ? 1.4 : 1.0));
+  const double mixed = whole > 0 && whole < tm256 ? cost256(whole * tn256, steps) + cost128(cdiv(M - whole * 256, 128) * tn128, steps) + 2.0 : 1e30;
+  if (mixed < c256 && mixed < c128 && mixed < c64) {
+    const int64_t m = whole * 256;
+    FzProb a = p, b = p;
+    a.M = (int)m;
+    b.M = (int)(M - m);
+    b.A = static_cast<const char*>(p.A) + (A_KS ? 2 * m : m * p.lda);
+    FzEpi e = ep;
+    e.out = static_cast<TO*>(ep.out) + m * NO;
+    if (ep.sa) e.sa = ep.sa + m;
+    if (ep.base) e.base = static_cast<const TO*>(ep.base) + m * NO * O;
+    // (p's planes are addressed by row: the 16-bit one and, behind all of it, the 8-bit one)
+    FzEpi f = ep;
+    FZ_TRY((launch_tile<K256, 256, 256 / O>(a, f, st)));
+    e.pre_row = ep.pre_row + m;
+    return launch_tile<K128, 128, 128 / O>(b, e, st);
+  }
+  if (c64 < c128 && c64 < c256) return launch_tile<K64, 64, 64>(p, ep, st);
+  if (c128 <= c256) return launch_tile<K128, 128, 128 / O>(p, ep, st);
+  return launch_tile<K256, 256, 256 / O>(p, ep, st);
 }
+
+// up to 32 rows: frozen_skinny.h.  x: the activations when the kernel quantises them itself, else null
+template <typename E, typename TI, typename TO, int MT, bool GATED, bool FUSED>
+int launch_skinny2(const TI* x, const FzProb& p, const FzEpi& ep, hipStream_t st) {
+  const int64_t NO = GATED ? ep.F : p.N;
+  auto go = [&](auto wc) {
+    constexpr int W = decltype(wc)::value;
+    const int red = (GATED ? 2 : 1) * MT * W * 16 * 20 * 4, rows = FUSED ? p.M * sk_pitch(p.K) : 0;
+    const int lds = red > rows ? red : rows;
+    FZ_TRY(allow_lds(&fz_skinny_kernel<E, TI, TO, MT, W, GATED, FUSED>, 96 * 1024));
+    hipLaunchKernelGGL((fz_skinny_kernel<E, TI, TO, MT, W, GATED, FUSED>), dim3((unsigned)cdiv(NO, 16)), dim3(W * 64), lds, st, x, p, ep);
+    return check_launch("fz_skinny");
+  };
+  // 8 waves share K; 16 where K is long and the columns alone do not fill the CUs twice
+  if (p.kb >= 4096 && NO <= 16 * 512) return go(std::integral_constant<int, 16>{});
+  return go(std::integral_constant<int, 8>{});
+}
+template <typename E, typename TI, typename TO, bool GATED, bool FUSED>
+int launch_skinny(const TI* x, const FzProb& p, const FzEpi& ep, hipStream_t st) {
+  if (p.M <= 16) return launch_skinny2<E, TI, TO, 1, GATED, FUSED>(x, p, ep, st);
+  return launch_skinny2<E, TI, TO, 2, GATED, FUSED>(x, p, ep, st);
+}
+constexpr int64_t SKINNY_ROWS = 32;
+inline bool skinny_fused(int64_t M, int64_t K) { return M <= SKINNY_ROWS && M * K <= SK_FUSED_ELEMS; }
 
 template <typename T>
 int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int K, hipStream_t st) {
@@ -109,10 +182,19 @@ int launch_stage(const TI* x, const float* col, TO* out, int64_t rows, int64_t c
   return check_launch("stage");
 }
 template <typename T>
-int launch_plane(const int8_t* q, int64_t ldq, const float* sw, T* out, float* alpha, int64_t O, int64_t I, int scaled, hipStream_t st) {
-  const int rows = std::is_same<T, _Float16>::value ? 16 : 4;  // fp16: every workgroup reads all scales first
-  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, sw, out, up(I, 8), alpha, (int)O, (int)I, rows, scaled);
+int launch_plane(const int8_t* q, int64_t ldq, const float* sw, const float* f, T* out, int64_t O, int64_t I, hipStream_t st) {
+  const int rows = 4;
+  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, sw, f, out, up(I, 8), (int)O, (int)I, rows);
   return check_launch("weight plane");
+}
+// fp16: f[0], f[1] (fz_range_kernel); other types need none
+template <typename E>
+int launch_range(const float* sw, int64_t n, int top, float* f, const float** out, hipStream_t st) {
+  *out = nullptr;
+  if (!std::is_same<E, _Float16>::value) return LYC_OK;
+  hipLaunchKernelGGL(fz_range_kernel, dim3(1), dim3(256), 0, st, sw, (int)n, top, f);
+  *out = f;
+  return check_launch("scale range");
 }
 
 // One operand of a product in the type the matrix cores take: the tensor itself, its staged copy, or its three bf16 planes.
@@ -160,6 +242,9 @@ int matmul8(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, in
   FzProb p = prob(aq, lda, 0, bq, ldb, 0, M, N, K, 1);
   FzEpi ep{};
   ep.out = y; ep.sa = sa; ep.sw = sb; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base;
+  if (M <= SKINNY_ROWS) {
+    FZ_DTYPE(dtype, return (launch_skinny<int8_t, T, T, false, false>(nullptr, p, ep, st)));
+  }
   FZ_DTYPE(dtype, return (launch_gemm<int8_t, T, false, false, FZ_LINEAR>(p, ep, st)));
   return LYC_OK;
 }
@@ -170,25 +255,28 @@ int check_q(const char* who, const char* what, const void* q, int64_t ld, int64_
   return LYC_OK;
 }
 
-// ---- dx of a frozen 8-bit layer: g [M, N] times (sw wq) [N, K] -------------------------------------------------------------------------
+// ---- dx of a frozen 8-bit layer: g [M, N] times (sw wq) [N, K].  16 bits: g as it is, times the plane of sw wq (one rounding each entry);
+//      32 bits: g sw in three planes times the integers, which are exact in bf16 ----------------------------------------------------------
 template <typename T>
 int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve ws, int64_t* bytes, int64_t M, int64_t N, int64_t K, hipStream_t st) {
   using E = typename Operand<T>::E;
+  constexpr bool F32 = sizeof(T) == 4;
   E* plane = ws.take<E>(N * up(K, 8));
-  float* alpha = ws.take<float>(1);
+  float* f = ws.take<float>(2);
   Operand<T> a(ws, M, N, true);
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
   }
-  constexpr bool F32 = sizeof(T) == 4;
-  FZ_TRY(launch_plane<E>(wq, ldw, sw, plane, alpha, N, K, !F32, st));
+  const float* range;
+  FZ_TRY(launch_range<E>(sw, N, 14, f, &range, st));
+  FZ_TRY(launch_plane<E>(wq, ldw, F32 ? nullptr : sw, range, plane, N, K, st));
   FZ_TRY(a.fill(g, F32 ? sw : nullptr, st));
   FzProb p = prob(a.p, a.ld, a.plane, plane, up(K, 8) * 2, 0, M, K, N, 2);
   segments(p, F32 ? 3 : 1);
   FzEpi ep{};
   ep.out = dx;
-  ep.alpha = std::is_same<T, _Float16>::value ? alpha : nullptr;
+  ep.alpha = range ? range + 1 : nullptr;
   return launch_gemm<E, T, false, true, FZ_PLAIN>(p, ep, st);
 }
 
@@ -202,10 +290,11 @@ struct Gated {
 };
 
 template <typename T>
-int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const T* base, T* h, T* pre, Carve ws, int64_t* bytes, hipStream_t st) {
+int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const T* base, T* h, void* pre, Carve ws, int64_t* bytes, hipStream_t st) {
   using E = typename Operand<T>::E;
   FzEpi ep{};
   ep.out = h; ep.pre = pre; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base; ep.sw = q.sw; ep.act = q.act; ep.gate_first = q.gate_first; ep.F = (int)q.F;
+  ep.pre_total = 2 * q.M * q.F;
   if (q.sw) {
     const int64_t ldq = up(q.I, 16);
     int8_t* xq = ws.take<int8_t>(q.M * ldq);
@@ -214,9 +303,14 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
       *bytes = ws.used;
       return LYC_OK;
     }
+    if (skinny_fused(q.M, q.I)) {
+      FzProb p = prob(nullptr, 0, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
+      return launch_skinny<int8_t, T, T, true, true>(x, p, ep, st);
+    }
     FZ_TRY(launch_quant<T>(x, q.I, xq, ldq, sa, q.M, (int)q.I, st));
     ep.sa = sa;
     FzProb p = prob(xq, ldq, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
+    if (q.M <= SKINNY_ROWS) return launch_skinny<int8_t, T, T, true, false>(nullptr, p, ep, st);
     return launch_gemm<int8_t, T, false, false, FZ_GATED>(p, ep, st);
   }
   Operand<T> a(ws, q.M, q.I, true), b(ws, 2 * q.F, q.I, true);
@@ -228,38 +322,48 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
   FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
   FzProb p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, 2 * q.F, q.I, 2);
   segments(p, sizeof(T) == 4 ? 6 : 1);
+  if constexpr (sizeof(T) == 2) {
+    if (q.M <= SKINNY_ROWS) return launch_skinny<E, T, T, true, false>(nullptr, p, ep, st);
+  }
   return launch_gemm<E, T, false, false, FZ_GATED>(p, ep, st);
 }
 
+// dp is written once, by one elementwise pass.  dx over an 8-bit weight takes dp sw (16 bits: rounded once, from fp32; 32 bits: staged in
+// three planes) times the weight's integers, which 16 bits hold exactly; over a 16 / 32-bit weight it takes dp and the weight.
 template <typename T>
-int gated_bwd(const Gated& q, const T* g, const T* pre, const T* x, T* dp, T* dx, T* dw, T* dbias, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
+int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T* dx, T* dw, T* dbias, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
   using E = typename Operand<T>::E;
   constexpr bool F32 = sizeof(T) == 4;
-  const bool held = flags & LYC_GATED_INT8;
-  const int64_t N = 2 * q.F, parts = cdiv(q.M, FZ_SUM_ROWS);
-  if (!(flags & LYC_GATED_DBASE)) dp = ws.take<T>(q.M * N);
-  const bool want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
-  Operand<T> a(ws, q.M, N, want_dx || want_dw);  // dp as the products' operand (K-contiguous for dx, K-strided for dw)
+  const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
+  const int64_t N = 2 * q.F, parts = cdiv(q.M, DG_ROWS);
+  const bool scaled = held && want_dx && !F32;  // dps
+  if (!(flags & LYC_GATED_DBASE)) dp = want_dw || (want_dx && !scaled) ? ws.take<T>(q.M * N) : nullptr;
+  E* dps = scaled ? ws.take<E>(q.M * up(N, 8)) : nullptr;
+  Operand<T> a(ws, q.M, N, want_dw || (want_dx && !scaled));  // dp as the products' operand (K-contiguous for dx, K-strided for dw)
   Operand<T> b(ws, N, q.I, want_dx && !held), xo(ws, q.M, q.I, want_dw);
   E* plane = want_dx && held ? ws.take<E>(N * up(q.I, 8)) : nullptr;
-  float* alpha = ws.take<float>(1);
+  float* f = ws.take<float>(2);
   float* part = flags & LYC_GATED_DBIAS ? ws.take<float>(parts * N) : nullptr;
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
   }
+  const float* range = nullptr;
+  if (scaled) FZ_TRY(launch_range<E>(q.sw, N, 7, f, &range, st));  // the largest sw f[0] near 1
   const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp);
-  hipLaunchKernelGGL((fz_dgate_kernel<T>), dim3(grid_of(q.M * cdiv(q.F, 8))), dim3(256), 0, st, g, pre, dp, q.M, (int)q.F, q.act, q.gate_first, vec);
+  hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)cdiv(q.F, DG_COLS), (unsigned)parts), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
+                     (int)q.F, q.act, q.gate_first, vec);
   FZ_TRY(check_launch("gated backward"));
-  if (want_dx || want_dw) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));
+  if (want_dw || (want_dx && !scaled)) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));
   if (want_dx) {
     FzEpi ep{};
     ep.out = dx;
     FzProb p;
     if (held) {
-      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, q.sw, plane, alpha, N, q.I, !F32, st));
-      p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
-      ep.alpha = std::is_same<T, _Float16>::value ? alpha : nullptr;
+      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, nullptr, nullptr, plane, N, q.I, st));
+      if (scaled) p = prob(dps, up(N, 8) * 2, 0, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
+      else p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
+      ep.alpha = range ? range + 1 : nullptr;
     } else {
       FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
       p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, q.I, N, 2);
@@ -276,8 +380,7 @@ int gated_bwd(const Gated& q, const T* g, const T* pre, const T* x, T* dp, T* dx
     FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(p, ep, st)));
   }
   if (part) {
-    hipLaunchKernelGGL((fz_colsum_kernel<T>), dim3((unsigned)cdiv(N, 256), (unsigned)parts), dim3(256), 0, st, dp, part, q.M, (int)N);
-    hipLaunchKernelGGL((fz_colsum_join_kernel<T>), dim3((unsigned)cdiv(N, 256)), dim3(256), 0, st, part, dbias, (int)parts, (int)N);
+    hipLaunchKernelGGL((fz_join_kernel<T>), dim3((unsigned)cdiv(N, 32)), dim3(256), 0, st, part, dbias, parts, (int)N);
     FZ_TRY(check_launch("column sums"));
   }
   return LYC_OK;
@@ -287,7 +390,7 @@ int check_gated(const char* who, const Gated& q, bool held, int dtype) {
   if (q.F > (1 << 19)) return fail(LYC_ERR_UNSUPPORTED, "%s: F=%ld exceeds 2^19", who, (long)q.F);
   FZ_TRY(check_dims(who, q.M, q.F < 1 ? 0 : 2 * q.F, q.I, dtype));
   if (q.act < 0 || q.act > 2) return fail(LYC_ERR_ARG, "%s: unknown activation %d", who, q.act);
-  if ((q.F + 512) * (held ? q.ldw : up(q.I, 8) * 2) >= ((int64_t)1 << 31)) return fail(LYC_ERR_UNSUPPORTED, "%s: half a weight of 2 GiB or more", who);
+  if ((q.F + 512) * (held ? q.ldw : up(q.I, 8) * 2) >= ((int64_t)1 << 30)) return fail(LYC_ERR_UNSUPPORTED, "%s: half a weight of 1 GiB or more", who);
   return LYC_OK;
 }
 
@@ -341,6 +444,12 @@ int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const floa
   int8_t* xq = c.take<int8_t>(M * ldq);
   float* sa = c.take<float>(M);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (skinny_fused(M, K)) {
+    FzProb p = prob(nullptr, 0, 0, wq, ldw, 0, M, N, K, 1);
+    FzEpi ep{};
+    ep.out = y; ep.sw = sw; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base;
+    FZ_DTYPE(dtype, return (launch_skinny<int8_t, T, T, false, true>(static_cast<const T*>(x), p, ep, st)));
+  }
   FZ_DTYPE(dtype, FZ_TRY(launch_quant<T>(static_cast<const T*>(x), K, xq, ldq, sa, M, (int)K, st)));
   return matmul8(xq, ldq, sa, wq, ldw, sw, bias, bias_f32, base, y, M, N, K, dtype, st);
 }
@@ -385,7 +494,7 @@ int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float*
   FZ_TRY(need16(who, "workspace", ws, lyc_gated_linear_workspace_bytes(M, I, F, dtype, sw ? LYC_GATED_INT8 : 0) == 0));
   if (sw) FZ_TRY(check_q(who, "w", w, ldw, I));
   else FZ_TRY(need16(who, "w", w));
-  FZ_DTYPE(dtype, return gated_fwd<T>(q, static_cast<const T*>(x), bias, bias_f32, static_cast<const T*>(base), static_cast<T*>(h), static_cast<T*>(pre),
+  FZ_DTYPE(dtype, return gated_fwd<T>(q, static_cast<const T*>(x), bias, bias_f32, static_cast<const T*>(base), static_cast<T*>(h), pre,
                                       Carve{static_cast<char*>(ws)}, nullptr, static_cast<hipStream_t>(stream)));
   return LYC_OK;
 }
@@ -405,7 +514,7 @@ int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const vo
   FZ_TRY(need16(who, "workspace", ws));
   const int flags = LYC_GATED_BACKWARD | (sw ? LYC_GATED_INT8 : 0) | (dbase ? LYC_GATED_DBASE : 0) | (dx ? LYC_GATED_DX : 0) | (dw ? LYC_GATED_DW : 0) |
                     (dbias ? LYC_GATED_DBIAS : 0);
-  FZ_DTYPE(dtype, return gated_bwd<T>(q, static_cast<const T*>(g), static_cast<const T*>(pre), static_cast<const T*>(x), static_cast<T*>(dbase),
+  FZ_DTYPE(dtype, return gated_bwd<T>(q, static_cast<const T*>(g), pre, static_cast<const T*>(x), static_cast<T*>(dbase),
                                       static_cast<T*>(dx), static_cast<T*>(dw), static_cast<T*>(dbias), flags, Carve{static_cast<char*>(ws)}, nullptr,
                                       static_cast<hipStream_t>(stream)));
   return LYC_OK;

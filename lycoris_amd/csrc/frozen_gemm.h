@@ -5,15 +5,20 @@
 //     dx              dx[m, i]  = sum_o dp[m, o] w[o, i]           A K-contiguous, B K-strided
 //     dw              dw[o, i]  = sum_m dp[m, o] x[m, i]           both K-strided
 //
-// The skeleton is gemm16d.h's: both operands go HBM -> LDS by LDS-DMA into a ring of K steps of 128 BYTES, fragments are read one K half
-// ahead of the MFMAs that use them, the MFMA roles are swapped and the n tiles formed in pairs so that a lane owns 8 consecutive output
-// columns of one row.  Since every address is formed in bytes, 8-bit operands (128 k per step, v_mfma_i32_16x16x64_i8) and 16-bit ones
-// (64 k, v_mfma_f32_16x16x32) run the same loop: a fragment is 16 bytes of one row either way, and the matrix pipe takes the same
-// 16 cycles for it.  What differs from gemm16d.h:
+// The skeleton is gemm16d.h's: both operands go HBM -> LDS by LDS-DMA into a ring of K steps, fragments are read one step ahead of the
+// MFMAs that use them, the MFMA roles are swapped and the n tiles formed in pairs so that a lane owns 8 consecutive output columns of one
+// row.  Every address is formed in bytes, so 8-bit operands (64 k per step, v_mfma_i32_16x16x64_i8) and 16-bit ones (32 k,
+// v_mfma_f32_16x16x32) run the same loop: a step is 64 bytes of K, a fragment 16 bytes of one row, an MFMA 16 cycles either way.
 //
-//   * the buffer descriptor is rebased on every K step (scalar adds beside the matrix pipe) instead of walked with a 32-bit offset: an
-//     operand may be larger than 4 GiB;
-//   * a K that is not a multiple of the step is masked in the DMA of the last step, 16 bytes at a time (both operands: 0 times a stray NaN
+// What bounds the loop, measured inside it (256 x 256 tile, 8 waves, cycles per 64-byte step; the MFMAs alone are 1024): 1450 with the
+// descriptor and tail arithmetic of every step in line (~100 scalar instructions between the barrier and the first MFMA), 1250 with it
+// behind a branch that is taken at the end of a segment only, 1205 - 1250 with one barrier per two steps.  The clock then is 1.75 - 1.95
+// GHz: the matrix pipe is near what the card's power allows (1.68 PFLOP/s bf16, 2.7 POP/s int8 inside the loop).  Ring depth beyond what
+// the waits need, LDS bank conflicts (SQ_LDS_BANK_CONFLICT) and L2 order were not what bounded it at 4096 rows; at 8192^3 the order was
+// (tiles in flight on an XCD as a block: 988 -> 872 us).
+//
+//   * the buffer descriptor is rebased on every K step: an operand may be larger than 4 GiB;
+//   * rows, columns and K outside the operand are masked in the DMA's lane offsets, 16 bytes at a time (both operands: 0 times a stray NaN
 //     would not be 0);
 //   * a product may be a sum of SEGMENTS over pairs of operand planes: 32-bit operands are held as three bf16 planes each
 //     (x = h + m + l, 24 bits) and multiplied as hh + hm + mh + hl + lh + mm; what is left out is below 2^-24 of a term;
@@ -49,27 +54,50 @@ struct FE<int8_t> {
 
 enum { FZ_ACT_GELU = 0, FZ_ACT_GELU_TANH = 1, FZ_ACT_SILU = 2 };
 
+// Phi(t) = erfc(-t / sqrt 2) / 2 with erfc(z) = w P(w) exp(-z^2), w = 1 / (1 + 0.45 z): P is the degree-7 polynomial of least largest
+// relative error on z = 0 .. 14 (3.5e-7, fitted to erfc in 64 bits); in fp32 Phi is off by 1.2e-6 of itself down to t = -6, where the
+// rounding of t^2 takes over.  About 20 operations, where the library's erfc takes three times that and a branch.
+__device__ __forceinline__ void fz_phi(float t, float& phi, float& e) {
+  const float z = 0.70710678f * fabsf(t);
+  const float w = __builtin_amdgcn_rcpf(fmaf(0.45f, z, 1.f));
+  float q = 0.0689046234f;
+  q = fmaf(q, w, -0.248889327f);
+  q = fmaf(q, w, 0.223910257f);
+  q = fmaf(q, w, 0.026233878f);
+  q = fmaf(q, w, 0.196168676f);
+  q = fmaf(q, w, 0.225782961f);
+  q = fmaf(q, w, 0.254004091f);
+  q = fmaf(q, w, 0.25388521f);
+  e = __builtin_amdgcn_exp2f(-0.72134752f * t * t);  // exp(-t^2 / 2)
+  const float h = 0.5f * q * w * e;
+  phi = t >= 0.f ? 1.f - h : h;
+}
+__device__ __forceinline__ float fz_sigmoid(float t) { return __builtin_amdgcn_rcpf(1.f + __expf(-t)); }
+
 // act(t) and its derivative in fp32
 __device__ __forceinline__ float fz_act(int act, float t) {
-  if (act == FZ_ACT_SILU) return t / (1.f + __expf(-t));
-  if (act == FZ_ACT_GELU) return 0.5f * t * erfcf(-0.70710678118654752f * t);
-  const float u = 0.79788456080286536f * (t + 0.044715f * t * t * t);
-  return t / (1.f + __expf(-2.f * u));  // 0.5 t (1 + tanh u)
+  if (act == FZ_ACT_SILU) return t * fz_sigmoid(t);
+  if (act == FZ_ACT_GELU) {
+    float phi, e;
+    fz_phi(t, phi, e);
+    return t * phi;
+  }
+  return t * fz_sigmoid(1.5957691216057308f * (t + 0.044715f * t * t * t));  // 0.5 t (1 + tanh u) = t sigmoid(2 u)
 }
 __device__ __forceinline__ void fz_act_grad(int act, float t, float& a, float& da) {
   if (act == FZ_ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-t));
+    const float s = fz_sigmoid(t);
     a = t * s;
     da = s + a * (1.f - s);
   } else if (act == FZ_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * t);
-    a = t * cdf;
-    da = cdf + t * 0.39894228040143268f * __expf(-0.5f * t * t);
+    float phi, e;
+    fz_phi(t, phi, e);
+    a = t * phi;
+    da = phi + t * 0.39894228040143268f * e;
   } else {
-    const float u = 0.79788456080286536f * (t + 0.044715f * t * t * t);
-    const float s = 1.f / (1.f + __expf(-2.f * u));
+    const float s = fz_sigmoid(1.5957691216057308f * (t + 0.044715f * t * t * t));
     a = t * s;
-    da = s + 2.f * a * (1.f - s) * 0.79788456080286536f * (1.f + 0.134145f * t * t);
+    da = s + a * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * t * t);
   }
 }
 
@@ -86,61 +114,72 @@ struct FzProb {
 enum { FZ_PLAIN = 0, FZ_LINEAR = 1, FZ_GATED = 2 };
 struct FzEpi {
   void* out;           // [M, N] (GATED: [M, F]), row pitch = N (F) elements
-  void* pre;           // GATED: p [M, 2 F] or null
+  void* pre;           // GATED: p [M, 2 F] for the backward pass (fz_store_pre8) or null
   const float* alpha;  // PLAIN: device scalar on the result, or null
   const float *sa, *sw;  // 8-bit: scales of A's rows, of B's rows
   const void* bias;    // [N] (GATED: [2 F]) or null; fp32 when bias_f32, else the output's type
   const void* base;    // [M, N] (GATED: [M, 2 F]) in the output's type, or null
+  int64_t pre_total, pre_row;  // elements of the whole p; its row that this launch's first row is
   int bias_f32, act, gate_first, F;
 };
 
-// One operand of one workgroup tile; gemm16d.h's G16DOperand with the tile split over W waves along this extent, NW in all.
+// One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A K step is 64 bytes of K: one MFMA deep.
+//   ROWS: tile extent; W: waves along it; NW: waves in all; KS: K-strided in memory; PAIRED: the n operand (paired tile order)
+// K-contiguous: LDS rows of 64 bytes, their four 16-byte chunks XOR-permuted on the DMA's source address -- by bits 2, 3 of the row in
+// natural order, 3, 4 in paired order -- so that the 16 rows of a fragment read fall on the 16 slots of a 256-byte bank row.
+// K-strided (16-bit): the image in memory order, read transposed (gemm16d.h).
 template <int ROWS, int W, int NW, bool KS, bool PAIRED, bool GATED>
 struct FzOperand {
-  static constexpr int PIECES = ROWS / 8, PPW = PIECES / NW;
+  static constexpr int PIECES = ROWS / 16, PPW = PIECES / NW;  // 1 KiB DMA pieces of a K step
   static constexpr int WEXT = ROWS / W, NT = WEXT / 16;
-  static constexpr int CH = ROWS / 8, PITCH = ROWS * 2;  // KS (16-bit): chunks and bytes per k row
-  static constexpr int NADDR = KS ? (PAIRED ? NT / 2 : NT) : 2;
+  static constexpr int CH = ROWS / 8, PITCH = ROWS * 2;  // KS: chunks and bytes per k row
+  static constexpr int NADDR = KS ? (PAIRED ? NT / 2 : NT) : 1;
+  static constexpr int SLOT = ROWS * 64;
   static_assert(PIECES % NW == 0 && (!PAIRED || NT % 2 == 0) && (!GATED || (PAIRED && !KS && NT % 4 == 0)), "tile shape");
 
+  static constexpr unsigned BAD = 0xc0000000u;  // a lane whose row or column lies outside the operand; bit 31 alone: outside this step
   unsigned voff[PPW], rd[NADDR];
-  bool tail;             // K-contiguous: this lane's chunk lies beyond K in the last step of a segment
   const char *org, *cur;  // the tile's first byte in plane 0; the next K step's
-  int64_t total, left;   // bytes behind them
-  unsigned kstep;
+  unsigned kstep, kleft;  // bytes a step advances; K-contiguous: bytes, K-strided: rows, of the last step of a segment
   __amdgpu_buffer_rsrc_t rs;
 
+  static __device__ __forceinline__ int swz(int r) {
+    const int j = (r >> (PAIRED ? 3 : 2)) & 3;
+    return ((j << 1) & 3) ^ ((j >> 1) * 3);  // 0 2 3 1
+  }
+  static __device__ __forceinline__ int piece_row(int j) {  // row (KC) or k row (KS) of this lane in piece j of its wave
+    const int wave = (int)(threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    if constexpr (!KS) return 16 * (wave + NW * j) + (lane >> 2);
+    else return 1024 / PITCH * (wave + NW * j) + lane / CH;
+  }
+  static __device__ __forceinline__ int piece_chunk(int j) {
+    const int lane = (int)threadIdx.x & 63;
+    if constexpr (!KS) return (lane & 3) ^ swz(piece_row(j));
+    else return (lane % CH) ^ g16d_swz_ks<PAIRED, CH>(piece_row(j));
+  }
   __device__ __forceinline__ void setup(const void* base, int64_t ld, int r0, int ext, int kdim, int kb, int stage_off, int wsel, int second) {
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if constexpr (!KS) {
-      const int64_t skip = (int64_t)r0 * ld;
-      org = static_cast<const char*>(base) + skip;
-      total = (int64_t)(ext - 1) * ld + kb - skip;
-      kstep = 128;
+      org = static_cast<const char*>(base) + (int64_t)r0 * ld;
+      kstep = 64;
+      kleft = ((kb - 1) & 63) + 1;
 #pragma unroll
       for (int j = 0; j < PPW; ++j) {
-        const int r = 8 * (wave + NW * j) + (lane >> 3), c = (lane & 7) ^ g16d_swz_kc<PAIRED>(r);
+        const int r = piece_row(j);
         // GATED: rows 0 .. BN / 2 are the half whose first row is `base`, the others the half `second` rows further on
         const int gr = !GATED || r < ROWS / 2 ? r : second + r - ROWS / 2;
-        voff[j] = (unsigned)gr * (unsigned)ld + (unsigned)c * 16u;
-        tail = ((kb - 1) & ~127) + c * 16 >= kb;  // c does not depend on j: 8 NW rows are a multiple of the swizzle's period
+        voff[j] = r0 + gr < ext ? (unsigned)gr * (unsigned)ld + (unsigned)piece_chunk(j) * 16u : BAD;
       }
       const int r = wsel * (GATED ? WEXT / 2 : WEXT) + (PAIRED ? 8 * (li >> 2) + (li & 3) : li);
-      const int x = g16d_swz_kc<PAIRED>(r);
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) rd[kk] = (unsigned)(stage_off + r * 128 + (((4 * kk + g) ^ x) << 4));
+      rd[0] = (unsigned)(stage_off + r * 64 + ((g ^ swz(r)) << 4));
     } else {
-      const int64_t skip = (int64_t)r0 * 2;
-      org = static_cast<const char*>(base) + skip;
-      total = (int64_t)(kdim - 1) * ld + (((int64_t)ext + 7) & ~7) * 2 - skip;
-      kstep = 64u * (unsigned)ld;
-      tail = false;
-      constexpr int RP = 1024 / PITCH;
+      org = static_cast<const char*>(base) + (int64_t)r0 * 2;
+      kstep = 32u * (unsigned)ld;
+      kleft = ((kdim - 1) & 31) + 1;
 #pragma unroll
       for (int j = 0; j < PPW; ++j) {
-        const int kr = RP * (wave + NW * j) + lane / CH, c = (lane % CH) ^ g16d_swz_ks<PAIRED, CH>(kr);
-        voff[j] = (r0 + 8 * c < ext) ? (unsigned)kr * (unsigned)ld + (unsigned)c * 16u : K4_OOB;
+        const int c = piece_chunk(j);
+        voff[j] = r0 + 8 * c < ext ? (unsigned)piece_row(j) * (unsigned)ld + (unsigned)c * 16u : BAD;
       }
       const int rho = li >> 2, quad = li & 3, x = g16d_swz_ks<PAIRED, CH>(rho), krow = 8 * g + rho;
 #pragma unroll
@@ -150,51 +189,50 @@ struct FzOperand {
       }
     }
   }
-  __device__ __forceinline__ void seek(int64_t plane_off) {
-    cur = org + plane_off;
-    left = total;
+  __device__ __forceinline__ void seek(int64_t plane_off) { cur = org + plane_off; }
+  // what lies beyond K in the last step of a segment reads as zero: on for that step, off again behind it
+  __device__ __forceinline__ void tail(bool on) {
+#pragma unroll
+    for (int j = 0; j < PPW; ++j) {
+      const bool out = KS ? (unsigned)piece_row(j) >= kleft : (unsigned)piece_chunk(j) * 16u >= kleft;
+      if (on) voff[j] |= out ? K4_OOB : 0u;
+      else if (voff[j] < BAD) voff[j] &= ~K4_OOB;
+    }
   }
-  // descriptor of the next K step; `dead`: nothing is left to fetch (the refills behind the last step read nothing and store zeros)
-  __device__ __forceinline__ void open(bool dead) {
-    const int64_t n = dead ? 0 : left;
-    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(cur), 0, (int)(n < 0 ? 0 : n > 0x7fffffff ? 0x7fffffff : n), K4_RSRC_FLAGS);
+  // descriptor of the next K step (rebased: an operand may exceed 4 GiB; rows, columns and K are masked above, so any size will do, and
+  // none once nothing is left to fetch: the refills behind the last step store zeros)
+  __device__ __forceinline__ void open(int records) {
+    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(cur), 0, records, K4_RSRC_FLAGS);
     cur += kstep;
-    left -= kstep;
   }
   template <int J>
-  __device__ __forceinline__ void issue_piece(char* slot, bool last) const {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const unsigned v = (!KS && last && tail) ? K4_OOB : voff[J];
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)(slot + (wave + NW * J) * 1024), 16, (int)v, 0, 0, 0);
+  __device__ __forceinline__ void issue_piece(char* slot_of_wave) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)(slot_of_wave + NW * J * 1024), 16, (int)voff[J], 0, 0, 0);
   }
   template <int... J>
-  __device__ __forceinline__ void issue(char* slot, bool last, std::integer_sequence<int, J...>) const {
-    (issue_piece<J>(slot, last), ...);
+  __device__ __forceinline__ void issue(char* slot_of_wave, std::integer_sequence<int, J...>) const {
+    (issue_piece<J>(slot_of_wave), ...);
   }
-  __device__ __forceinline__ void issue(char* slot, bool last) const { issue(slot, last, std::make_integer_sequence<int, PPW>{}); }
+  __device__ __forceinline__ void issue(char* slot_of_wave) const { issue(slot_of_wave, std::make_integer_sequence<int, PPW>{}); }
 
   static constexpr int NRAW = KS ? 2 * NT : NT;
   using RawT = typename std::conditional<KS, u32x2, u32x4>::type;
-  // LDS byte offset of tile TI behind rd[]: K-contiguous tiles of 16 rows (natural) or pairs of 32 (paired); GATED: the second half of
+  // LDS byte offset of tile TI behind rd[0]: K-contiguous tiles of 16 rows (natural) or pairs of 32 (paired); GATED: the second half of
   // the tiles lies BN / 2 rows further on
   static constexpr int kc_off(int ti) {
-    if (!PAIRED) return ti * 2048;
+    if (!PAIRED) return ti * 1024;
     const int half = GATED && ti >= NT / 2, t = half ? ti - NT / 2 : ti;
-    return half * (ROWS / 2) * 128 + (t >> 1) * 4096 + (t & 1) * 512;
+    return half * (ROWS / 2) * 64 + (t >> 1) * 2048 + (t & 1) * 256;
   }
-  template <int KK, int... TI>
-  __device__ __forceinline__ void read(unsigned sb, RawT (&f)[NRAW], std::integer_sequence<int, TI...>) const {
-    if constexpr (!KS) {
-      ((f[TI] = g16d_read128(sb + rd[KK], kc_off(TI))), ...);
-    } else {
-      ((f[2 * TI] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], KK * 32 * PITCH + (PAIRED ? (TI & 1) * 8 : 0)),
-        f[2 * TI + 1] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], KK * 32 * PITCH + (PAIRED ? (TI & 1) * 8 : 0) + 4 * PITCH)),
-       ...);
-    }
-  }
-  template <int KK>
+  // read I of the NRAW that make up the wave's fragments of the step in the slot at LDS byte address sb
+  template <int I>
   __device__ __forceinline__ void read(unsigned sb, RawT (&f)[NRAW]) const {
-    read<KK>(sb, f, std::make_integer_sequence<int, NT>{});
+    if constexpr (!KS) {
+      f[I] = g16d_read128(sb + rd[0], kc_off(I));
+    } else {
+      constexpr int TI = I / 2;
+      f[I] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], (PAIRED ? (TI & 1) * 8 : 0) + (I & 1) * 4 * PITCH);
+    }
   }
   static __device__ __forceinline__ void tie(RawT (&f)[NRAW]) {
 #pragma unroll
@@ -243,27 +281,98 @@ __device__ __forceinline__ void fz_bias8(const FzEpi& ep, int64_t at, int n, int
   if (ep.bias_f32) fz_load8<float>(ep.bias, at, n, N, vec, v);
   else fz_load8<T>(ep.bias, at, n, N, vec, v);
 }
+// p for the backward pass: fp32 as it is; 16-bit types keep 24 bits of the fp32 value (sign, exponent, 15 bits: off by 2^-17), as a plane of
+// its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p alone would cost the gradients as much as their own rounding
+// does twice over.  total: elements of p
+template <typename TO>
+__device__ __forceinline__ void fz_store_pre8(void* pre, int64_t total, int64_t at, int n, int N, bool vec, const float (&v)[8]) {
+  if constexpr (sizeof(TO) == 4) {
+    fz_store8<float>(pre, at, n, N, vec, v);
+  } else {
+    uint16_t* hi = static_cast<uint16_t*>(pre) + at;
+    uint8_t* lo = reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(pre) + total) + at;
+    unsigned u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned b = __float_as_uint(v[e]);
+      u[e] = (b & 0x7f800000u) == 0x7f800000u ? b : b + 0x80u;
+    }
+    if (vec) {
+      u32x4 h;
+      u32x2 l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = __builtin_amdgcn_perm(u[2 * e + 1], u[2 * e], 0x07060302u);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned x = __builtin_amdgcn_perm(u[4 * e + 1], u[4 * e], 0x0c0c0501u), y = __builtin_amdgcn_perm(u[4 * e + 3], u[4 * e + 2], 0x0c0c0501u);
+        l[e] = x | (y << 16);
+      }
+      *reinterpret_cast<u32x4*>(hi) = h;
+      *reinterpret_cast<u32x2*>(lo) = l;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < N) {
+          hi[e] = (uint16_t)(u[e] >> 16);
+          lo[e] = (uint8_t)(u[e] >> 8);
+        }
+    }
+  }
+}
+template <typename TO>
+__device__ __forceinline__ void fz_load_pre8(const void* pre, int64_t total, int64_t at, int n, int N, bool vec, float (&v)[8]) {
+  if constexpr (sizeof(TO) == 4) {
+    fz_load8<float>(pre, at, n, N, vec, v);
+  } else {
+    const uint16_t* hi = static_cast<const uint16_t*>(pre) + at;
+    const uint8_t* lo = reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(pre) + total) + at;
+    if (vec) {
+      const u32x4 h = *reinterpret_cast<const u32x4*>(hi);
+      const u32x2 l = *reinterpret_cast<const u32x2*>(lo);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = __uint_as_float(((h[e >> 1] >> (16 * (e & 1))) << 16) | (((l[e >> 2] >> (8 * (e & 3))) & 0xffu) << 8));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = n + e < N ? __uint_as_float(((unsigned)hi[e] << 16) | ((unsigned)lo[e] << 8)) : 0.f;
+    }
+  }
+}
 inline __host__ __device__ bool fz_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Workgroup -> tile: the 8 XCDs (workgroups round-robin) as a grid over the output as in gemm16d.h; inside an XCD's block the tiles go in
+// bands of 8 row tiles, column by column, so that the 32 or 64 in flight at a time are a block of it and share both operands in the L2.
+__device__ __forceinline__ bool fz_tile(int b, int tiles_m, int tiles_n, const G16DMap& mp, int& tm, int& tn) {
+  constexpr int BAND = 8;
+  const int xcd = b & 7, idx = b >> 3;
+  const int band = idx / (BAND * mp.tn_per), in = idx - band * BAND * mp.tn_per;
+  const int h = min(BAND, mp.tm_per - band * BAND);
+  if (h <= 0) return false;
+  const int ln = in / h, lm = band * BAND + in - ln * h;
+  tm = (xcd & ((1 << mp.lgm) - 1)) * mp.tm_per + lm;
+  tn = (xcd >> mp.lgm) * mp.tn_per + ln;
+  return tm < tiles_m && tn < tiles_n;
+}
+
+// items issued before MFMA q when n are spread evenly over the first `over` MFMAs
+constexpr int fz_share(int q, int n, int over) { return over < 1 || q >= over ? n : (q * n + over - 1) / over; }
 
 // E: operand type; TO: type of out / base / pre; BM x BN tile, waves WR x WC; D: ring slots
 template <typename E, typename TO, int BM, int BN, int WR, int WC, int D, bool A_KS, bool B_KS, int EPI>
 struct FzKernel {
-  static constexpr int NW = WR * WC, STAGE = (BM + BN) * 128, LDS = D * STAGE;
+  static constexpr int NW = WR * WC, STAGE = (BM + BN) * 64, LDS = D * STAGE;
   static constexpr bool GATED = EPI == FZ_GATED;
   using OA = FzOperand<BM, WR, NW, A_KS, false, false>;
   using OB = FzOperand<BN, WC, NW, B_KS, true, GATED>;
   static constexpr int MI = OA::NT, NI = OB::NT, C = OA::PPW + OB::PPW;
-  static_assert(D >= 2 && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
+  static_assert(D >= 4 && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
 
   static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b) {
     constexpr int BNO = GATED ? BN / 2 : BN;  // output columns of a tile
     const int NO = GATED ? ep.F : p.N;
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (NO + BNO - 1) / BNO;
-    const G16DMap mp = gemm16d_map(tiles_m, tiles_n, p.M, p.N);
-    const int xcd = b & 7, idx = b >> 3;
-    const int ln = idx / mp.tm_per, lm = idx - ln * mp.tm_per;
-    const int tm = (xcd & ((1 << mp.lgm) - 1)) * mp.tm_per + lm, tn = (xcd >> mp.lgm) * mp.tn_per + ln;
-    if (ln >= mp.tn_per || tm >= tiles_m || tn >= tiles_n) return;
+    int tm, tn;
+    if (!fz_tile(b, tiles_m, tiles_n, gemm16d_map(tiles_m, tiles_n, p.M, p.N), tm, tn)) return;
     const int m0 = tm * BM, n0 = tn * BNO;
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -275,33 +384,42 @@ struct FzKernel {
     oa.setup(p.A, p.lda, m0, p.M, p.K, p.kb, 0, wr, 0);
     // the value rows lead the tile: with the gate half first in memory the descriptor starts at the gate rows and the halves swap
     // places in the tile instead of the offset becoming negative
-    ob.setup(p.B, p.ldb, n0, p.N, p.K, p.kb, BM * 128, wc, GATED ? ep.F : 0);
+    ob.setup(p.B, p.ldb, n0, p.N, p.K, p.kb, OA::SLOT, wc, GATED ? ep.F : 0);
 
-    constexpr int ES = FE<E>::SIZE, STEP = 128 / ES;
+    constexpr int ES = FE<E>::SIZE, STEP = 64 / ES;
     const int nk = (p.K + STEP - 1) / STEP, steps = nk * p.nseg;
-    int seg = 0, kin = 0;  // of the next step to issue
+    int seg = 0, left = nk, records = 0x7fffffff;  // of the next step to issue: its segment, the steps left in it
     auto plane = [](unsigned t, int s) { return (int64_t)((t >> (4 * s)) & 15u); };
     oa.seek(plane(p.pa, 0) * p.a_plane);
     ob.seek(plane(p.pb, 0) * p.b_plane);
-    bool last = false;
     auto open = [&]() {
-      const bool dead = seg >= p.nseg;
-      last = kin == nk - 1;
-      oa.open(dead);
-      ob.open(dead);
-      if (++kin == nk) {
-        kin = 0;
-        ++seg;
-        if (seg < p.nseg) {
-          oa.seek(plane(p.pa, seg) * p.a_plane);
-          ob.seek(plane(p.pb, seg) * p.b_plane);
+      if (left <= 1) {
+        if (left == 0) {
+          if (++seg < p.nseg) {
+            oa.seek(plane(p.pa, seg) * p.a_plane);
+            ob.seek(plane(p.pb, seg) * p.b_plane);
+            oa.tail(false);
+            ob.tail(false);
+            left = nk;
+          } else {
+            records = 0;
+            left = 0x40000000;
+          }
+        }
+        if (left == 1) {
+          oa.tail(true);
+          ob.tail(true);
         }
       }
+      --left;
+      oa.open(records);
+      ob.open(records);
     };
-    for (int s = 0; s < D; ++s) {
+    char* const wslot = smem + wave * 1024;  // this wave's first DMA piece of slot 0
+    for (int s = 0; s < D - 1; ++s) {
       open();
-      oa.issue(smem + s * STAGE, last);
-      ob.issue(smem + s * STAGE + BM * 128, last);
+      oa.issue(wslot + s * STAGE);
+      ob.issue(wslot + s * STAGE + OA::SLOT);
     }
 
     using Acc = typename FE<E>::acc;
@@ -311,60 +429,66 @@ struct FzKernel {
 #pragma unroll
       for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = Acc{0, 0, 0, 0};
 
-    constexpr int NH = MI * NI, STRIDE = NH / C, R1 = OA::NRAW + OB::NRAW;
-    static_assert(STRIDE >= 1, "refill interleave");
+    // Two steps between barriers.  When the waves meet before step s (even), its fragments are in everyone's registers and step s - 1 is
+    // done: both slots are free and take steps s - 1 + D and s + D, one in each half; steps s + 1 and s + 2 have landed (all DMA but the
+    // newest D - 4 steps').  The fragments of the next step are read and its refill is issued BETWEEN the MFMAs: reads over the first
+    // 5/8 of the step, so that they have landed at its end, the DMA pieces evenly.
+    constexpr int NH = MI * NI, RA = OA::NRAW, RB = OB::NRAW, R = RA + RB;
     const unsigned sbase = (unsigned)(size_t)(k4_lds_ptr)smem;
-    typename OA::RawT a0[OA::NRAW], a1[OA::NRAW];
-    typename OB::RawT b0[OB::NRAW], b1[OB::NRAW];
-    k4_wait_vm<(D - 1) * C>();
-    __builtin_amdgcn_s_barrier();
+    struct Frags {
+      typename OA::RawT a[RA];
+      typename OB::RawT b[RB];
+    } f0, f1;
+    auto read_one = [&](auto ic, unsigned sb, Frags& f) {
+      constexpr int I = decltype(ic)::value;
+      if constexpr (I < RB) ob.template read<I>(sb, f.b);
+      else oa.template read<I - RB>(sb, f.a);
+    };
+    k4_wait_vm<(D - 2) * C>();
+    __builtin_amdgcn_s_barrier();  // raw: __syncthreads() would drain the DMA queue
     asm volatile("" ::: "memory");
-    ob.template read<0>(sbase, b0);
-    oa.template read<0>(sbase, a0);
-    int slot = 0;
-    for (int ks = 0; ks < steps; ++ks) {
-      const unsigned sb = sbase + (unsigned)(slot * STAGE);
-      char* fill = smem + slot * STAGE;
-      const int next = slot + 1 == D ? 0 : slot + 1;
-      ob.template read<1>(sb, b1);
-      oa.template read<1>(sb, a1);
-      g16d_lgkm<(R1 > 15 ? 15 : R1)>();
-      OB::tie(b0);
-      OA::tie(a0);
-      __builtin_amdgcn_sched_barrier(0);
-      g16d_for_each([&](auto qc) {
-        constexpr int Q = decltype(qc)::value;
-        acc[Q % MI][Q / MI] = FE<E>::mma(OB::get(b0, Q / MI), OA::get(a0, Q % MI), acc[Q % MI][Q / MI]);
-      }, std::make_integer_sequence<int, NH>{});
-      __builtin_amdgcn_sched_barrier(0);
-      g16d_lgkm<0>();
-      OB::tie(b1);
-      OA::tie(a1);
-      k4_wait_vm<(D - 2) * C>();
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const unsigned sn = sbase + (unsigned)(next * STAGE);
-      ob.template read<0>(sn, b0);
-      oa.template read<0>(sn, a0);
+    g16d_for_each([&](auto ic) { read_one(ic, sbase, f0); }, std::make_integer_sequence<int, R>{});
+    int read_at = 0, fill_at = (D - 1) * STAGE;  // bytes
+    auto step = [&](Frags& now, Frags& then, auto meet) {
+      char* fill = wslot + fill_at;
+      fill_at = fill_at == (D - 1) * STAGE ? 0 : fill_at + STAGE;
+      read_at = read_at == (D - 1) * STAGE ? 0 : read_at + STAGE;
+      const unsigned sn = sbase + (unsigned)read_at;
       open();
+      if constexpr (decltype(meet)::value) k4_wait_vm<(D - 4) * C>();
+      g16d_lgkm<0>();
+      OB::tie(now.b);
+      OA::tie(now.a);
+      if constexpr (decltype(meet)::value) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       g16d_for_each([&](auto qc) {
         constexpr int Q = decltype(qc)::value;
-        acc[Q % MI][Q / MI] = FE<E>::mma(OB::get(b1, Q / MI), OA::get(a1, Q % MI), acc[Q % MI][Q / MI]);
-        if constexpr ((Q + 1) % STRIDE == 0 && (Q + 1) / STRIDE <= C) {
-          constexpr int P = (Q + 1) / STRIDE - 1;
+        acc[Q % MI][Q / MI] = FE<E>::mma(OB::get(now.b, Q / MI), OA::get(now.a, Q % MI), acc[Q % MI][Q / MI]);
+        constexpr int r0 = fz_share(Q, R, NH * 5 / 8), r1 = fz_share(Q + 1, R, NH * 5 / 8), d0 = Q * C / NH, d1 = (Q + 1) * C / NH;
+        if constexpr (r1 > r0 || d1 > d0) {
           __builtin_amdgcn_sched_barrier(0);
-          if constexpr (P < OA::PPW) oa.template issue_piece<P>(fill, last);
-          else ob.template issue_piece<P - OA::PPW>(fill + BM * 128, last);
+          g16d_for_each([&](auto ic) { read_one(std::integral_constant<int, r0 + decltype(ic)::value>{}, sn, then); },
+                        std::make_integer_sequence<int, r1 - r0>{});
+          g16d_for_each([&](auto ic) {
+            constexpr int P = d0 + decltype(ic)::value;
+            if constexpr (P < OA::PPW) oa.template issue_piece<P>(fill);
+            else ob.template issue_piece<P - OA::PPW>(fill + OA::SLOT);
+          }, std::make_integer_sequence<int, d1 - d0>{});
           __builtin_amdgcn_sched_barrier(0);
         }
       }, std::make_integer_sequence<int, NH>{});
-      slot = next;
+    };
+    for (int s = 0; s < steps; s += 2) {  // an odd number of steps ends with one of zeros
+      step(f0, f1, std::true_type{});
+      step(f1, f0, std::false_type{});
     }
     // the reads and refills behind the last step have landed before their registers and LDS are given up
     g16d_lgkm<0>();
-    OB::tie(b0);
-    OA::tie(a0);
+    OB::tie(f0.b);
+    OA::tie(f0.a);
+    OB::tie(f1.b);
+    OA::tie(f1.a);
     k4_wait_vm<0>();
     __builtin_amdgcn_sched_barrier(0);
 
@@ -439,9 +563,10 @@ struct FzKernel {
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] += bs[e];
           }
-          if (ep.pre) {  // what the backward pass reads, rounded to the activation type
-            fz_store8<TO>(ep.pre, row + vrow + n, n, NO, vo && full, v);
-            fz_store8<TO>(ep.pre, row + grow + n, n, NO, vo && full, t);
+          if (ep.pre) {
+            const int64_t prow = row + ep.pre_row * 2 * NO;
+            fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + vrow + n, n, NO, vo && full, v);
+            fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + grow + n, n, NO, vo && full, t);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);

@@ -250,6 +250,10 @@ struct GatedArgs {
     ldw = w.stride(0);
   }
 };
+// what the backward pass reads p from: 3 bytes an element for 16-bit activations, 4 for fp32
+Tensor pre_of(const Tensor& x, int64_t M, int64_t N) {
+  return at::empty({M * N * (x.scalar_type() == at::kFloat ? 4 : 3)}, x.options().dtype(at::kByte));
+}
 std::tuple<Tensor, Tensor> gated_fwd(const Tensor& x, const Tensor& w, const OptTensor& sw, const OptTensor& bias, const OptTensor& base, int64_t act,
                                      bool gate_first, bool keep) {
   need_hip(x, "x");
@@ -265,7 +269,7 @@ std::tuple<Tensor, Tensor> gated_fwd(const Tensor& x, const Tensor& w, const Opt
   Tensor r = rows_of(x, I);
   OptTensor bi = bias_of(bias, 2 * F, x.scalar_type()), ba = base_of(base, x, 2 * F);
   const int64_t M = r.size(0);
-  Tensor h = at::empty(with_last(x, F), x.options()), pre = at::empty({keep ? M : 0, 2 * F}, x.options());
+  Tensor h = at::empty(with_last(x, F), x.options()), pre = pre_of(x, keep ? M : 0, 2 * F);
   Tensor ws = scratch(x, lyc_gated_linear_workspace_bytes(M, I, F, code, a.sw ? LYC_GATED_INT8 : 0), "gated_linear");
   check_rc(lyc_gated_linear_fwd(r.const_data_ptr(), a.w.const_data_ptr(), a.ldw, a.sw, dptr(bi), bias_f32(bi), dptr(ba), h.mutable_data_ptr(),
                                 keep ? pre.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), M, I, F, (int)act, gate_first, code, stream_of(x)),
@@ -285,7 +289,7 @@ Tensor gated_linear_meta(const Tensor& x, const Tensor& w, const OptTensor& sw, 
 }
 std::tuple<Tensor, Tensor> gated_forward_meta(const Tensor& x, const Tensor& w, const OptTensor& sw, const OptTensor& bias, const OptTensor& base, int64_t act,
                                               bool gate_first) {
-  return {gated_linear_meta(x, w, sw, bias, base, act, gate_first), at::empty({x.numel() / w.size(1), w.size(0)}, x.options())};
+  return {gated_linear_meta(x, w, sw, bias, base, act, gate_first), pre_of(x, x.numel() / w.size(1), w.size(0))};
 }
 // (dbase [M, 2 F], dx, dw, dbias); what is not asked for comes back empty
 std::tuple<Tensor, Tensor, Tensor, Tensor> gated_backward_meta(const Tensor& g, const Tensor& pre, const Tensor& x, const Tensor& w, const OptTensor& sw,
@@ -329,6 +333,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     ctx->save_for_backward({pre, w.requires_grad() ? x : Tensor(), w, has(sw) ? *sw : Tensor()});
     ctx->saved_data["bias"] = edge(bias, 2 + has(sw));
     ctx->saved_data["base"] = edge(base, 2 + has(sw) + has(bias));
+    ctx->saved_data["dt"] = (int64_t)x.scalar_type();
     ctx->saved_data["act"] = act;
     ctx->saved_data["gf"] = gate_first;
     ctx->saved_data["bdt"] = (int64_t)(has(bias) ? bias->scalar_type() : x.scalar_type());
@@ -345,7 +350,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1), dbias = wanted(ctx, "bias"), dbase = wanted(ctx, "base");
     if (!(dx || dw || dbias || dbase)) return out;
     OptTensor sw = opt(s[3]);
-    Tensor g = grads[0].to(s[0].scalar_type());
+    Tensor g = grads[0].to((at::ScalarType)ctx->saved_data["dt"].toInt());
     auto [b, x, w, bi] = op.call(g, s[0], s[1].defined() ? s[1] : g, s[2], sw, ctx->saved_data["act"].toInt(), ctx->saved_data["gf"].toBool(), dbase, dx, dw, dbias);
     if (dx) out[0] = x;
     if (dw) out[1] = w;

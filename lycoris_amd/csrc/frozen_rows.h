@@ -103,35 +103,38 @@ __global__ __launch_bounds__(256) void fz_quant_long_kernel(const T* __restrict_
   }
 }
 
-// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): out[o, i] = sw[o] q[o, i] f, one rounding ---------------------
-// f = 1 in bf16.  fp16 has 5 exponent bits and the scales of a weight may lie anywhere: f = 2^e brings the largest entry to [2^13, 2^14),
-// and the product's alpha (`alpha[0] = 2^-e`) takes it out again; every workgroup finds the same e from the scales.  scaled = 0: the
-// integers themselves (exact in bf16; the fp32 product folds sw into the other operand).
-template <typename T>
-__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ sw, T* __restrict__ out, int64_t ldo,
-                                                       float* __restrict__ alpha, int O, int I, int rows_per_wg, int scaled) {
+// ---- fp16 only: the power of two that brings an 8-bit weight's scales into its range --------------------------------------------------
+// The gradients' products take sw either inside the weight plane (sw q) or inside the other operand (sw dp).  fp16 has 5 exponent bits and
+// the scales of a weight may lie anywhere: they are multiplied by f[0] = 2^e, which brings 127 max|sw| to [2^-1, 1) 2^`top`, and the product's
+// alpha, f[1] = 2^-e, takes it out again.
+__global__ __launch_bounds__(256) void fz_range_kernel(const float* __restrict__ sw, int n, int top, float* __restrict__ f) {
   __shared__ float red[4];
-  float f = 1.f;
-  if constexpr (std::is_same<T, _Float16>::value) {
-    float mx = 0.f;
-    for (int o = threadIdx.x; o < O; o += 256) {
-      const float a = fabsf(sw[o]);
-      if (a <= 3.4e38f) mx = fmaxf(mx, a);
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const int e = mx > 1e-30f && mx < 1e30f ? 6 - ilogbf(mx) : 0;  // 127 mx < 2^(ilogb + 8)
-    f = ldexpf(1.f, e);
-    if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = ldexpf(1.f, -e);
+  float mx = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float a = fabsf(sw[i]);
+    if (a <= 3.4e38f) mx = fmaxf(mx, a);
   }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  if (threadIdx.x) return;
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int e = mx > 1e-30f && mx < 1e30f ? top - 8 - ilogbf(mx) : 0;  // 127 mx < 2^(ilogb + 8)
+  f[0] = ldexpf(1.f, e);
+  f[1] = ldexpf(1.f, -e);
+}
+
+// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): out[o, i] = sw[o] f[0] q[o, i], one rounding; without sw the
+// integers themselves, which 16 bits hold exactly.  f: fz_range_kernel's, or null
+template <typename T>
+__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ sw, const float* __restrict__ f,
+                                                       T* __restrict__ out, int64_t ldo, int O, int I, int rows_per_wg) {
   const int chunks = (int)(ldo >> 3);
   for (int r = 0; r < rows_per_wg; ++r) {
     const int o = blockIdx.x * rows_per_wg + r;
     if (o >= O) return;
-    const float s = scaled ? sw[o] * f : 1.f;
+    const float s = sw ? sw[o] * (f ? f[0] : 1.f) : 1.f;
     for (int c = threadIdx.x; c < chunks; c += 256) {
       T t[8];
       if (8 * c + 8 <= I) {
@@ -178,49 +181,89 @@ __global__ __launch_bounds__(256) void fz_stage_kernel(const TI* __restrict__ x,
 }
 
 // ---- gated backward, elementwise: dp = (g act(gate), g value act'(gate)) in the order of p's halves -----------------------------------
-template <typename T>
-__global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const T* __restrict__ pre, T* __restrict__ dp, int64_t M, int F, int act,
-                                                       int gate_first, int vec) {
-  const int chunks = (F + 7) >> 3;
-  const int64_t n = M * chunks;
+// One pass over g and p writes what the rest of the backward pass reads: dp (rounded to the activation type: a gradient, and the operand of
+// dw and dx), dps = sw f[0] dp (one rounding; dx over an 8-bit weight whose plane is its integers, [M, up(2 F, 8)]), and the column sums of
+// dp before rounding, as one partial row per workgroup row (fixed order: the same bits every time).
+// A workgroup takes DG_COLS columns of each half and DG_ROWS rows; a thread 8 columns of every 8th row.
+constexpr int DG_COLS = 256, DG_ROWS = 64;
+template <typename T, typename E>
+__global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const void* __restrict__ pre, T* __restrict__ dp, E* __restrict__ dps,
+                                                       const float* __restrict__ sw, const float* __restrict__ f, float* __restrict__ part, int64_t M, int F,
+                                                       int act, int gate_first, int vec) {
+  __shared__ float sums[2][DG_COLS];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int k = blockIdx.x * DG_COLS + tx * 8;
+  const int64_t m0 = (int64_t)blockIdx.y * DG_ROWS;
   const int vo = gate_first ? F : 0, go = gate_first ? 0 : F;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / chunks;
-    const int k = (int)(i - m * chunks) * 8;
-    const bool full = vec && k + 8 <= F;
-    float gv[8], v[8], t[8], dv[8], dt[8];
-    fz_load8<T>(g, m * F + k, k, F, full, gv);
-    fz_load8<T>(pre, m * 2 * F + vo + k, k, F, full, v);
-    fz_load8<T>(pre, m * 2 * F + go + k, k, F, full, t);
+  const bool full = vec && k + 8 <= F;
+  const int64_t N = 2 * (int64_t)F, lds = (N + 7) & ~7;
+  float sv[8], st[8], cv[8], ct[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float a, da;
-      fz_act_grad(act, t[e], a, da);
-      dv[e] = gv[e] * a;
-      dt[e] = gv[e] * v[e] * da;
+  for (int e = 0; e < 8; ++e) cv[e] = ct[e] = 0.f;
+  if (dps && k < F) {
+    fz_load8<float>(sw, vo + k, k, F, false, sv);
+    fz_load8<float>(sw, go + k, k, F, false, st);
+    const float scale = f ? f[0] : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sv[e] *= scale, st[e] *= scale;
+  }
+  if (k < F) {
+    for (int r = ty; r < DG_ROWS && m0 + r < M; r += 8) {
+      const int64_t m = m0 + r;
+      float gv[8], v[8], t[8], dv[8], dt[8];
+      fz_load8<T>(g, m * F + k, k, F, full, gv);
+      fz_load_pre8<T>(pre, M * N, m * N + vo + k, k, F, full, v);
+      fz_load_pre8<T>(pre, M * N, m * N + go + k, k, F, full, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float a, da;
+        fz_act_grad(act, t[e], a, da);
+        dv[e] = gv[e] * a;
+        dt[e] = gv[e] * v[e] * da;
+        cv[e] += dv[e];
+        ct[e] += dt[e];
+      }
+      if (dp) {
+        fz_store8<T>(dp, m * N + vo + k, k, F, full, dv);
+        fz_store8<T>(dp, m * N + go + k, k, F, full, dt);
+      }
+      if (dps) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dv[e] *= sv[e], dt[e] *= st[e];
+        fz_store8<E>(dps, m * lds + vo + k, k, F, full, dv);
+        fz_store8<E>(dps, m * lds + go + k, k, F, full, dt);
+      }
     }
-    fz_store8<T>(dp, m * 2 * F + vo + k, k, F, full, dv);
-    fz_store8<T>(dp, m * 2 * F + go + k, k, F, full, dt);
+  }
+  if (!part) return;
+  for (int i = 0; i < 8; ++i) {  // rows of threads one after the other
+    if (ty == i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sums[0][tx * 8 + e] = cv[e] + (i ? sums[0][tx * 8 + e] : 0.f);
+        sums[1][tx * 8 + e] = ct[e] + (i ? sums[1][tx * 8 + e] : 0.f);
+      }
+    }
+    __syncthreads();
+  }
+  for (int h = 0; h < 2; ++h) {
+    const int c = blockIdx.x * DG_COLS + threadIdx.x;
+    if (c < F) part[(int64_t)blockIdx.y * N + (h ? go : vo) + c] = sums[h][threadIdx.x];
   }
 }
-
-// ---- column sums of [M, N] in two passes (fixed order: the same bits every time): partials of FZ_SUM_ROWS rows, then their sum ---------
-constexpr int FZ_SUM_ROWS = 256;
+// the partial rows' sum: 8 threads a column, joined in a fixed order
 template <typename T>
-__global__ __launch_bounds__(256) void fz_colsum_kernel(const T* __restrict__ x, float* __restrict__ part, int64_t M, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  const int64_t m0 = (int64_t)blockIdx.y * FZ_SUM_ROWS, m1 = m0 + FZ_SUM_ROWS < M ? m0 + FZ_SUM_ROWS : M;
+__global__ __launch_bounds__(256) void fz_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t parts, int N) {
+  __shared__ float red[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = blockIdx.x * 32 + tx;
   float s = 0.f;
-  for (int64_t m = m0; m < m1; ++m) s += (float)x[m * N + n];
-  part[(int64_t)blockIdx.y * N + n] = s;
-}
-template <typename T>
-__global__ __launch_bounds__(256) void fz_colsum_join_kernel(const float* __restrict__ part, T* __restrict__ out, int parts, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  float s = 0.f;
-  for (int r = 0; r < parts; ++r) s += part[(int64_t)r * N + n];
+  if (n < N)
+    for (int64_t r = ty; r < parts; r += 8) s += part[r * N + n];
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty || n >= N) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += red[i][tx];
   out[n] = (T)s;
 }
 

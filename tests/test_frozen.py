@@ -100,7 +100,7 @@ def test_c_abi_refuses_before_any_launch():
            ("lyc_gated_linear_fwd", (p, p, 0, None, None, 0, None, p, None, p, 2, 8, 4, 3, 0, bf, None), "activation"),
            ("lyc_gated_linear_fwd", (p, p, 8, p, None, 0, None, p, None, p, 2, 8, 4, 0, 0, bf, None), "multiple of 16"),
            ("lyc_gated_linear_fwd", (p + 4, p, 0, None, None, 0, None, p, None, p, 2, 8, 4, 0, 0, bf, None), "aligned"),
-           ("lyc_gated_linear_fwd", (p, p, 0, None, None, 0, None, p, None, p, 2, 1 << 15, 1 << 16, 0, 0, bf, None), "2 GiB"),
+           ("lyc_gated_linear_fwd", (p, p, 0, None, None, 0, None, p, None, p, 2, 1 << 15, 1 << 16, 0, 0, bf, None), "1 GiB"),
            ("lyc_gated_linear_bwd", (p, p, p, p, 16, p, None, p, p, None, p, 2, 8, 4, 0, 0, bf, None), "frozen"),
            ("lyc_gated_linear_bwd", (p, None, p, p, 0, None, None, p, None, None, p, 2, 8, 4, 0, 0, bf, None), "null")]
     for name, args, word in bad:
