@@ -473,8 +473,9 @@ int lyc_rows_to_nchw(const void* rows, void* t, int64_t B, int64_t C, int64_t P,
  * `ws`: device scratch of the *_workspace_bytes(...) bytes (-1: bad arguments), 16-byte aligned, no need to clear.        */
 int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int64_t K, int dtype, void* stream);
 /* y = (sa[m] sb[n]) sum_k aq[m, k] bq[n, k] + bias[n] + base[m, n].  aq's rows hold ZEROS from K up to the next multiple of 16. */
+int64_t lyc_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int lyc_int8_matmul(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32,
-                    const void* base, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+                    const void* base, void* y, void* ws, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
 int64_t lyc_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int backward);
 int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* y, void* ws,
                         int64_t M, int64_t N, int64_t K, int dtype, void* stream);

@@ -71,7 +71,7 @@ SIGNATURES = {
     "lyc_nchw_to_rows": [_vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_rows_to_nchw": [_vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_int8_quantize": [_vp, _i64, _vp, _i64, _fp, _i64, _i64, _i32, _vp],
-    "lyc_int8_matmul": [_vp, _i64, _fp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
+    "lyc_int8_matmul": [_vp, _i64, _fp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_int8_linear_fwd": [_vp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_int8_linear_bwd": [_vp, _vp, _i64, _fp, _vp, _vp, _i64, _i64, _i64, _i32, _vp],
     "lyc_gated_linear_fwd": [_vp, _vp, _i64, _fp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
@@ -91,6 +91,7 @@ VALUE_SIGNATURES = {
     "lyc_lokr_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32], ctypes.c_int),  # 1 / 0, not an error code
     "lyc_locon_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32], ctypes.c_int),
     "lyc_loha_wgrad_deferrable": ([_vp, _vp, _i64, _i32, _i32, _i32, _i32], ctypes.c_int),
+    "lyc_int8_matmul_workspace_bytes": ([_i64, _i64, _i64, _i32], ctypes.c_int64),
     "lyc_int8_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
     "lyc_gated_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
     "lyc_loha_plane_cacheable": ([_fp, _fp, _fp, _fp, _i32, _i32, _i32, _i32], ctypes.c_int),

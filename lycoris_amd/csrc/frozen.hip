@@ -67,66 +67,102 @@ int allow_lds(Kern kern, int bytes) {
   return LYC_OK;
 }
 
+int grid_of(int64_t chunks) { return (int)(cdiv(chunks, 256) < 16384 ? cdiv(chunks, 256) : 16384); }
+
 template <typename K, int BM, int BNO>
 int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
-  const G16DMap mp = gemm16d_map((int)cdiv(p.M, BM), (int)cdiv(K::GATED ? ep.F : p.N, BNO), p.M, p.N);
+  const int per = fz_per_xcd(cdiv(p.M, BM) * cdiv(K::GATED ? ep.F : p.N, BNO));
   FZ_TRY(allow_lds(&fz_gemm_kernel<K>, K::LDS));
-  hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * mp.tm_per * mp.tn_per)), dim3(K::NW * 64), K::LDS, st, p, ep);
+  hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * per), p.ksplit > 1 ? p.ksplit : 1), dim3(K::NW * 64), K::LDS, st, p, ep);
   return check_launch("fz_gemm");
 }
 
-// Which tiles for a product of M x NO outputs and `steps` 64-byte steps of K: 256 x 256 (one workgroup a CU), 128 x 128 (two) or 64 x 64
-// (three) -- and, where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those tiles over the rows that fill whole
-// rounds and 128 x 128 ones over the rest.  The rule compares estimates in microseconds: a round costs what a step costs times the steps,
-// plus what a tile's beginning and end leave exposed.
-struct TileCost {
-  double step, tile;
+// Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.  Tiles of 256 x 256 (one
+// workgroup a CU), 128 x 128 (two) or 64 x 64 (three); where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those
+// over the rows that fill whole rounds and 128 x 128 ones over the rest; where the tiles are few and K is long, K in parts.
+// The rule compares estimates in microseconds: a round costs what a step costs times the steps, plus what a tile's beginning and end leave
+// exposed -- of its epilogue's bytes, at a CU's share of HBM, all with one workgroup a CU, half of it where a second one computes meanwhile.
+struct Plan {
+  int tile = 128, ksplit = 1;
+  int64_t whole = 0;  // row tiles of 256 ahead of the 128s
+  double us = 1e30;
 };
-constexpr TileCost T256{0.66, 6.0}, T128_2{0.44, 3.0}, T128_1{0.28, 4.0}, T64_3{0.36, 2.5}, T64_2{0.26, 2.5}, T64_1{0.18, 3.0};
-double round_cost(TileCost c, double steps) { return c.step * steps + c.tile; }
-double cost256(int64_t tiles, double steps) { return (double)cdiv(tiles, 256) * round_cost(T256, steps); }
-double cost128(int64_t tiles, double steps) {
-  const int64_t r = tiles % 512;
-  return (double)(tiles / 512) * round_cost(T128_2, steps) + (r == 0 ? 0.0 : round_cost(r <= 256 ? T128_1 : T128_2, steps));
+struct Rate {
+  double step, tile, shown;
+};
+constexpr Rate R256{0.72, 4.0, 1.0}, R128_2{0.48, 2.5, 0.5}, R128_1{0.30, 3.0, 1.0}, R64_3{0.36, 2.0, 0.35}, R64_2{0.26, 2.0, 0.5}, R64_1{0.18, 2.5, 1.0};
+constexpr double CU_BYTES_PER_US = 19900.0;
+double rounds_cost(int64_t tiles, int wgs, const Rate* by_load, double steps, double bytes) {
+  const int64_t per = fz_per_xcd(tiles), slots = 32 * wgs, full = per / slots, rest = per % slots;
+  auto one = [&](int load) { return by_load[load - 1].step * steps + by_load[load - 1].tile + by_load[load - 1].shown * load * bytes / CU_BYTES_PER_US; };
+  return (double)full * one(wgs) + (rest ? one((int)cdiv(rest, 32)) : 0.0);
 }
-double cost64(int64_t tiles, double steps) {
-  const int64_t r = tiles % 768;
-  return (double)(tiles / 768) * round_cost(T64_3, steps) + (r == 0 ? 0.0 : round_cost(r <= 256 ? T64_1 : r <= 512 ? T64_2 : T64_3, steps));
+// eb: bytes the epilogue moves per output; split: may K be split
+Plan plan_gemm(int64_t M, int64_t NO, double steps, bool gated, double eb, bool split) {
+  static constexpr Rate r256[] = {R256}, r128[] = {R128_1, R128_2}, r64[] = {R64_1, R64_2, R64_3};
+  const int o = gated ? 2 : 1;
+  auto cost = [&](int tile, int64_t rows, double st, double e, int parts) {
+    const int64_t tn = cdiv(NO, tile == 64 ? 64 : tile / o), tiles = cdiv(rows, tile) * tn * parts;
+    const double out = tile == 64 ? 64.0 * 64.0 : (double)tile * tile / o;
+    if (tile == 256) return rounds_cost(tiles, 1, r256, st, out * e);
+    if (tile == 128) return rounds_cost(tiles, 2, r128, st, out * e);
+    return rounds_cost(tiles, 3, r64, gated ? 1.4 * st : st, out * e);
+  };
+  Plan best;
+  auto offer = [&](int tile, int ks, int64_t whole, double us) {
+    if (us < best.us) best = Plan{tile, ks, whole, us};
+  };
+  for (int tile : {128, 64, 256}) {
+    offer(tile, 1, 0, cost(tile, M, steps, eb, 1));
+    if (!split) continue;
+    for (int ks = 2; ks <= 8 && steps / ks >= 12; ++ks)  // the sums are written, read and finished by a second launch
+      offer(tile, ks, 0, cost(tile, M, cdiv((int64_t)steps, ks), 4.0, ks) + 3.0 + (double)M * NO * (4.0 * ks + eb) / (256 * CU_BYTES_PER_US));
+  }
+  const int64_t tn = cdiv(NO, 256 / o), tm = cdiv(M, 256), whole = tm * tn / 256 * 256 / tn;
+  if (whole > 0 && whole < tm) offer(128, 1, whole, cost(256, whole * 256, steps, eb, 1) + cost(128, M - whole * 256, steps, eb, 1) + 1.0);
+  return best;
 }
+template <typename E, int EPI>
+Plan plan_of(int64_t M, int64_t NO, int64_t K, int nseg, double eb) {
+  return plan_gemm(M, NO, (double)cdiv(K * FE<E>::SIZE, 64) * nseg, EPI == FZ_GATED, eb, EPI != FZ_GATED);
+}
+// bytes of a plan's partial sums
+int64_t part_bytes(const Plan& pl, int64_t M, int64_t N) { return pl.ksplit > 1 ? pl.ksplit * M * N * 4 : 0; }
 
 template <typename E, typename TO, bool A_KS, bool B_KS, int EPI>
-int launch_gemm(const FzProb& p, const FzEpi& ep, hipStream_t st) {
+int launch_gemm(const Plan& pl, FzProb p, FzEpi ep, void* part, hipStream_t st) {
   constexpr bool G = EPI == FZ_GATED;
   constexpr int O = G ? 2 : 1;  // B rows an output column takes
   using K256 = FzKernel<E, TO, 256, 256, 2, 4, 5, A_KS, B_KS, EPI>;
   using K128 = FzKernel<E, TO, 128, 128, 4, 2, 5, A_KS, B_KS, EPI>;
   using K64 = FzKernel<E, TO, 64, 64 * O, 2, 2, 6, A_KS, B_KS, EPI>;
-  const int64_t M = p.M, NO = G ? ep.F : p.N;
-  const double steps = (double)cdiv((int64_t)p.K * FE<E>::SIZE, 64) * p.nseg;
-  const int64_t tn256 = cdiv(NO, 256 / O), tn128 = cdiv(NO, 128 / O);
-  const int64_t tm256 = cdiv(M, 256), whole = tm256 * tn256 / 256 * 256 / tn256;  // row tiles that fill whole rounds
-  const double c256 = cost256(tm256 * tn256, steps), c128 = cost128(cdiv(M, 128) * tn128, steps);
-  const double c64 = cost64(cdiv(M, 64) * cdiv(NO, 64), steps * (G ? 1.4 : 1.0));
-  const double mixed = whole > 0 && whole < tm256 ? cost256(whole * tn256, steps) + cost128(cdiv(M - whole * 256, 128) * tn128, steps) + 2.0 : 1e30;
-  if (mixed < c256 && mixed < c128 && mixed < c64) {
-    const int64_t m = whole * 256;
+  const int64_t NO = G ? ep.F : p.N;
+  p.ksplit = pl.ksplit;
+  ep.part = part;
+  if (pl.whole) {
+    const int64_t m = pl.whole * 256;
     FzProb a = p, b = p;
     a.M = (int)m;
-    b.M = (int)(M - m);
+    b.M = (int)(p.M - m);
     b.A = static_cast<const char*>(p.A) + (A_KS ? 2 * m : m * p.lda);
     FzEpi e = ep;
     e.out = static_cast<TO*>(ep.out) + m * NO;
     if (ep.sa) e.sa = ep.sa + m;
     if (ep.base) e.base = static_cast<const TO*>(ep.base) + m * NO * O;
-    // (p's planes are addressed by row: the 16-bit one and, behind all of it, the 8-bit one)
-    FzEpi f = ep;
-    FZ_TRY((launch_tile<K256, 256, 256 / O>(a, f, st)));
-    e.pre_row = ep.pre_row + m;
+    e.pre_row = ep.pre_row + m;  // (p's two planes are addressed by row)
+    FZ_TRY((launch_tile<K256, 256, 256 / O>(a, ep, st)));
     return launch_tile<K128, 128, 128 / O>(b, e, st);
   }
-  if (c64 < c128 && c64 < c256) return launch_tile<K64, 64, 64>(p, ep, st);
-  if (c128 <= c256) return launch_tile<K128, 128, 128 / O>(p, ep, st);
-  return launch_tile<K256, 256, 256 / O>(p, ep, st);
+  if (pl.tile == 64) FZ_TRY((launch_tile<K64, 64, 64>(p, ep, st)));
+  else if (pl.tile == 128) FZ_TRY((launch_tile<K128, 128, 128 / O>(p, ep, st)));
+  else FZ_TRY((launch_tile<K256, 256, 256 / O>(p, ep, st)));
+  if constexpr (!G) {
+    if (p.ksplit > 1) {
+      hipLaunchKernelGGL((fz_reduce_kernel<E, TO>), dim3(grid_of((int64_t)p.M * cdiv(p.N, 8))), dim3(256), 0, st, p, ep);
+      return check_launch("fz_reduce");
+    }
+  }
+  return LYC_OK;
 }
 
 // up to 32 rows: frozen_skinny.h.  x: the activations when the kernel quantises them itself, else null
@@ -162,16 +198,17 @@ int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, 
     hipLaunchKernelGGL((fz_quant_kernel<T, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
   };
   using std::integral_constant;
+  // a wave a row while its registers hold it; rows of 2048 columns and more are spread over a workgroup
   if (c <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (c <= 128) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (c <= 192) go(integral_constant<int, 64>{}, integral_constant<int, 3>{});
   else if (c <= 256) go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
   else if (c <= 512) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (c <= 768) go(integral_constant<int, 256>{}, integral_constant<int, 3>{});
   else if (c <= 1024) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
   else hipLaunchKernelGGL((fz_quant_long_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
   return check_launch("int8_quantize");
 }
-
-int grid_of(int64_t chunks) { return (int)(cdiv(chunks, 256) < 16384 ? cdiv(chunks, 256) : 16384); }
 
 // x [rows, cols] contiguous -> NP planes of [rows, up(cols, 8)]
 template <typename TI, typename TO, int NP>
@@ -237,15 +274,18 @@ FzProb prob(const void* A, int64_t lda, int64_t a_plane, const void* B, int64_t 
   return p;
 }
 
+// (the estimate takes a base operand for granted: the workspace is sized before it is known)
+Plan plan8(int64_t M, int64_t N, int64_t K, int dtype) { return plan_of<int8_t, FZ_LINEAR>(M, N, K, 1, dtype == LYC_F32 ? 8.0 : 4.0); }
+int64_t part8(int64_t M, int64_t N, int64_t K, int dtype) { return M <= SKINNY_ROWS ? 0 : part_bytes(plan8(M, N, K, dtype), M, N); }
 int matmul8(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32, const void* base,
-            void* y, int64_t M, int64_t N, int64_t K, int dtype, hipStream_t st) {
+            void* y, void* part, int64_t M, int64_t N, int64_t K, int dtype, hipStream_t st) {
   FzProb p = prob(aq, lda, 0, bq, ldb, 0, M, N, K, 1);
   FzEpi ep{};
   ep.out = y; ep.sa = sa; ep.sw = sb; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base;
   if (M <= SKINNY_ROWS) {
     FZ_DTYPE(dtype, return (launch_skinny<int8_t, T, T, false, false>(nullptr, p, ep, st)));
   }
-  FZ_DTYPE(dtype, return (launch_gemm<int8_t, T, false, false, FZ_LINEAR>(p, ep, st)));
+  FZ_DTYPE(dtype, return (launch_gemm<int8_t, T, false, false, FZ_LINEAR>(plan8(M, N, K, dtype), p, ep, part, st)));
   return LYC_OK;
 }
 
@@ -264,6 +304,8 @@ int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve
   E* plane = ws.take<E>(N * up(K, 8));
   float* f = ws.take<float>(2);
   Operand<T> a(ws, M, N, true);
+  const Plan pl = plan_of<E, FZ_PLAIN>(M, K, N, F32 ? 3 : 1, sizeof(T));
+  char* part = ws.take<char>(part_bytes(pl, M, K));
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
@@ -277,7 +319,7 @@ int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve
   FzEpi ep{};
   ep.out = dx;
   ep.alpha = range ? range + 1 : nullptr;
-  return launch_gemm<E, T, false, true, FZ_PLAIN>(p, ep, st);
+  return launch_gemm<E, T, false, true, FZ_PLAIN>(pl, p, ep, part, st);
 }
 
 // ---- gated projection ---------------------------------------------------------------------------------------------------------------------
@@ -295,15 +337,17 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
   FzEpi ep{};
   ep.out = h; ep.pre = pre; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base; ep.sw = q.sw; ep.act = q.act; ep.gate_first = q.gate_first; ep.F = (int)q.F;
   ep.pre_total = 2 * q.M * q.F;
+  const double eb = (double)sizeof(T) * (base ? 3 : 1) + (pre ? sizeof(T) == 4 ? 8.0 : 6.0 : 0.0);  // what the epilogue moves per output
   if (q.sw) {
     const int64_t ldq = up(q.I, 16);
-    int8_t* xq = ws.take<int8_t>(q.M * ldq);
-    float* sa = ws.take<float>(q.M);
+    const bool fused = skinny_fused(q.M, q.I);
+    int8_t* xq = fused ? nullptr : ws.take<int8_t>(q.M * ldq);
+    float* sa = fused ? nullptr : ws.take<float>(q.M);
     if (bytes) {
       *bytes = ws.used;
       return LYC_OK;
     }
-    if (skinny_fused(q.M, q.I)) {
+    if (fused) {
       FzProb p = prob(nullptr, 0, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
       return launch_skinny<int8_t, T, T, true, true>(x, p, ep, st);
     }
@@ -311,7 +355,7 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
     ep.sa = sa;
     FzProb p = prob(xq, ldq, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
     if (q.M <= SKINNY_ROWS) return launch_skinny<int8_t, T, T, true, false>(nullptr, p, ep, st);
-    return launch_gemm<int8_t, T, false, false, FZ_GATED>(p, ep, st);
+    return launch_gemm<int8_t, T, false, false, FZ_GATED>(plan_of<int8_t, FZ_GATED>(q.M, q.F, q.I, 1, eb), p, ep, nullptr, st);
   }
   Operand<T> a(ws, q.M, q.I, true), b(ws, 2 * q.F, q.I, true);
   if (bytes) {
@@ -325,7 +369,14 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
   if constexpr (sizeof(T) == 2) {
     if (q.M <= SKINNY_ROWS) return launch_skinny<E, T, T, true, false>(nullptr, p, ep, st);
   }
-  return launch_gemm<E, T, false, false, FZ_GATED>(p, ep, st);
+  return launch_gemm<E, T, false, false, FZ_GATED>(plan_of<E, FZ_GATED>(q.M, q.F, q.I, sizeof(T) == 4 ? 6 : 1, eb), p, ep, nullptr, st);
+}
+
+// rows a workgroup of the elementwise pass takes: as many as leave 1024 workgroups (four a CU), 64 at most (fewer partial column sums)
+int dgate_rows(int64_t M, int64_t F) {
+  int rows = 64;
+  while (rows > 8 && cdiv(F, DG_COLS) * cdiv(M, rows) < 1024) rows /= 2;
+  return rows;
 }
 
 // dp is written once, by one elementwise pass.  dx over an 8-bit weight takes dp sw (16 bits: rounded once, from fp32; 32 bits: staged in
@@ -335,7 +386,8 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   using E = typename Operand<T>::E;
   constexpr bool F32 = sizeof(T) == 4;
   const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
-  const int64_t N = 2 * q.F, parts = cdiv(q.M, DG_ROWS);
+  const int rows = dgate_rows(q.M, q.F);
+  const int64_t N = 2 * q.F, parts = cdiv(q.M, rows);
   const bool scaled = held && want_dx && !F32;  // dps
   if (!(flags & LYC_GATED_DBASE)) dp = want_dw || (want_dx && !scaled) ? ws.take<T>(q.M * N) : nullptr;
   E* dps = scaled ? ws.take<E>(q.M * up(N, 8)) : nullptr;
@@ -344,6 +396,9 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   E* plane = want_dx && held ? ws.take<E>(N * up(q.I, 8)) : nullptr;
   float* f = ws.take<float>(2);
   float* part = flags & LYC_GATED_DBIAS ? ws.take<float>(parts * N) : nullptr;
+  const Plan pdx = plan_of<E, FZ_PLAIN>(q.M, q.I, N, F32 ? (held ? 3 : 6) : 1, sizeof(T)), pdw = plan_of<E, FZ_PLAIN>(N, q.I, q.M, F32 ? 6 : 1, sizeof(T));
+  const int64_t sdx = want_dx ? part_bytes(pdx, q.M, q.I) : 0, sdw = want_dw ? part_bytes(pdw, N, q.I) : 0;
+  char* sums = ws.take<char>(sdx > sdw ? sdx : sdw);
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
@@ -352,7 +407,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   if (scaled) FZ_TRY(launch_range<E>(q.sw, N, 7, f, &range, st));  // the largest sw f[0] near 1
   const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp);
   hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)cdiv(q.F, DG_COLS), (unsigned)parts), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
-                     (int)q.F, q.act, q.gate_first, vec);
+                     (int)q.F, q.act, q.gate_first, vec, rows);
   FZ_TRY(check_launch("gated backward"));
   if (want_dw || (want_dx && !scaled)) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));
   if (want_dx) {
@@ -369,7 +424,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
       p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, q.I, N, 2);
     }
     segments(p, F32 ? (held ? 3 : 6) : 1);
-    FZ_TRY((launch_gemm<E, T, false, true, FZ_PLAIN>(p, ep, st)));
+    FZ_TRY((launch_gemm<E, T, false, true, FZ_PLAIN>(pdx, p, ep, sums, st)));
   }
   if (want_dw) {
     FZ_TRY(xo.fill(x, nullptr, st));
@@ -377,7 +432,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
     segments(p, F32 ? 6 : 1);
     FzEpi ep{};
     ep.out = dw;
-    FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(p, ep, st)));
+    FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(pdw, p, ep, sums, st)));
   }
   if (part) {
     hipLaunchKernelGGL((fz_join_kernel<T>), dim3((unsigned)cdiv(N, 32)), dim3(256), 0, st, part, dbias, parts, (int)N);
@@ -408,22 +463,29 @@ int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float*
   return LYC_OK;
 }
 
+int64_t lyc_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  return check_dims("int8_matmul", M, N, K, dtype) == LYC_OK ? part8(M, N, K, dtype) : -1;
+}
+
 int lyc_int8_matmul(const int8_t* aq, int64_t lda, const float* sa, const int8_t* bq, int64_t ldb, const float* sb, const void* bias, int bias_f32,
-                    const void* base, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
+                    const void* base, void* y, void* ws, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
   FZ_TRY(check_dims("int8_matmul", M, N, K, dtype));
   if (M == 0) return LYC_OK;
   if (!sa || !sb || !y) return fail(LYC_ERR_ARG, "int8_matmul: null pointer");
   FZ_TRY(check_q("int8_matmul", "a", aq, lda, K));
   FZ_TRY(check_q("int8_matmul", "b", bq, ldb, K));
-  return matmul8(aq, lda, sa, bq, ldb, sb, bias, bias_f32, base, y, M, N, K, dtype, static_cast<hipStream_t>(stream));
+  FZ_TRY(need16("int8_matmul", "workspace", ws, lyc_int8_matmul_workspace_bytes(M, N, K, dtype) == 0));
+  return matmul8(aq, lda, sa, bq, ldb, sb, bias, bias_f32, base, y, ws, M, N, K, dtype, static_cast<hipStream_t>(stream));
 }
 
 int64_t lyc_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int backward) {
   if (check_dims("int8_linear", M, N, K, dtype) != LYC_OK) return -1;
   Carve ws{nullptr};
   if (!backward) {
+    if (skinny_fused(M, K)) return 0;
     ws.take<int8_t>(M * up(K, 16));
     ws.take<float>(M);
+    ws.take<char>(part8(M, N, K, dtype));
     return ws.used;
   }
   int64_t n = 0;
@@ -437,7 +499,7 @@ int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const floa
   FZ_TRY(check_dims(who, M, N, K, dtype));
   if (M == 0) return LYC_OK;
   if (!x || !sw || !y) return fail(LYC_ERR_ARG, "%s: null pointer", who);
-  FZ_TRY(need16(who, "workspace", ws));
+  FZ_TRY(need16(who, "workspace", ws, skinny_fused(M, K)));
   FZ_TRY(check_q(who, "wq", wq, ldw, K));
   Carve c{static_cast<char*>(ws)};
   const int64_t ldq = up(K, 16);
@@ -451,7 +513,7 @@ int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const floa
     FZ_DTYPE(dtype, return (launch_skinny<int8_t, T, T, false, true>(static_cast<const T*>(x), p, ep, st)));
   }
   FZ_DTYPE(dtype, FZ_TRY(launch_quant<T>(static_cast<const T*>(x), K, xq, ldq, sa, M, (int)K, st)));
-  return matmul8(xq, ldq, sa, wq, ldw, sw, bias, bias_f32, base, y, M, N, K, dtype, st);
+  return matmul8(xq, ldq, sa, wq, ldw, sw, bias, bias_f32, base, y, c.take<char>(part8(M, N, K, dtype)), M, N, K, dtype, st);
 }
 
 int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const float* sw, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int dtype,

@@ -109,10 +109,12 @@ struct FzProb {
   int M, N, K, kb;
   int nseg;
   unsigned pa, pb;
+  int ksplit;  // the steps go to this many workgroups a tile (blockIdx.y); more than one: raw sums to FzEpi::part
 };
 
 enum { FZ_PLAIN = 0, FZ_LINEAR = 1, FZ_GATED = 2 };
 struct FzEpi {
+  void* part;          // ksplit > 1: [ksplit, M, N] fp32 (8-bit: int32), which fz_reduce_kernel finishes
   void* out;           // [M, N] (GATED: [M, F]), row pitch = N (F) elements
   void* pre;           // GATED: p [M, 2 F] for the backward pass (fz_store_pre8) or null
   const float* alpha;  // PLAIN: device scalar on the result, or null
@@ -340,18 +342,21 @@ __device__ __forceinline__ void fz_load_pre8(const void* pre, int64_t total, int
 }
 inline __host__ __device__ bool fz_al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Workgroup -> tile: the 8 XCDs (workgroups round-robin) as a grid over the output as in gemm16d.h; inside an XCD's block the tiles go in
-// bands of 8 row tiles, column by column, so that the 32 or 64 in flight at a time are a block of it and share both operands in the L2.
-__device__ __forceinline__ bool fz_tile(int b, int tiles_m, int tiles_n, const G16DMap& mp, int& tm, int& tn) {
+// Workgroup -> tile.  The tiles are numbered in bands of 8 row tiles, column by column inside a band, and each of the 8 XCDs (workgroups go
+// round-robin over them) takes one contiguous eighth of the numbers: the 32 or 64 tiles in flight on an XCD are a block that shares both
+// operands in its L2, and no XCD has more than one tile more than another (a grid of XCDs over the output left 35 tiles to one and 10 to
+// another of a 51 x 5 problem: two rounds of its 32 CUs instead of one).
+__host__ __device__ inline int fz_per_xcd(int64_t tiles) { return (int)((tiles + 7) >> 3); }
+__device__ __forceinline__ bool fz_tile(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
   constexpr int BAND = 8;
-  const int xcd = b & 7, idx = b >> 3;
-  const int band = idx / (BAND * mp.tn_per), in = idx - band * BAND * mp.tn_per;
-  const int h = min(BAND, mp.tm_per - band * BAND);
-  if (h <= 0) return false;
-  const int ln = in / h, lm = band * BAND + in - ln * h;
-  tm = (xcd & ((1 << mp.lgm) - 1)) * mp.tm_per + lm;
-  tn = (xcd >> mp.lgm) * mp.tn_per + ln;
-  return tm < tiles_m && tn < tiles_n;
+  const int tiles = tiles_m * tiles_n, per = fz_per_xcd(tiles);
+  const int t = (b & 7) * per + (b >> 3);
+  if ((b >> 3) >= per || t >= tiles) return false;
+  const int band = t / (BAND * tiles_n), in = t - band * BAND * tiles_n;
+  const int h = min(BAND, tiles_m - band * BAND);
+  tn = in / h;
+  tm = band * BAND + in - tn * h;
+  return true;
 }
 
 // items issued before MFMA q when n are spread evenly over the first `over` MFMAs
@@ -367,12 +372,12 @@ struct FzKernel {
   static constexpr int MI = OA::NT, NI = OB::NT, C = OA::PPW + OB::PPW;
   static_assert(D >= 4 && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
 
-  static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b) {
+  static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b, int z) {
     constexpr int BNO = GATED ? BN / 2 : BN;  // output columns of a tile
     const int NO = GATED ? ep.F : p.N;
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (NO + BNO - 1) / BNO;
     int tm, tn;
-    if (!fz_tile(b, tiles_m, tiles_n, gemm16d_map(tiles_m, tiles_n, p.M, p.N), tm, tn)) return;
+    if (!fz_tile(b, tiles_m, tiles_n, tm, tn)) return;
     const int m0 = tm * BM, n0 = tn * BNO;
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -387,15 +392,27 @@ struct FzKernel {
     ob.setup(p.B, p.ldb, n0, p.N, p.K, p.kb, OA::SLOT, wc, GATED ? ep.F : 0);
 
     constexpr int ES = FE<E>::SIZE, STEP = 64 / ES;
-    const int nk = (p.K + STEP - 1) / STEP, steps = nk * p.nseg;
+    const int nk = (p.K + STEP - 1) / STEP;
+    int steps = nk * p.nseg;
     int seg = 0, left = nk, records = 0x7fffffff;  // of the next step to issue: its segment, the steps left in it
+    int todo = 0x40000000;                         // steps left to issue at all, where the range ends inside a segment
     auto plane = [](unsigned t, int s) { return (int64_t)((t >> (4 * s)) & 15u); };
-    oa.seek(plane(p.pa, 0) * p.a_plane);
-    ob.seek(plane(p.pb, 0) * p.b_plane);
+    int first = 0;
+    if constexpr (!GATED) {
+      if (p.ksplit > 1) {
+        const int from = (int)((int64_t)steps * z / p.ksplit), to = (int)((int64_t)steps * (z + 1) / p.ksplit);
+        seg = from / nk;
+        first = from - seg * nk;
+        left = nk - first;
+        steps = todo = to - from;
+      }
+    }
+    oa.seek(plane(p.pa, seg) * p.a_plane + (int64_t)first * oa.kstep);
+    ob.seek(plane(p.pb, seg) * p.b_plane + (int64_t)first * ob.kstep);
     auto open = [&]() {
       if (left <= 1) {
         if (left == 0) {
-          if (++seg < p.nseg) {
+          if (++seg < p.nseg && todo > 0) {
             oa.seek(plane(p.pa, seg) * p.a_plane);
             ob.seek(plane(p.pb, seg) * p.b_plane);
             oa.tail(false);
@@ -412,6 +429,9 @@ struct FzKernel {
         }
       }
       --left;
+      if constexpr (!GATED) {
+        if (todo-- == 0) records = 0;
+      }
       oa.open(records);
       ob.open(records);
     };
@@ -491,6 +511,31 @@ struct FzKernel {
     OA::tie(f1.a);
     k4_wait_vm<0>();
     __builtin_amdgcn_sched_barrier(0);
+
+    if constexpr (!GATED) {
+      if (p.ksplit > 1) {  // raw sums, 16 bytes a lane
+        char* part = static_cast<char*>(ep.part) + (int64_t)z * p.M * p.N * 4;
+        const bool v4 = (p.N & 3) == 0;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+          const int m = m0 + wr * (BM / WR) + 16 * mi + li;
+#pragma unroll
+          for (int ni = 0; ni < NI; ++ni) {
+            const int n = n0 + wc * (BN / WC) + 32 * (ni >> 1) + 8 * g + 4 * (ni & 1);
+            if (m >= p.M || n >= p.N) continue;
+            char* at = part + ((int64_t)m * p.N + n) * 4;
+            if (v4) {
+              *reinterpret_cast<Acc*>(at) = acc[mi][ni];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) reinterpret_cast<decltype(+acc[mi][ni][0])*>(at)[e] = acc[mi][ni][e];
+            }
+          }
+        }
+        return;
+      }
+    }
 
     // ---- epilogue: acc[mi][2 q + e] of lane (li, g) is row 16 mi + li, columns 32 q + 8 g + 4 e .. + 3 of the wave's part ----------
     constexpr int NQ = GATED ? NI / 4 : NI / 2;
@@ -583,7 +628,56 @@ constexpr int fz_waves_per_simd() { return K::NW * (2 * K::LDS <= 160 * 1024 ? 2
 template <typename K>
 __global__ __launch_bounds__(K::NW * 64, fz_waves_per_simd<K>()) void fz_gemm_kernel(FzProb p, FzEpi ep) {
   extern __shared__ __attribute__((aligned(1024))) char fz_smem[];
-  K::run(p, ep, fz_smem, (int)blockIdx.x);
+  K::run(p, ep, fz_smem, (int)blockIdx.x, (int)blockIdx.y);
+}
+
+// the sums of a split K joined in the order of K, then the epilogue (PLAIN, LINEAR)
+template <typename E, typename TO>
+__global__ __launch_bounds__(256) void fz_reduce_kernel(FzProb p, FzEpi ep) {
+  using S = typename std::conditional<FE<E>::SIZE == 1, int, float>::type;
+  const int N = p.N, chunks = (N + 7) >> 3;
+  const int64_t plane = (int64_t)p.M * N, total = (int64_t)p.M * chunks;
+  const bool pitch8 = (N & 7) == 0, vo = pitch8 && fz_al16(ep.out) && fz_al16(ep.base), vb = pitch8 && fz_al16(ep.bias), vs = pitch8 && fz_al16(ep.sw);
+  const float alpha = ep.alpha ? *ep.alpha : 1.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / chunks;
+    const int n = (int)(i - m * chunks) * 8;
+    const S* src = static_cast<const S*>(ep.part) + m * N + n;
+    S s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0;
+    for (int z = 0; z < p.ksplit; ++z, src += plane) {
+      if (pitch8) {
+        const u32x4 a = reinterpret_cast<const u32x4*>(src)[0], b = reinterpret_cast<const u32x4*>(src)[1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += __builtin_bit_cast(S, e < 4 ? a[e & 3] : b[e & 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < N) s[e] += src[e];
+      }
+    }
+    float v[8], t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)s[e] * alpha;
+    if (ep.sw) {
+      const float sa = ep.sa[m];
+      fz_load8<float>(ep.sw, n, n, N, vs, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * sa * t[e];
+    }
+    if (ep.bias) {
+      fz_bias8<TO>(ep, n, n, N, vb, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    if (ep.base) {
+      fz_load8<TO>(ep.base, m * N + n, n, N, vo, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
+    fz_store8<TO>(ep.out, m * N + n, n, N, vo, v);
+  }
 }
 
 }  // namespace lyc

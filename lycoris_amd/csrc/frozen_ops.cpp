@@ -27,6 +27,7 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void check_rc(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, "): ", lyc_last_error()); }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) == 0; }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+void* mptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const void* dptr(const OptTensor& t) { return has(t) ? t->const_data_ptr() : nullptr; }
 
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
@@ -46,6 +47,7 @@ void need_hip(const Tensor& x, const char* what) {
 
 // [.., K] -> contiguous, 16-byte aligned [M, K]
 Tensor rows_of(const Tensor& x, int64_t K) {
+  if (x.dim() == 2 && x.is_contiguous() && aligned(x)) return x;  // no new tensor: host time per call
   Tensor r = x.reshape({x.numel() / K, K}).contiguous();
   return aligned(r) ? r : r.clone();
 }
@@ -59,7 +61,7 @@ Tensor rows8(const Tensor& q, bool zero_tail) {
 }
 Tensor scales_of(const Tensor& s, int64_t n, const char* what) {
   TORCH_CHECK(s.scalar_type() == at::kFloat && s.numel() == n, "lycoris_amd: ", what, " must be ", n, " float32 values, got ", s.sizes(), " ", s.scalar_type());
-  return s.reshape({n}).contiguous();
+  return s.dim() == 1 && s.is_contiguous() ? s : s.reshape({n}).contiguous();
 }
 // bias as the kernels read it: the activation type or fp32
 OptTensor bias_of(const OptTensor& b, int64_t n, at::ScalarType act) {
@@ -84,6 +86,7 @@ std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
 }
 Tensor scratch(const Tensor& x, int64_t bytes, const char* what) {
   TORCH_CHECK(bytes >= 0, what, ": ", lyc_last_error());
+  if (bytes == 0) return Tensor();
   return at::empty({bytes}, x.options().dtype(at::kByte));
 }
 void check_act_x(const Tensor& x, int64_t K, const char* what) {
@@ -93,6 +96,11 @@ void check_act_x(const Tensor& x, int64_t K, const char* what) {
 void check_w8(const Tensor& wq, const char* what) {
   TORCH_CHECK(wq.dim() == 2 && wq.scalar_type() == at::kChar && wq.size(0) > 0 && wq.size(1) > 0, what, ": the 8-bit operand must be a non-empty int8 matrix, got ",
               wq.sizes(), " ", wq.scalar_type());
+}
+// a plain device tensor outside of tracing and batching: the device function can be called without another trip through the dispatcher
+bool eager(const Tensor& t) {
+  const c10::DispatchKeySet ks = t.key_set();
+  return t.is_cuda() && !ks.has(c10::DispatchKey::Python) && !ks.has(c10::DispatchKey::Functionalize) && !ks.has(c10::DispatchKey::FuncTorchBatched);
 }
 void once(const char* what) { TORCH_CHECK(!c10::GradMode::is_enabled(), what, " can be differentiated once only (create_graph is not supported)"); }
 
@@ -145,8 +153,9 @@ Tensor int8_matmul(const Tensor& aq, const Tensor& sa, const Tensor& bq, const T
   Tensor fa = scales_of(sa, M, "the scale of a"), fb = scales_of(sb, N, "the scale of b");
   OptTensor bi = bias_of(bias, N, dtype);
   Tensor y = at::empty(with_last(aq, N), aq.options().dtype(dtype));
+  Tensor ws = scratch(aq, lyc_int8_matmul_workspace_bytes(M, N, K, code), "int8_matmul");
   check_rc(lyc_int8_matmul(a.const_data_ptr<int8_t>(), a.stride(0), fa.const_data_ptr<float>(), b.const_data_ptr<int8_t>(), b.stride(0),
-                           fb.const_data_ptr<float>(), dptr(bi), bias_f32(bi), nullptr, y.mutable_data_ptr(), M, N, K, code, stream_of(aq)), "int8_matmul");
+                           fb.const_data_ptr<float>(), dptr(bi), bias_f32(bi), nullptr, y.mutable_data_ptr(), mptr(ws), M, N, K, code, stream_of(aq)), "int8_matmul");
   return y;
 }
 Tensor int8_matmul_meta(const Tensor& aq, const Tensor& sa, const Tensor& bq, const Tensor& sb, const OptTensor& bias, at::ScalarType dtype) {
@@ -173,7 +182,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& wq, const Tensor& sw, const Op
   Tensor y = at::empty(with_last(x, N), x.options());
   Tensor ws = scratch(x, lyc_int8_linear_workspace_bytes(M, N, K, code, 0), "int8_linear");
   check_rc(lyc_int8_linear_fwd(r.const_data_ptr(), w.const_data_ptr<int8_t>(), w.stride(0), s.const_data_ptr<float>(), dptr(bi), bias_f32(bi), dptr(ba),
-                               y.mutable_data_ptr(), ws.mutable_data_ptr(), M, N, K, code, stream_of(x)), "int8_linear");
+                               y.mutable_data_ptr(), mptr(ws), M, N, K, code, stream_of(x)), "int8_linear");
   return y;
 }
 Tensor int8_linear_meta(const Tensor& x, const Tensor& wq, const Tensor& sw, const OptTensor& bias, const OptTensor& base) {
@@ -190,7 +199,7 @@ Tensor int8_linear_bwd(const Tensor& g, const Tensor& wq, const Tensor& sw) {
   Tensor dx = at::empty(with_last(g, K), g.options());
   Tensor ws = scratch(g, lyc_int8_linear_workspace_bytes(M, N, K, code, 1), "int8_linear backward");
   check_rc(lyc_int8_linear_bwd(r.const_data_ptr(), w.const_data_ptr<int8_t>(), w.stride(0), s.const_data_ptr<float>(), dx.mutable_data_ptr(),
-                               ws.mutable_data_ptr(), M, N, K, code, stream_of(g)), "int8_linear backward");
+                               mptr(ws), M, N, K, code, stream_of(g)), "int8_linear backward");
   return dx;
 }
 Tensor int8_linear_bwd_meta(const Tensor& g, const Tensor& wq, const Tensor& sw) { return at::empty(with_last(g, wq.size(1)), g.options()); }
@@ -203,7 +212,7 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
     ctx->save_for_backward({wq, sw});  // not x: the layer is frozen
     ctx->saved_data["dt"] = (int64_t)x.scalar_type();
     ctx->saved_data["base"] = edge(base, 3 + has(bias));
-    return op.call(x, wq, sw, bias, base);
+    return eager(x) ? int8_linear(x, wq, sw, bias, base) : op.call(x, wq, sw, bias, base);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("int8_linear");
@@ -213,7 +222,7 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::_int8_linear_backward", "")
                          .typed<Tensor(const Tensor&, const Tensor&, const Tensor&)>();
     Tensor g = grads[0].to((at::ScalarType)ctx->saved_data["dt"].toInt());
-    if (ctx->needs_input_grad(0)) out[0] = op.call(g, s[0], s[1]);
+    if (ctx->needs_input_grad(0)) out[0] = eager(g) ? int8_linear_bwd(g, s[0], s[1]) : op.call(g, s[0], s[1]);
     if (wanted(ctx, "base")) out[4] = g;
     return out;
   }
@@ -222,6 +231,10 @@ bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return has(t) && t->requires_grad(); }
 Tensor int8_linear_autograd(const Tensor& x, const Tensor& wq, const Tensor& sw, const OptTensor& bias, const OptTensor& base) {
   TORCH_CHECK(!wants(sw) && !wants(bias), "int8_linear: the layer is frozen, its scale and bias cannot require a gradient");
+  if (eager(x) && !(c10::GradMode::is_enabled() && (wants(x) || wants(base)))) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return int8_linear(x, wq, sw, bias, base);
+  }
   return Int8LinearFn::apply(x, wq, sw, bias, base);
 }
 
@@ -272,7 +285,7 @@ std::tuple<Tensor, Tensor> gated_fwd(const Tensor& x, const Tensor& w, const Opt
   Tensor h = at::empty(with_last(x, F), x.options()), pre = pre_of(x, keep ? M : 0, 2 * F);
   Tensor ws = scratch(x, lyc_gated_linear_workspace_bytes(M, I, F, code, a.sw ? LYC_GATED_INT8 : 0), "gated_linear");
   check_rc(lyc_gated_linear_fwd(r.const_data_ptr(), a.w.const_data_ptr(), a.ldw, a.sw, dptr(bi), bias_f32(bi), dptr(ba), h.mutable_data_ptr(),
-                                keep ? pre.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), M, I, F, (int)act, gate_first, code, stream_of(x)),
+                                keep ? pre.mutable_data_ptr() : nullptr, mptr(ws), M, I, F, (int)act, gate_first, code, stream_of(x)),
            "gated_linear");
   return {h, pre};
 }
@@ -318,7 +331,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& g, const
   auto p = [](bool want, const Tensor& t) { return want ? t.mutable_data_ptr() : nullptr; };
   check_rc(lyc_gated_linear_bwd(gr.const_data_ptr(), pre.const_data_ptr(), dw ? xr.const_data_ptr() : nullptr, a.w.const_data_ptr(), a.ldw, a.sw,
                                 p(dbase, std::get<0>(out)), p(dx, std::get<1>(out)), p(dw, std::get<2>(out)), p(dbias, std::get<3>(out)),
-                                ws.mutable_data_ptr(), M, I, F, (int)act, gate_first, code, stream_of(g)), "gated_linear backward");
+                                mptr(ws), M, I, F, (int)act, gate_first, code, stream_of(g)), "gated_linear backward");
   return out;
 }
 
@@ -328,7 +341,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::_gated_linear_forward", "")
                          .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool)>();
-    auto [h, pre] = op.call(x, w, sw, bias, base, act, gate_first);
+    auto [h, pre] = eager(x) ? gated_forward(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
     // x is read by dw alone
     ctx->save_for_backward({pre, w.requires_grad() ? x : Tensor(), w, has(sw) ? *sw : Tensor()});
     ctx->saved_data["bias"] = edge(bias, 2 + has(sw));
@@ -351,7 +364,10 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     if (!(dx || dw || dbias || dbase)) return out;
     OptTensor sw = opt(s[3]);
     Tensor g = grads[0].to((at::ScalarType)ctx->saved_data["dt"].toInt());
-    auto [b, x, w, bi] = op.call(g, s[0], s[1].defined() ? s[1] : g, s[2], sw, ctx->saved_data["act"].toInt(), ctx->saved_data["gf"].toBool(), dbase, dx, dw, dbias);
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool gf = ctx->saved_data["gf"].toBool();
+    const Tensor& xs = s[1].defined() ? s[1] : g;
+    auto [b, x, w, bi] = eager(g) ? gated_backward(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias) : op.call(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias);
     if (dx) out[0] = x;
     if (dw) out[1] = w;
     if (dbias) out[3] = bi.to((at::ScalarType)ctx->saved_data["bdt"].toInt());
@@ -365,7 +381,7 @@ Tensor gated_linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& 
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::gated_linear", "")
                          .typed<Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool)>();
-    return op.call(x, w, sw, bias, base, act, gate_first);
+    return eager(x) ? gated_linear(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
   }
   return GatedLinearFn::apply(x, w, sw, bias, base, act, gate_first);
 }

@@ -184,16 +184,16 @@ __global__ __launch_bounds__(256) void fz_stage_kernel(const TI* __restrict__ x,
 // One pass over g and p writes what the rest of the backward pass reads: dp (rounded to the activation type: a gradient, and the operand of
 // dw and dx), dps = sw f[0] dp (one rounding; dx over an 8-bit weight whose plane is its integers, [M, up(2 F, 8)]), and the column sums of
 // dp before rounding, as one partial row per workgroup row (fixed order: the same bits every time).
-// A workgroup takes DG_COLS columns of each half and DG_ROWS rows; a thread 8 columns of every 8th row.
-constexpr int DG_COLS = 256, DG_ROWS = 64;
+// A workgroup takes DG_COLS columns of each half and `rows` rows; a thread 8 columns of every 8th row.
+constexpr int DG_COLS = 256;
 template <typename T, typename E>
 __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const void* __restrict__ pre, T* __restrict__ dp, E* __restrict__ dps,
                                                        const float* __restrict__ sw, const float* __restrict__ f, float* __restrict__ part, int64_t M, int F,
-                                                       int act, int gate_first, int vec) {
+                                                       int act, int gate_first, int vec, int rows) {
   __shared__ float sums[2][DG_COLS];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int k = blockIdx.x * DG_COLS + tx * 8;
-  const int64_t m0 = (int64_t)blockIdx.y * DG_ROWS;
+  const int64_t m0 = (int64_t)blockIdx.y * rows;
   const int vo = gate_first ? F : 0, go = gate_first ? 0 : F;
   const bool full = vec && k + 8 <= F;
   const int64_t N = 2 * (int64_t)F, lds = (N + 7) & ~7;
@@ -208,7 +208,8 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
     for (int e = 0; e < 8; ++e) sv[e] *= scale, st[e] *= scale;
   }
   if (k < F) {
-    for (int r = ty; r < DG_ROWS && m0 + r < M; r += 8) {
+#pragma unroll 2
+    for (int r = ty; r < rows && m0 + r < M; r += 8) {
       const int64_t m = m0 + r;
       float gv[8], v[8], t[8], dv[8], dt[8];
       fz_load8<T>(g, m * F + k, k, F, full, gv);
@@ -257,8 +258,10 @@ __global__ __launch_bounds__(256) void fz_join_kernel(const float* __restrict__ 
   __shared__ float red[8][32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, n = blockIdx.x * 32 + tx;
   float s = 0.f;
-  if (n < N)
+  if (n < N) {
+#pragma unroll 8
     for (int64_t r = ty; r < parts; r += 8) s += part[r * N + n];
+  }
   red[ty][tx] = s;
   __syncthreads();
   if (ty || n >= N) return;

@@ -91,9 +91,9 @@ def test_c_abi_refuses_before_any_launch():
            ("lyc_int8_quantize", (None, 8, p, 16, p, 2, 8, bf, None), "null"), ("lyc_int8_quantize", (p, 4, p, 16, p, 2, 8, bf, None), "pitch of x"),
            ("lyc_int8_quantize", (p, 8, p, 24, p, 2, 8, bf, None), "multiple of 16"), ("lyc_int8_quantize", (p, 8, p + 8, 16, p, 2, 8, bf, None), "aligned"),
            ("lyc_int8_quantize", (p, 1 << 18, p, 1 << 18, p, 2, 1 << 18, bf, None), "exceed"),
-           ("lyc_int8_matmul", (p, 16, p, p, 8, p, None, 0, None, p, 2, 3, 8, bf, None), "multiple of 16"),
-           ("lyc_int8_matmul", (p, 16, None, p, 16, p, None, 0, None, p, 2, 3, 8, bf, None), "null"),
-           ("lyc_int8_linear_fwd", (p, p, 16, p, None, 0, None, p, None, 2, 3, 8, bf, None), "workspace"),
+           ("lyc_int8_matmul", (p, 16, p, p, 8, p, None, 0, None, p, p, 2, 3, 8, bf, None), "multiple of 16"),
+           ("lyc_int8_matmul", (p, 16, None, p, 16, p, None, 0, None, p, p, 2, 3, 8, bf, None), "null"),
+           ("lyc_int8_linear_fwd", (p, p, 16, p, None, 0, None, p, None, 64, 3, 8, bf, None), "workspace"),
            ("lyc_int8_linear_fwd", (p, p, 16, p, None, 0, None, p, p, -1, 3, 8, bf, None), "bad dims"),
            ("lyc_int8_linear_bwd", (p + 2, p, 16, p, p, p, 2, 3, 8, bf, None), "aligned"),
            ("lyc_gated_linear_fwd", (p, p, 0, None, None, 0, None, p, None, p, 2, 8, 0, 0, 0, bf, None), "bad dims"),
@@ -108,7 +108,7 @@ def test_c_abi_refuses_before_any_launch():
             N.call(name, *args)
     lib = N.load()
     assert lib.lyc_int8_linear_workspace_bytes(4, 8, 0, bf, 0) == -1 and lib.lyc_gated_linear_workspace_bytes(4, 8, 0, bf, 0) == -1
-    assert lib.lyc_int8_linear_workspace_bytes(4, 8, 20, bf, 0) >= 4 * 32 + 16
+    assert lib.lyc_int8_linear_workspace_bytes(64, 8, 20, bf, 0) >= 64 * 32 + 256 and lib.lyc_int8_linear_workspace_bytes(4, 8, 20, bf, 0) == 0
     assert lib.lyc_gated_linear_workspace_bytes(4, 64, 8, bf, 0) == 0  # nothing to stage
     for name in ("lyc_int8_quantize", ):  # nothing to do is no error
         N.call(name, None, 8, None, 16, None, 0, 8, bf, None)
