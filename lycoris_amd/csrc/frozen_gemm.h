@@ -283,42 +283,34 @@ __device__ __forceinline__ void fz_bias8(const FzEpi& ep, int64_t at, int n, int
   if (ep.bias_f32) fz_load8<float>(ep.bias, at, n, N, vec, v);
   else fz_load8<T>(ep.bias, at, n, N, vec, v);
 }
-// p for the backward pass: fp32 as it is; 16-bit types keep 24 bits of the fp32 value (sign, exponent, 15 bits: off by 2^-17), as a plane of
-// its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p alone would cost the gradients as much as their own rounding
-// does twice over.  total: elements of p
+// p for the backward pass: fp32 as it is; 16-bit types keep the upper 24 bits of the fp32 value (sign, exponent, 15 bits: off by less than
+// 2^-15, infinities and NaNs stay what they are), as a plane of its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p
+// alone would cost the gradients as much as their own rounding does.  total: elements of p
+__device__ __forceinline__ void fz_split24(const float (&v)[8], u32x4& hi, u32x2& lo) {
+  unsigned u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[e]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) hi[e] = __builtin_amdgcn_perm(u[2 * e + 1], u[2 * e], 0x07060302u);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned x = __builtin_amdgcn_perm(u[4 * e + 1], u[4 * e], 0x0c0c0501u), y = __builtin_amdgcn_perm(u[4 * e + 3], u[4 * e + 2], 0x0c0c0501u);
+    lo[e] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+  }
+}
 template <typename TO>
-__device__ __forceinline__ void fz_store_pre8(void* pre, int64_t total, int64_t at, int n, int N, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void fz_store_pre8(void* pre, int64_t total, int64_t at, int n, int N, const float (&v)[8]) {
   if constexpr (sizeof(TO) == 4) {
-    fz_store8<float>(pre, at, n, N, vec, v);
+    fz_store8<float>(pre, at, n, N, false, v);
   } else {
     uint16_t* hi = static_cast<uint16_t*>(pre) + at;
     uint8_t* lo = reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(pre) + total) + at;
-    unsigned u[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned b = __float_as_uint(v[e]);
-      u[e] = (b & 0x7f800000u) == 0x7f800000u ? b : b + 0x80u;
-    }
-    if (vec) {
-      u32x4 h;
-      u32x2 l;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = __builtin_amdgcn_perm(u[2 * e + 1], u[2 * e], 0x07060302u);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned x = __builtin_amdgcn_perm(u[4 * e + 1], u[4 * e], 0x0c0c0501u), y = __builtin_amdgcn_perm(u[4 * e + 3], u[4 * e + 2], 0x0c0c0501u);
-        l[e] = x | (y << 16);
+    for (int e = 0; e < 8; ++e)
+      if (n + e < N) {
+        hi[e] = (uint16_t)(__float_as_uint(v[e]) >> 16);
+        lo[e] = (uint8_t)(__float_as_uint(v[e]) >> 8);
       }
-      *reinterpret_cast<u32x4*>(hi) = h;
-      *reinterpret_cast<u32x2*>(lo) = l;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (n + e < N) {
-          hi[e] = (uint16_t)(u[e] >> 16);
-          lo[e] = (uint8_t)(u[e] >> 8);
-        }
-    }
   }
 }
 template <typename TO>
@@ -537,86 +529,165 @@ struct FzKernel {
       }
     }
 
-    // ---- epilogue: acc[mi][2 q + e] of lane (li, g) is row 16 mi + li, columns 32 q + 8 g + 4 e .. + 3 of the wave's part ----------
+    // ---- epilogue: acc[mi][2 q + e] of lane (li, g) is row 16 mi + li, columns 32 q + 8 g + 4 e .. + 3 of the wave's part.  It is vector
+    //      work that the matrix pipe waits for with one workgroup a CU (a 256 x 256 tile of 4 operations an element: 2 us), so addresses
+    //      are 32-bit offsets into descriptors of the tile's rows: rows beyond M lie beyond them, columns beyond NO are masked ------------
     constexpr int NQ = GATED ? NI / 4 : NI / 2;
-    const bool pitch8 = (NO & 7) == 0;
-    const bool vo = pitch8 && fz_al16(ep.out) && (!GATED || (fz_al16(ep.pre) && fz_al16(ep.base))) && fz_al16(ep.base);
-    const bool vb = pitch8 && fz_al16(ep.bias), vs = pitch8 && fz_al16(ep.sw);
     const float alpha = EPI == FZ_PLAIN && ep.alpha ? *ep.alpha : 1.f;
+    const bool vec = (NO & 7) == 0 && fz_al16(ep.out) && fz_al16(ep.base) && fz_al16(ep.pre) && fz_al16(ep.bias) && fz_al16(ep.sw);
+    const int col0 = wc * (BNO / WC) + 8 * g, row0 = wr * (BM / WR) + li;
+    float sa[MI];
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int n = n0 + wc * (BNO / WC) + 32 * q + 8 * g;
-      const bool nok = n < NO, full = n + 8 <= NO;
-      float s1[8], s2[8], c1[8], c2[8];
+    for (int mi = 0; mi < MI; ++mi) sa[mi] = ep.sa && m0 + row0 + 16 * mi < p.M ? ep.sa[m0 + row0 + 16 * mi] : 1.f;
+    // value (or the sum itself) and, GATED, gate of 8 columns: the tile's first half holds the rows that come first in w
+    auto take = [&](int mi, int q, float (&v)[8], float (&t)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s1[e] = s2[e] = 1.f, c1[e] = c2[e] = 0.f;
-      if (nok && EPI != FZ_PLAIN) {
-        if (ep.sw) {
-          fz_load8<float>(ep.sw, vrow + n, n, NO, vs && full, s1);
-          if (GATED) fz_load8<float>(ep.sw, grow + n, n, NO, vs && full, s2);
-        }
-        if (ep.bias) {
-          fz_bias8<TO>(ep, vrow + n, n, NO, vb && full, c1);
-          if (GATED) fz_bias8<TO>(ep, grow + n, n, NO, vb && full, c2);
+      for (int e = 0; e < 8; ++e) {
+        const float a = (float)acc[mi][2 * q + (e >> 2)][e & 3];
+        if constexpr (GATED) {
+          const float b = (float)acc[mi][NI / 2 + 2 * q + (e >> 2)][e & 3];
+          v[e] = ep.gate_first ? b : a;
+          t[e] = ep.gate_first ? a : b;
+        } else {
+          v[e] = a;
         }
       }
+    };
+    auto scale = [&](int mi, const float (&s)[8], const float (&c)[8], float (&v)[8]) {
 #pragma unroll
-      for (int mi = 0; mi < MI; ++mi) {
-        const int m = m0 + wr * (BM / WR) + 16 * mi + li;
-        if (m >= p.M || !nok) continue;
-        float v[8];
-        if constexpr (!GATED) {
+      for (int e = 0; e < 8; ++e) v[e] = FE<E>::SIZE == 1 ? fmaf(v[e] * sa[mi], s[e], c[e]) : v[e] + c[e];
+    };
+    auto columns = [&](int n, bool wide, float (&s1)[8], float (&s2)[8], float (&c1)[8], float (&c2)[8]) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = (float)acc[mi][2 * q + (e >> 2)][e & 3];
-          if constexpr (EPI == FZ_LINEAR) {
-            const float sa = ep.sa[m];
+      for (int e = 0; e < 8; ++e) s1[e] = s2[e] = 1.f, c1[e] = c2[e] = 0.f;
+      if (EPI == FZ_PLAIN || n >= NO) return;
+      if (FE<E>::SIZE == 1) {
+        fz_load8<float>(ep.sw, vrow + n, n, NO, wide, s1);
+        if (GATED) fz_load8<float>(ep.sw, grow + n, n, NO, wide, s2);
+      }
+      if (ep.bias) {
+        fz_bias8<TO>(ep, vrow + n, n, NO, wide, c1);
+        if (GATED) fz_bias8<TO>(ep, grow + n, n, NO, wide, c2);
+      }
+    };
+    if (vec) {
+      constexpr int H = GATED ? 2 : 1, TS = (int)sizeof(TO);
+      const int64_t rows = p.M - m0, prow = m0 + ep.pre_row, prows = ep.pre_total / (2 * (int64_t)NO) - prow;
+      auto open_rows = [&](const void* base, int64_t row, int64_t pitch, int64_t n) {
+        const int64_t bytes = n * pitch;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + row * pitch, 0,
+                                                 (int)(bytes > 0x7fffffff ? 0x7fffffff : bytes), K4_RSRC_FLAGS);
+      };
+      const int po = NO * TS, pb = po * H, ph = NO * (TS == 4 ? 8 : 4), pl = NO * 2;  // pitches: out, base, p and its 8-bit plane
+      const __amdgpu_buffer_rsrc_t ro = open_rows(ep.out, m0, po, rows), rb = open_rows(ep.base, m0, pb, ep.base ? rows : 0);
+      __amdgpu_buffer_rsrc_t rh = ro, rl = ro;
+      if (GATED && ep.pre) {
+        rh = open_rows(ep.pre, prow, ph, rows < prows ? rows : prows);
+        if (TS == 2) rl = open_rows(static_cast<char*>(ep.pre) + 2 * ep.pre_total, prow, pl, rows < prows ? rows : prows);
+      }
+      auto fetch = [&](unsigned off, int col, float (&x)[8]) {
+        TO t[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] * sa * s1[e] + c1[e];
-            if (ep.base) {
-              float bs[8];
-              fz_load8<TO>(ep.base, (int64_t)m * NO + n, n, NO, vo && full, bs);
+        for (int i = 0; i < TS / 2; ++i)
+          reinterpret_cast<u32x4*>(t)[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(off + col * TS + 16 * i), 0, 0));
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] += bs[e];
-            }
-          } else {
+        for (int e = 0; e < 8; ++e) x[e] += (float)t[e];
+      };
+      auto put_pre = [&](unsigned hoff, unsigned loff, int col, const float (&x)[8]) {
+        if constexpr (TS == 4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}), rh,
+                                                   (int)(hoff + col * 4 + 16 * i), 0, 0);
+        } else {
+          u32x4 hi;
+          u32x2 lo;
+          fz_split24(x, hi, lo);
+          __builtin_amdgcn_raw_buffer_store_b128(hi, rh, (int)(hoff + col * 2), 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b64(lo, rl, (int)(loff + col), 0, 0);
+        }
+      };
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int n = n0 + col0 + 32 * q;
+        const bool in = n < NO;
+        float s1[8], s2[8], c1[8], c2[8];
+        columns(n, true, s1, s2, c1, c2);
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+          const int r = row0 + 16 * mi;
+          float v[8], t[8];
+          take(mi, q, v, t);
+          if constexpr (EPI == FZ_PLAIN) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= alpha;
-          }
-          fz_store8<TO>(ep.out, (int64_t)m * NO + n, n, NO, vo && full, v);
-        } else {
-          float t[8];
-          // the tile's first half holds the rows that come first in w: the gate's when gate_first
+          } else {
+            scale(mi, s1, c1, v);
+            if (GATED) scale(mi, s2, c2, t);
+            if (ep.base) {
+              const unsigned off = in ? (unsigned)(r * pb + n * TS) : K4_OOB;
+              fetch(off, vrow, v);
+              if (GATED) fetch(off, grow, t);
+            }
+            if constexpr (GATED) {
+              if (ep.pre) {
+                const unsigned hoff = in ? (unsigned)(r * ph + n * (TS == 4 ? 4 : 2)) : K4_OOB, loff = in ? (unsigned)(r * pl + n) : K4_OOB;
+                put_pre(hoff, loff, vrow, v);
+                put_pre(hoff, loff, grow, t);
+              }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float f = (float)acc[mi][2 * q + (e >> 2)][e & 3], h = (float)acc[mi][NI / 2 + 2 * q + (e >> 2)][e & 3];
-            v[e] = ep.gate_first ? h : f;
-            t[e] = ep.gate_first ? f : h;
+              for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);
+            }
           }
-          const float sa = ep.sa ? ep.sa[m] : 1.f;
+          const unsigned off = in ? (unsigned)(r * po + n * TS) : K4_OOB;
+          TO o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] = v[e] * sa * s1[e] + c1[e];
-            t[e] = t[e] * sa * s2[e] + c2[e];
-          }
-          const int64_t row = (int64_t)m * 2 * NO;
-          if (ep.base) {
-            float bs[8];
-            fz_load8<TO>(ep.base, row + vrow + n, n, NO, vo && full, bs);
+          for (int e = 0; e < 8; ++e) o[e] = (TO)v[e];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += bs[e];
-            fz_load8<TO>(ep.base, row + grow + n, n, NO, vo && full, bs);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] += bs[e];
-          }
-          if (ep.pre) {
-            const int64_t prow = row + ep.pre_row * 2 * NO;
-            fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + vrow + n, n, NO, vo && full, v);
-            fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + grow + n, n, NO, vo && full, t);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);
-          fz_store8<TO>(ep.out, (int64_t)m * NO + n, n, NO, vo && full, v);
+          for (int i = 0; i < TS / 2; ++i) __builtin_amdgcn_raw_buffer_store_b128(reinterpret_cast<u32x4*>(o)[i], ro, (int)(off + 16 * i), 0, 0);
         }
+      }
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int n = n0 + col0 + 32 * q;
+      float s1[8], s2[8], c1[8], c2[8], x[8];
+      columns(n, false, s1, s2, c1, c2);
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) {
+        const int64_t m = m0 + row0 + 16 * mi;
+        if (m >= p.M || n >= NO) continue;
+        float v[8], t[8];
+        take(mi, q, v, t);
+        if constexpr (EPI == FZ_PLAIN) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= alpha;
+        } else {
+          scale(mi, s1, c1, v);
+          if (GATED) scale(mi, s2, c2, t);
+          const int64_t row = m * (GATED ? 2 : 1) * NO;
+          if (ep.base) {
+            fz_load8<TO>(ep.base, row + vrow + n, n, NO, false, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += x[e];
+            if (GATED) {
+              fz_load8<TO>(ep.base, row + grow + n, n, NO, false, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) t[e] += x[e];
+            }
+          }
+          if constexpr (GATED) {
+            if (ep.pre) {
+              const int64_t prow = row + ep.pre_row * 2 * NO;
+              fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + vrow + n, n, NO, v);
+              fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + grow + n, n, NO, t);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);
+          }
+        }
+        fz_store8<TO>(ep.out, m * NO + n, n, NO, false, v);
       }
     }
   }

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(W * 64) void fz_skinny_kernel(const TI* __restrict_
       if (ep.base) v[h] += (float)static_cast<const TO*>(ep.base)[(int64_t)m * H * NO + at];
       if (GATED && ep.pre) {
         float one[8] = {v[h]};
-        fz_store_pre8<TO>(ep.pre, ep.pre_total, (int64_t)m * 2 * NO + at, NO - 1, NO, false, one);
+        fz_store_pre8<TO>(ep.pre, ep.pre_total, (int64_t)m * 2 * NO + at, NO - 1, NO, one);
       }
     }
     float y = v[0];
