@@ -69,62 +69,76 @@ int allow_lds(Kern kern, int bytes) {
 
 int grid_of(int64_t chunks) { return (int)(cdiv(chunks, 256) < 16384 ? cdiv(chunks, 256) : 16384); }
 
-template <typename K, int BM, int BNO>
+template <typename K, int BM>
 int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
-  const int per = fz_per_xcd(cdiv(p.M, BM) * cdiv(K::GATED ? ep.F : p.N, BNO));
+  const int per = fz_per_xcd(cdiv(p.M, BM) * cdiv(K::GATED ? ep.F : p.N, K::BNO));
   FZ_TRY(allow_lds(&fz_gemm_kernel<K>, K::LDS));
   hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * per), p.ksplit > 1 ? p.ksplit : 1), dim3(K::NW * 64), K::LDS, st, p, ep);
   return check_launch("fz_gemm");
 }
 
-// Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.  Tiles of 256 x 256 (one
-// workgroup a CU), 128 x 128 (two) or 64 x 64 (three); where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those
-// over the rows that fill whole rounds and 128 x 128 ones over the rest; where the tiles are few and K is long, K in parts.
+// Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.
+//   256 x 256, 256 x 160, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (three of 4 waves; gated: 64 x 128);
+//   where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those over the rows that fill whole rounds and
+//   128 x 128 ones over the rest; where the tiles are few and K is long, K in parts.
+// The tiles of 160 columns are there for outputs of 320, 640 and 1280 channels, which they cut into as many tiles as CUs: 4096 x 1280 are 256
+// of 128 x 160 (dx with K = 10240: 103 us, against 156 with 128 x 128 and 182 with 256 x 256), 16384 x 1280 are 512 of 256 x 160 (8-bit, K =
+// 5120: 123 us, against 151 and 149).  With whole rounds of the larger tile that wins (dx 16384 x 5120, K = 1280: 181 us, against 239 and 242).
 // The rule compares estimates in microseconds: a round costs what a step costs times the steps, plus what a tile's beginning and end leave
 // exposed -- of its epilogue's bytes, at a CU's share of HBM, all with one workgroup a CU, half of it where a second one computes meanwhile.
 struct Plan {
-  int tile = 128, ksplit = 1;
-  int64_t whole = 0;  // row tiles of 256 ahead of the 128s
+  int tile = 128, ksplit = 1;  // tile: 64, 128, 160 (128 x 160), 256, 416 (256 x 160)
+  int64_t whole = 0;           // row tiles of 256 ahead of the 128s
   double us = 1e30;
 };
 struct Rate {
   double step, tile, shown;
 };
-constexpr Rate R256{0.72, 4.0, 1.0}, R128_2{0.48, 2.5, 0.5}, R128_1{0.30, 3.0, 1.0}, R64_3{0.36, 2.0, 0.35}, R64_2{0.26, 2.0, 0.5}, R64_1{0.18, 2.5, 1.0};
+struct Tile {
+  int id, bm, bn, wgs;
+  Rate rate[3];  // with 1, 2, 3 workgroups on the CU
+};
+constexpr Tile TILES[] = {{128, 128, 128, 2, {{0.30, 3.0, 1.0}, {0.62, 2.5, 0.5}}},
+                          {64, 64, 64, 3, {{0.18, 2.5, 1.0}, {0.26, 2.0, 0.5}, {0.36, 2.0, 0.35}}},
+                          {160, 128, 160, 1, {{0.31, 3.0, 1.0}}},
+                          {416, 256, 160, 1, {{0.58, 4.0, 1.0}}},
+                          {256, 256, 256, 1, {{0.76, 5.0, 1.0}}}};
 constexpr double CU_BYTES_PER_US = 19900.0;
-double rounds_cost(int64_t tiles, int wgs, const Rate* by_load, double steps, double bytes) {
-  const int64_t per = fz_per_xcd(tiles), slots = 32 * wgs, full = per / slots, rest = per % slots;
-  auto one = [&](int load) { return by_load[load - 1].step * steps + by_load[load - 1].tile + by_load[load - 1].shown * load * bytes / CU_BYTES_PER_US; };
-  return (double)full * one(wgs) + (rest ? one((int)cdiv(rest, 32)) : 0.0);
+double rounds_cost(int64_t tiles, const Tile& t, double steps, double bytes) {
+  const int64_t per = fz_per_xcd(tiles), slots = 32 * t.wgs, full = per / slots, rest = per % slots;
+  auto one = [&](int load) { return t.rate[load - 1].step * steps + t.rate[load - 1].tile + t.rate[load - 1].shown * load * bytes / CU_BYTES_PER_US; };
+  return (double)full * one(t.wgs) + (rest ? one((int)cdiv(rest, 32)) : 0.0);
 }
-// eb: bytes the epilogue moves per output; split: may K be split
-Plan plan_gemm(int64_t M, int64_t NO, double steps, bool gated, double eb, bool split) {
-  static constexpr Rate r256[] = {R256}, r128[] = {R128_1, R128_2}, r64[] = {R64_1, R64_2, R64_3};
+// eb: bytes the epilogue moves per output
+Plan plan_gemm(int64_t M, int64_t NO, double steps, bool gated, double eb) {
   const int o = gated ? 2 : 1;
-  auto cost = [&](int tile, int64_t rows, double st, double e, int parts) {
-    const int64_t tn = cdiv(NO, tile == 64 ? 64 : tile / o), tiles = cdiv(rows, tile) * tn * parts;
-    const double out = tile == 64 ? 64.0 * 64.0 : (double)tile * tile / o;
-    if (tile == 256) return rounds_cost(tiles, 1, r256, st, out * e);
-    if (tile == 128) return rounds_cost(tiles, 2, r128, st, out * e);
-    return rounds_cost(tiles, 3, r64, gated ? 1.4 * st : st, out * e);
+  auto cost = [&](const Tile& t, int64_t rows, double st, double e, int parts) {
+    const int bno = t.id == 64 ? 64 : t.bn / o;
+    Tile u = t;
+    if (gated)  // the activation's vector work, and 64 x 64 outputs take 128 rows of w
+      for (Rate& r : u.rate) {
+        r.tile += t.id == 256 ? 4.0 : t.id == 128 ? 1.0 : 2.0;
+        if (t.id == 64) r.step *= 2.0;
+      }
+    return rounds_cost(cdiv(rows, t.bm) * cdiv(NO, bno) * parts, u, st, (double)t.bm * bno * e);
   };
   Plan best;
   auto offer = [&](int tile, int ks, int64_t whole, double us) {
     if (us < best.us) best = Plan{tile, ks, whole, us};
   };
-  for (int tile : {128, 64, 256}) {
-    offer(tile, 1, 0, cost(tile, M, steps, eb, 1));
-    if (!split) continue;
-    for (int ks = 2; ks <= 8 && steps / ks >= 12; ++ks)  // the sums are written, read and finished by a second launch
-      offer(tile, ks, 0, cost(tile, M, cdiv((int64_t)steps, ks), 4.0, ks) + 3.0 + (double)M * NO * (4.0 * ks + eb) / (256 * CU_BYTES_PER_US));
+  for (const Tile& t : TILES) {
+    if (gated && (t.id == 160 || t.id == 416)) continue;
+    offer(t.id, 1, 0, cost(t, M, steps, eb, 1));
+    for (int ks = 2; !gated && ks <= 8 && steps / ks >= 12; ++ks)  // the sums are written, read and finished by a second launch
+      offer(t.id, ks, 0, cost(t, M, cdiv((int64_t)steps, ks), 4.0, ks) + 3.0 + (double)M * NO * (4.0 * ks + eb) / (256 * CU_BYTES_PER_US));
   }
   const int64_t tn = cdiv(NO, 256 / o), tm = cdiv(M, 256), whole = tm * tn / 256 * 256 / tn;
-  if (whole > 0 && whole < tm) offer(128, 1, whole, cost(256, whole * 256, steps, eb, 1) + cost(128, M - whole * 256, steps, eb, 1) + 1.0);
+  if (whole > 0 && whole < tm) offer(128, 1, whole, cost(TILES[4], whole * 256, steps, eb, 1) + cost(TILES[0], M - whole * 256, steps, eb, 1) + 4.0);
   return best;
 }
 template <typename E, int EPI>
 Plan plan_of(int64_t M, int64_t NO, int64_t K, int nseg, double eb) {
-  return plan_gemm(M, NO, (double)cdiv(K * FE<E>::SIZE, 64) * nseg, EPI == FZ_GATED, eb, EPI != FZ_GATED);
+  return plan_gemm(M, NO, (double)cdiv(K * FE<E>::SIZE, 64) * nseg, EPI == FZ_GATED, eb);
 }
 // bytes of a plan's partial sums
 int64_t part_bytes(const Plan& pl, int64_t M, int64_t N) { return pl.ksplit > 1 ? pl.ksplit * M * N * 4 : 0; }
@@ -150,19 +164,29 @@ int launch_gemm(const Plan& pl, FzProb p, FzEpi ep, void* part, hipStream_t st) 
     if (ep.sa) e.sa = ep.sa + m;
     if (ep.base) e.base = static_cast<const TO*>(ep.base) + m * NO * O;
     e.pre_row = ep.pre_row + m;  // (p's two planes are addressed by row)
-    FZ_TRY((launch_tile<K256, 256, 256 / O>(a, ep, st)));
-    return launch_tile<K128, 128, 128 / O>(b, e, st);
+    FZ_TRY((launch_tile<K256, 256>(a, ep, st)));
+    return launch_tile<K128, 128>(b, e, st);
   }
-  if (pl.tile == 64) FZ_TRY((launch_tile<K64, 64, 64>(p, ep, st)));
-  else if (pl.tile == 128) FZ_TRY((launch_tile<K128, 128, 128 / O>(p, ep, st)));
-  else FZ_TRY((launch_tile<K256, 256, 256 / O>(p, ep, st)));
   if constexpr (!G) {
-    if (p.ksplit > 1) {
-      hipLaunchKernelGGL((fz_reduce_kernel<E, TO>), dim3(grid_of((int64_t)p.M * cdiv(p.N, 8))), dim3(256), 0, st, p, ep);
-      return check_launch("fz_reduce");
+    using K160 = FzKernel<E, TO, 128, 160, 4, 2, 6, A_KS, B_KS, EPI>;
+    using K416 = FzKernel<E, TO, 256, 160, 4, 2, 5, A_KS, B_KS, EPI>;
+    switch (pl.tile) {
+      case 64: FZ_TRY((launch_tile<K64, 64>(p, ep, st))); break;
+      case 128: FZ_TRY((launch_tile<K128, 128>(p, ep, st))); break;
+      case 160: FZ_TRY((launch_tile<K160, 128>(p, ep, st))); break;
+      case 416: FZ_TRY((launch_tile<K416, 256>(p, ep, st))); break;
+      default: FZ_TRY((launch_tile<K256, 256>(p, ep, st)));
+    }
+    if (p.ksplit == 1) return LYC_OK;
+    hipLaunchKernelGGL((fz_reduce_kernel<E, TO>), dim3(grid_of((int64_t)p.M * cdiv(p.N, 8))), dim3(256), 0, st, p, ep);
+    return check_launch("fz_reduce");
+  } else {
+    switch (pl.tile) {
+      case 64: return launch_tile<K64, 64>(p, ep, st);
+      case 128: return launch_tile<K128, 128>(p, ep, st);
+      default: return launch_tile<K256, 256>(p, ep, st);
     }
   }
-  return LYC_OK;
 }
 
 // up to 32 rows: frozen_skinny.h.  x: the activations when the kernel quantises them itself, else null

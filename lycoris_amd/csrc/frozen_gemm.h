@@ -126,18 +126,22 @@ struct FzEpi {
 };
 
 // One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A K step is 64 bytes of K: one MFMA deep.
-//   ROWS: tile extent; W: waves along it; NW: waves in all; KS: K-strided in memory; PAIRED: the n operand (paired tile order)
+//   ROWS: tile extent; W: waves along it; NW: waves in all; KS: K-strided in memory; PAIRED: the n operand (paired tile order; with an odd
+//   number of 16-row tiles a wave, as in 160 rows over two waves, the last one is in natural order)
 // K-contiguous: LDS rows of 64 bytes, their four 16-byte chunks XOR-permuted on the DMA's source address -- by bits 2, 3 of the row in
 // natural order, 3, 4 in paired order -- so that the 16 rows of a fragment read fall on the 16 slots of a 256-byte bank row.
 // K-strided (16-bit): the image in memory order, read transposed (gemm16d.h).
 template <int ROWS, int W, int NW, bool KS, bool PAIRED, bool GATED>
 struct FzOperand {
-  static constexpr int PIECES = ROWS / 16, PPW = PIECES / NW;  // 1 KiB DMA pieces of a K step
-  static constexpr int WEXT = ROWS / W, NT = WEXT / 16;
-  static constexpr int CH = ROWS / 8, PITCH = ROWS * 2;  // KS: chunks and bytes per k row
-  static constexpr int NADDR = KS ? (PAIRED ? NT / 2 : NT) : 1;
-  static constexpr int SLOT = ROWS * 64;
-  static_assert(PIECES % NW == 0 && (!PAIRED || NT % 2 == 0) && (!GATED || (PAIRED && !KS && NT % 4 == 0)), "tile shape");
+  static constexpr int LROWS = KS && ROWS > 128 ? 256 : ROWS;  // KS: LDS rows of a power of two of bytes (the permutation is an XOR)
+  static constexpr int PIECES = LROWS / 16, PPW = (PIECES + NW - 1) / NW;  // 1 KiB DMA pieces of a K step; a wave without one fetches nothing
+  static constexpr bool SPARE = PIECES % NW != 0;                          // ... into a spare piece of LDS: every wave's count is the same
+  static constexpr int WEXT = ROWS / W, NT = WEXT / 16, NP = NT / 2;
+  static constexpr bool ODD = PAIRED && NT % 2 != 0;
+  static constexpr int CH = LROWS / 8, PITCH = LROWS * 2;  // KS: chunks and bytes per k row
+  static constexpr int NADDR = KS ? (PAIRED ? NP + ODD : NT) : 1 + ODD;
+  static constexpr int SLOT = LROWS * 64;
+  static_assert(WEXT % 16 == 0 && (!GATED || (PAIRED && !KS && NT % 4 == 0 && !SPARE)), "tile shape");
 
   static constexpr unsigned BAD = 0xc0000000u;  // a lane whose row or column lies outside the operand; bit 31 alone: outside this step
   unsigned voff[PPW], rd[NADDR];
@@ -170,10 +174,14 @@ struct FzOperand {
         const int r = piece_row(j);
         // GATED: rows 0 .. BN / 2 are the half whose first row is `base`, the others the half `second` rows further on
         const int gr = !GATED || r < ROWS / 2 ? r : second + r - ROWS / 2;
-        voff[j] = r0 + gr < ext ? (unsigned)gr * (unsigned)ld + (unsigned)piece_chunk(j) * 16u : BAD;
+        voff[j] = r0 + gr < ext && (!SPARE || r < ROWS) ? (unsigned)gr * (unsigned)ld + (unsigned)piece_chunk(j) * 16u : BAD;
       }
       const int r = wsel * (GATED ? WEXT / 2 : WEXT) + (PAIRED ? 8 * (li >> 2) + (li & 3) : li);
       rd[0] = (unsigned)(stage_off + r * 64 + ((g ^ swz(r)) << 4));
+      if constexpr (ODD) {
+        const int o = wsel * WEXT + 32 * NP + li;
+        rd[1] = (unsigned)(stage_off + o * 64 + ((g ^ swz(o)) << 4));
+      }
     } else {
       org = static_cast<const char*>(base) + (int64_t)r0 * 2;
       kstep = 32u * (unsigned)ld;
@@ -181,12 +189,12 @@ struct FzOperand {
 #pragma unroll
       for (int j = 0; j < PPW; ++j) {
         const int c = piece_chunk(j);
-        voff[j] = r0 + 8 * c < ext ? (unsigned)piece_row(j) * (unsigned)ld + (unsigned)c * 16u : BAD;
+        voff[j] = r0 + 8 * c < ext && 8 * c < ROWS && (!SPARE || piece_row(j) < 32) ? (unsigned)piece_row(j) * (unsigned)ld + (unsigned)c * 16u : BAD;
       }
       const int rho = li >> 2, quad = li & 3, x = g16d_swz_ks<PAIRED, CH>(rho), krow = 8 * g + rho;
 #pragma unroll
       for (int t = 0; t < NADDR; ++t) {
-        const int col = wsel * WEXT + (PAIRED ? 32 * t + 8 * quad : 16 * t + 4 * quad);
+        const int col = wsel * WEXT + (!PAIRED ? 16 * t + 4 * quad : ODD && t == NP ? 32 * NP + 4 * quad : 32 * t + 8 * quad);
         rd[t] = (unsigned)(stage_off + krow * PITCH + (((col >> 3) ^ x) << 4) + (col & 7) * 2);
       }
     }
@@ -208,14 +216,18 @@ struct FzOperand {
     cur += kstep;
   }
   template <int J>
-  __device__ __forceinline__ void issue_piece(char* slot_of_wave) const {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)(slot_of_wave + NW * J * 1024), 16, (int)voff[J], 0, 0, 0);
+  __device__ __forceinline__ void issue_piece(char* slot_of_wave, char* spare) const {
+    char* dst = slot_of_wave + NW * J * 1024;
+    if constexpr (SPARE && (J + 1) * NW > PIECES) {
+      if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) + NW * J >= PIECES) dst = spare;
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)dst, 16, (int)voff[J], 0, 0, 0);
   }
   template <int... J>
-  __device__ __forceinline__ void issue(char* slot_of_wave, std::integer_sequence<int, J...>) const {
-    (issue_piece<J>(slot_of_wave), ...);
+  __device__ __forceinline__ void issue(char* slot_of_wave, char* spare, std::integer_sequence<int, J...>) const {
+    (issue_piece<J>(slot_of_wave, spare), ...);
   }
-  __device__ __forceinline__ void issue(char* slot_of_wave) const { issue(slot_of_wave, std::make_integer_sequence<int, PPW>{}); }
+  __device__ __forceinline__ void issue(char* slot_of_wave, char* spare) const { issue(slot_of_wave, spare, std::make_integer_sequence<int, PPW>{}); }
 
   static constexpr int NRAW = KS ? 2 * NT : NT;
   using RawT = typename std::conditional<KS, u32x2, u32x4>::type;
@@ -230,7 +242,8 @@ struct FzOperand {
   template <int I>
   __device__ __forceinline__ void read(unsigned sb, RawT (&f)[NRAW]) const {
     if constexpr (!KS) {
-      f[I] = g16d_read128(sb + rd[0], kc_off(I));
+      if constexpr (ODD && I == NT - 1) f[I] = g16d_read128(sb + rd[1], 0);
+      else f[I] = g16d_read128(sb + rd[0], kc_off(I));
     } else {
       constexpr int TI = I / 2;
       f[I] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], (PAIRED ? (TI & 1) * 8 : 0) + (I & 1) * 4 * PITCH);
@@ -246,21 +259,26 @@ struct FzOperand {
   }
 };
 
-// 8 consecutive entries of a row vector (out of range: 0)
-template <typename T>
-__device__ __forceinline__ void fz_load8(const void* p, int64_t at, int n, int N, bool vec, float (&v)[8]) {
+// CN (4 or 8) consecutive entries of a row vector (out of range: 0)
+template <typename T, int CN>
+__device__ __forceinline__ void fz_load(const void* p, int64_t at, int n, int N, bool vec, float (&v)[CN]) {
   const T* src = static_cast<const T*>(p) + at;
   if (vec) {
-    T t[8];
-    constexpr int Q = (int)sizeof(T) * 8 / 16;
+    using V = typename std::conditional<sizeof(T) * CN == 8, u32x2, u32x4>::type;
+    T t[CN];
+    constexpr int Q = (int)(sizeof(T) * CN / sizeof(V));
 #pragma unroll
-    for (int q = 0; q < Q; ++q) reinterpret_cast<u32x4*>(t)[q] = reinterpret_cast<const u32x4*>(src)[q];
+    for (int q = 0; q < Q; ++q) reinterpret_cast<V*>(t)[q] = reinterpret_cast<const V*>(src)[q];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+    for (int e = 0; e < CN; ++e) v[e] = (float)t[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = n + e < N ? (float)src[e] : 0.f;
+    for (int e = 0; e < CN; ++e) v[e] = n + e < N ? (float)src[e] : 0.f;
   }
+}
+template <typename T>
+__device__ __forceinline__ void fz_load8(const void* p, int64_t at, int n, int N, bool vec, float (&v)[8]) {
+  fz_load<T, 8>(p, at, n, N, vec, v);
 }
 template <typename T>
 __device__ __forceinline__ void fz_store8(void* p, int64_t at, int n, int N, bool vec, const float (&v)[8]) {
@@ -278,10 +296,10 @@ __device__ __forceinline__ void fz_store8(void* p, int64_t at, int n, int N, boo
       if (n + e < N) dst[e] = (T)v[e];
   }
 }
-template <typename T>
-__device__ __forceinline__ void fz_bias8(const FzEpi& ep, int64_t at, int n, int N, bool vec, float (&v)[8]) {
-  if (ep.bias_f32) fz_load8<float>(ep.bias, at, n, N, vec, v);
-  else fz_load8<T>(ep.bias, at, n, N, vec, v);
+template <typename T, int CN>
+__device__ __forceinline__ void fz_bias(const FzEpi& ep, int64_t at, int n, int N, bool vec, float (&v)[CN]) {
+  if (ep.bias_f32) fz_load<float, CN>(ep.bias, at, n, N, vec, v);
+  else fz_load<T, CN>(ep.bias, at, n, N, vec, v);
 }
 // p for the backward pass: fp32 as it is; 16-bit types keep the upper 24 bits of the fp32 value (sign, exponent, 15 bits: off by less than
 // 2^-15, infinities and NaNs stay what they are), as a plane of its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p
@@ -357,15 +375,15 @@ constexpr int fz_share(int q, int n, int over) { return over < 1 || q >= over ? 
 // E: operand type; TO: type of out / base / pre; BM x BN tile, waves WR x WC; D: ring slots
 template <typename E, typename TO, int BM, int BN, int WR, int WC, int D, bool A_KS, bool B_KS, int EPI>
 struct FzKernel {
-  static constexpr int NW = WR * WC, STAGE = (BM + BN) * 64, LDS = D * STAGE;
+  static constexpr int NW = WR * WC, BNO = EPI == FZ_GATED ? BN / 2 : BN;  // BNO: output columns of a tile
   static constexpr bool GATED = EPI == FZ_GATED;
   using OA = FzOperand<BM, WR, NW, A_KS, false, false>;
   using OB = FzOperand<BN, WC, NW, B_KS, true, GATED>;
+  static constexpr int STAGE = OA::SLOT + OB::SLOT, LDS = D * STAGE + (OA::SPARE || OB::SPARE ? 1024 : 0);
   static constexpr int MI = OA::NT, NI = OB::NT, C = OA::PPW + OB::PPW;
   static_assert(D >= 4 && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
 
   static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b, int z) {
-    constexpr int BNO = GATED ? BN / 2 : BN;  // output columns of a tile
     const int NO = GATED ? ep.F : p.N;
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (NO + BNO - 1) / BNO;
     int tm, tn;
@@ -427,11 +445,11 @@ struct FzKernel {
       oa.open(records);
       ob.open(records);
     };
-    char* const wslot = smem + wave * 1024;  // this wave's first DMA piece of slot 0
+    char *const wslot = smem + wave * 1024, *const spare = smem + D * STAGE;  // this wave's first DMA piece of slot 0
     for (int s = 0; s < D - 1; ++s) {
       open();
-      oa.issue(wslot + s * STAGE);
-      ob.issue(wslot + s * STAGE + OA::SLOT);
+      oa.issue(wslot + s * STAGE, spare);
+      ob.issue(wslot + s * STAGE + OA::SLOT, spare);
     }
 
     using Acc = typename FE<E>::acc;
@@ -484,8 +502,8 @@ struct FzKernel {
                         std::make_integer_sequence<int, r1 - r0>{});
           g16d_for_each([&](auto ic) {
             constexpr int P = d0 + decltype(ic)::value;
-            if constexpr (P < OA::PPW) oa.template issue_piece<P>(fill);
-            else ob.template issue_piece<P - OA::PPW>(fill + OA::SLOT);
+            if constexpr (P < OA::PPW) oa.template issue_piece<P>(fill, spare);
+            else ob.template issue_piece<P - OA::PPW>(fill + OA::SLOT, spare);
           }, std::make_integer_sequence<int, d1 - d0>{});
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -513,7 +531,7 @@ struct FzKernel {
           const int m = m0 + wr * (BM / WR) + 16 * mi + li;
 #pragma unroll
           for (int ni = 0; ni < NI; ++ni) {
-            const int n = n0 + wc * (BN / WC) + 32 * (ni >> 1) + 8 * g + 4 * (ni & 1);
+            const int n = n0 + wc * (BN / WC) + (OB::ODD && ni == NI - 1 ? 16 * ni + 4 * g : 32 * (ni >> 1) + 8 * g + 4 * (ni & 1));
             if (m >= p.M || n >= p.N) continue;
             char* at = part + ((int64_t)m * p.N + n) * 4;
             if (v4) {
@@ -529,167 +547,154 @@ struct FzKernel {
       }
     }
 
-    // ---- epilogue: acc[mi][2 q + e] of lane (li, g) is row 16 mi + li, columns 32 q + 8 g + 4 e .. + 3 of the wave's part.  It is vector
-    //      work that the matrix pipe waits for with one workgroup a CU (a 256 x 256 tile of 4 operations an element: 2 us), so addresses
-    //      are 32-bit offsets into descriptors of the tile's rows: rows beyond M lie beyond them, columns beyond NO are masked ------------
-    constexpr int NQ = GATED ? NI / 4 : NI / 2;
+    // ---- epilogue: acc[mi][2 q + e] of lane (li, g) is row 16 mi + li, columns 32 q + 8 g + 4 e .. + 3 of the wave's part; an odd last
+    //      tile is columns 16 ni + 4 g .. + 3.  It is vector work that the matrix pipe waits for with one workgroup a CU, so addresses
+    //      are 32-bit offsets into descriptors of the tile's rows: rows beyond M lie beyond them, columns beyond NO are masked.
+    //      Measured on 256 x 256 tiles: 4 us with two scales and no more, 8 us with the gelu of 128 columns; a workgroup's beginning,
+    //      before its first step's operands have landed, is 1.3 - 2 us --------------------------------------------------------------
+    constexpr int TS = (int)sizeof(TO), H = GATED ? 2 : 1;
     const float alpha = EPI == FZ_PLAIN && ep.alpha ? *ep.alpha : 1.f;
     const bool vec = (NO & 7) == 0 && fz_al16(ep.out) && fz_al16(ep.base) && fz_al16(ep.pre) && fz_al16(ep.bias) && fz_al16(ep.sw);
-    const int col0 = wc * (BNO / WC) + 8 * g, row0 = wr * (BM / WR) + li;
+    const int row0 = wr * (BM / WR) + li, colw = n0 + wc * (BNO / WC);
     float sa[MI];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) sa[mi] = ep.sa && m0 + row0 + 16 * mi < p.M ? ep.sa[m0 + row0 + 16 * mi] : 1.f;
-    // value (or the sum itself) and, GATED, gate of 8 columns: the tile's first half holds the rows that come first in w
-    auto take = [&](int mi, int q, float (&v)[8], float (&t)[8]) {
+
+    const int64_t rows = p.M - m0, prow = m0 + ep.pre_row;
+    auto open_rows = [&](const void* base, int64_t row, int64_t pitch, bool have) {
+      const int64_t bytes = have ? rows * pitch : 0;
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + row * pitch, 0,
+                                               (int)(bytes > 0x7fffffff ? 0x7fffffff : bytes), K4_RSRC_FLAGS);
+    };
+    const int po = NO * TS, pb = po * H, ph = NO * (TS == 4 ? 8 : 4), pl = NO * 2;  // pitches: out, base, p and its 8-bit plane
+    const __amdgpu_buffer_rsrc_t ro = open_rows(ep.out, m0, po, true), rb = open_rows(ep.base, m0, pb, ep.base != nullptr);
+    const __amdgpu_buffer_rsrc_t rh = open_rows(ep.pre, prow, ph, GATED && ep.pre),
+                                 rl = open_rows(static_cast<char*>(ep.pre) + 2 * ep.pre_total, prow, pl, GATED && ep.pre && TS == 2);
+
+    // CN columns from n on, of every row tile; get(mi, e, half): their sums
+    auto emit = [&](auto cn, int n, auto get) {
+      constexpr int CN = decltype(cn)::value;
+      const bool in = n < NO;
+      float s1[CN], s2[CN], c1[CN], c2[CN];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = (float)acc[mi][2 * q + (e >> 2)][e & 3];
+      for (int e = 0; e < CN; ++e) s1[e] = s2[e] = 1.f, c1[e] = c2[e] = 0.f;
+      if (EPI != FZ_PLAIN && in) {
+        if (FE<E>::SIZE == 1) {
+          fz_load<float, CN>(ep.sw, vrow + n, n, NO, vec, s1);
+          if (GATED) fz_load<float, CN>(ep.sw, grow + n, n, NO, vec, s2);
+        }
+        if (ep.bias) {
+          fz_bias<TO, CN>(ep, vrow + n, n, NO, vec, c1);
+          if (GATED) fz_bias<TO, CN>(ep, grow + n, n, NO, vec, c2);
+        }
+      }
+      auto fetch = [&](const __amdgpu_buffer_rsrc_t& r, unsigned off, float (&x)[CN]) {  // adds
+        TO t[CN];
+        if constexpr (TS * CN == 8) {
+          reinterpret_cast<u32x2*>(t)[0] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+        } else {
+#pragma unroll
+          for (int i = 0; i < TS * CN / 16; ++i)
+            reinterpret_cast<u32x4*>(t)[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, 0));
+        }
+#pragma unroll
+        for (int e = 0; e < CN; ++e) x[e] += (float)t[e];
+      };
+      auto store = [&](const __amdgpu_buffer_rsrc_t& r, unsigned off, const float (&x)[CN]) {
+        TO t[CN];
+#pragma unroll
+        for (int e = 0; e < CN; ++e) t[e] = (TO)x[e];
+        if constexpr (TS * CN == 8) {
+          __builtin_amdgcn_raw_buffer_store_b64(reinterpret_cast<u32x2*>(t)[0], r, (int)off, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < TS * CN / 16; ++i) __builtin_amdgcn_raw_buffer_store_b128(reinterpret_cast<u32x4*>(t)[i], r, (int)(off + 16 * i), 0, 0);
+        }
+      };
+      auto keep = [&](unsigned hoff, unsigned loff, int col, const float (&x)[CN]) {  // p for the backward pass
         if constexpr (GATED) {
-          const float b = (float)acc[mi][NI / 2 + 2 * q + (e >> 2)][e & 3];
-          v[e] = ep.gate_first ? b : a;
-          t[e] = ep.gate_first ? a : b;
-        } else {
-          v[e] = a;
-        }
-      }
-    };
-    auto scale = [&](int mi, const float (&s)[8], const float (&c)[8], float (&v)[8]) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = FE<E>::SIZE == 1 ? fmaf(v[e] * sa[mi], s[e], c[e]) : v[e] + c[e];
-    };
-    auto columns = [&](int n, bool wide, float (&s1)[8], float (&s2)[8], float (&c1)[8], float (&c2)[8]) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s1[e] = s2[e] = 1.f, c1[e] = c2[e] = 0.f;
-      if (EPI == FZ_PLAIN || n >= NO) return;
-      if (FE<E>::SIZE == 1) {
-        fz_load8<float>(ep.sw, vrow + n, n, NO, wide, s1);
-        if (GATED) fz_load8<float>(ep.sw, grow + n, n, NO, wide, s2);
-      }
-      if (ep.bias) {
-        fz_bias8<TO>(ep, vrow + n, n, NO, wide, c1);
-        if (GATED) fz_bias8<TO>(ep, grow + n, n, NO, wide, c2);
-      }
-    };
-    if (vec) {
-      constexpr int H = GATED ? 2 : 1, TS = (int)sizeof(TO);
-      const int64_t rows = p.M - m0, prow = m0 + ep.pre_row, prows = ep.pre_total / (2 * (int64_t)NO) - prow;
-      auto open_rows = [&](const void* base, int64_t row, int64_t pitch, int64_t n) {
-        const int64_t bytes = n * pitch;
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + row * pitch, 0,
-                                                 (int)(bytes > 0x7fffffff ? 0x7fffffff : bytes), K4_RSRC_FLAGS);
-      };
-      const int po = NO * TS, pb = po * H, ph = NO * (TS == 4 ? 8 : 4), pl = NO * 2;  // pitches: out, base, p and its 8-bit plane
-      const __amdgpu_buffer_rsrc_t ro = open_rows(ep.out, m0, po, rows), rb = open_rows(ep.base, m0, pb, ep.base ? rows : 0);
-      __amdgpu_buffer_rsrc_t rh = ro, rl = ro;
-      if (GATED && ep.pre) {
-        rh = open_rows(ep.pre, prow, ph, rows < prows ? rows : prows);
-        if (TS == 2) rl = open_rows(static_cast<char*>(ep.pre) + 2 * ep.pre_total, prow, pl, rows < prows ? rows : prows);
-      }
-      auto fetch = [&](unsigned off, int col, float (&x)[8]) {
-        TO t[8];
-#pragma unroll
-        for (int i = 0; i < TS / 2; ++i)
-          reinterpret_cast<u32x4*>(t)[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(off + col * TS + 16 * i), 0, 0));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += (float)t[e];
-      };
-      auto put_pre = [&](unsigned hoff, unsigned loff, int col, const float (&x)[8]) {
-        if constexpr (TS == 4) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}), rh,
-                                                   (int)(hoff + col * 4 + 16 * i), 0, 0);
-        } else {
-          u32x4 hi;
-          u32x2 lo;
-          fz_split24(x, hi, lo);
-          __builtin_amdgcn_raw_buffer_store_b128(hi, rh, (int)(hoff + col * 2), 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b64(lo, rl, (int)(loff + col), 0, 0);
-        }
-      };
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int n = n0 + col0 + 32 * q;
-        const bool in = n < NO;
-        float s1[8], s2[8], c1[8], c2[8];
-        columns(n, true, s1, s2, c1, c2);
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-          const int r = row0 + 16 * mi;
-          float v[8], t[8];
-          take(mi, q, v, t);
-          if constexpr (EPI == FZ_PLAIN) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= alpha;
+          if constexpr (TS == 4) {
+            store(rh, hoff + col * 4, x);
           } else {
-            scale(mi, s1, c1, v);
-            if (GATED) scale(mi, s2, c2, t);
-            if (ep.base) {
-              const unsigned off = in ? (unsigned)(r * pb + n * TS) : K4_OOB;
-              fetch(off, vrow, v);
-              if (GATED) fetch(off, grow, t);
-            }
-            if constexpr (GATED) {
-              if (ep.pre) {
-                const unsigned hoff = in ? (unsigned)(r * ph + n * (TS == 4 ? 4 : 2)) : K4_OOB, loff = in ? (unsigned)(r * pl + n) : K4_OOB;
-                put_pre(hoff, loff, vrow, v);
-                put_pre(hoff, loff, grow, t);
-              }
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);
-            }
+            u32x4 hi;
+            u32x2 lo;
+            fz_split24(x, hi, lo);
+            __builtin_amdgcn_raw_buffer_store_b128(hi, rh, (int)(hoff + col * 2), 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b64(lo, rl, (int)(loff + col), 0, 0);
           }
-          const unsigned off = in ? (unsigned)(r * po + n * TS) : K4_OOB;
-          TO o[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = (TO)v[e];
-#pragma unroll
-          for (int i = 0; i < TS / 2; ++i) __builtin_amdgcn_raw_buffer_store_b128(reinterpret_cast<u32x4*>(o)[i], ro, (int)(off + 16 * i), 0, 0);
         }
-      }
-      return;
-    }
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int n = n0 + col0 + 32 * q;
-      float s1[8], s2[8], c1[8], c2[8], x[8];
-      columns(n, false, s1, s2, c1, c2);
+      };
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) {
-        const int64_t m = m0 + row0 + 16 * mi;
-        if (m >= p.M || n >= NO) continue;
-        float v[8], t[8];
-        take(mi, q, v, t);
+        const int r = row0 + 16 * mi;
+        const int64_t m = m0 + r;
+        if (!vec && (m >= p.M || !in)) continue;
+        float v[CN], t[CN];
+#pragma unroll
+        for (int e = 0; e < CN; ++e) {
+          const float a = (float)get(mi, e, 0), b = GATED ? (float)get(mi, e, 1) : 0.f;
+          v[e] = GATED && ep.gate_first ? b : a;  // the tile's first half holds the rows that come first in w
+          t[e] = ep.gate_first ? a : b;
+        }
         if constexpr (EPI == FZ_PLAIN) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= alpha;
+          for (int e = 0; e < CN; ++e) v[e] *= alpha;
         } else {
-          scale(mi, s1, c1, v);
-          if (GATED) scale(mi, s2, c2, t);
-          const int64_t row = m * (GATED ? 2 : 1) * NO;
+#pragma unroll
+          for (int e = 0; e < CN; ++e) {
+            v[e] = FE<E>::SIZE == 1 ? fmaf(v[e] * sa[mi], s1[e], c1[e]) : v[e] + c1[e];
+            if (GATED) t[e] = FE<E>::SIZE == 1 ? fmaf(t[e] * sa[mi], s2[e], c2[e]) : t[e] + c2[e];
+          }
           if (ep.base) {
-            fz_load8<TO>(ep.base, row + vrow + n, n, NO, false, x);
+            if (vec) {
+              const unsigned off = in ? (unsigned)(r * pb + n * TS) : K4_OOB;
+              fetch(rb, off + vrow * TS, v);
+              if (GATED) fetch(rb, off + grow * TS, t);
+            } else {
+              float x[CN];
+              fz_load<TO, CN>(ep.base, m * H * NO + vrow + n, n, NO, false, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += x[e];
-            if (GATED) {
-              fz_load8<TO>(ep.base, row + grow + n, n, NO, false, x);
+              for (int e = 0; e < CN; ++e) v[e] += x[e];
+              if (GATED) {
+                fz_load<TO, CN>(ep.base, m * H * NO + grow + n, n, NO, false, x);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) t[e] += x[e];
+                for (int e = 0; e < CN; ++e) t[e] += x[e];
+              }
             }
           }
           if constexpr (GATED) {
             if (ep.pre) {
-              const int64_t prow = row + ep.pre_row * 2 * NO;
-              fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + vrow + n, n, NO, v);
-              fz_store_pre8<TO>(ep.pre, ep.pre_total, prow + grow + n, n, NO, t);
+              if (vec) {
+                const unsigned hoff = in ? (unsigned)(r * ph + n * (TS == 4 ? 4 : 2)) : K4_OOB, loff = in ? (unsigned)(r * pl + n) : K4_OOB;
+                keep(hoff, loff, vrow, v);
+                keep(hoff, loff, grow, t);
+              } else {
+                const int64_t at = (m + ep.pre_row) * 2 * NO;
+                fz_store_pre8<TO>(ep.pre, ep.pre_total, at + vrow + n, n, NO, v);
+                fz_store_pre8<TO>(ep.pre, ep.pre_total, at + grow + n, n, NO, t);
+              }
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= fz_act(ep.act, t[e]);
+            for (int e = 0; e < CN; ++e) v[e] *= fz_act(ep.act, t[e]);
           }
         }
-        fz_store8<TO>(ep.out, m * NO + n, n, NO, false, v);
+        if (vec) {
+          store(ro, in ? (unsigned)(r * po + n * TS) : K4_OOB, v);
+        } else {
+          TO* dst = static_cast<TO*>(ep.out) + m * NO + n;
+#pragma unroll
+          for (int e = 0; e < CN; ++e)
+            if (n + e < NO) dst[e] = (TO)v[e];
+        }
       }
-    }
+    };
+    constexpr int NQ = GATED ? NI / 4 : NI / 2;
+    g16d_for_each([&](auto qc) {
+      constexpr int Q = decltype(qc)::value;
+      emit(std::integral_constant<int, 8>{}, colw + 32 * Q + 8 * g, [&](int mi, int e, int half) { return acc[mi][half * (NI / 2) + 2 * Q + (e >> 2)][e & 3]; });
+    }, std::make_integer_sequence<int, NQ>{});
+    if constexpr (OB::ODD)
+      emit(std::integral_constant<int, 4>{}, colw + 16 * (NI - 1) + 4 * g, [&](int mi, int e, int) { return acc[mi][NI - 1][e]; });
   }
 };
 
@@ -738,7 +743,7 @@ __global__ __launch_bounds__(256) void fz_reduce_kernel(FzProb p, FzEpi ep) {
       for (int e = 0; e < 8; ++e) v[e] = v[e] * sa * t[e];
     }
     if (ep.bias) {
-      fz_bias8<TO>(ep, n, n, N, vb, t);
+      fz_bias<TO, 8>(ep, n, n, N, vb, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += t[e];
     }
