@@ -78,17 +78,16 @@ int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
 }
 
 // Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.
-//   256 x 256, 256 x 160, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (three of 4 waves; gated: 64 x 128);
-//   where the 256 x 256 tiles would leave a mostly empty last round of the 256 CUs, those over the rows that fill whole rounds and
-//   128 x 128 ones over the rest; where the tiles are few and K is long, K in parts.
-// The tiles of 160 columns are there for outputs of 320, 640 and 1280 channels, which they cut into as many tiles as CUs: 4096 x 1280 are 256
-// of 128 x 160 (dx with K = 10240: 103 us, against 156 with 128 x 128 and 182 with 256 x 256), 16384 x 1280 are 512 of 256 x 160 (8-bit, K =
-// 5120: 123 us, against 151 and 149).  With whole rounds of the larger tile that wins (dx 16384 x 5120, K = 1280: 181 us, against 239 and 242).
-// The rule compares estimates in microseconds: a round costs what a step costs times the steps, plus what a tile's beginning and end leave
-// exposed -- of its epilogue's bytes, at a CU's share of HBM, all with one workgroup a CU, half of it where a second one computes meanwhile.
+//   256 x 256, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (three of 4 waves; gated: 64 x 128); where the tiles are few
+//   and K is long, K in parts whose sums a second launch joins.
+// The tile of 160 columns is there for outputs of 320, 640 and 1280 channels, which it cuts into as many tiles as CUs: 4096 x 1280 are 256 (dx
+// with K = 10240, inputs out of HBM: 117 us, against 161 with 128 x 128 and 256 with 256 x 256); with whole rounds of the larger tile that wins
+// (dx 16384 x 5120, K = 1280: 213 us, against 240 with 128 x 128 and 289 with 128 x 160).
+// The rule compares estimates in microseconds, from sweeps of 30 shapes with inputs out of HBM: a round costs what a step costs times the
+// steps, plus what a tile's beginning and end leave exposed -- of its epilogue's bytes, at a CU's share of HBM, less where a second
+// workgroup computes meanwhile.
 struct Plan {
-  int tile = 128, ksplit = 1;  // tile: 64, 128, 160 (128 x 160), 256, 416 (256 x 160)
-  int64_t whole = 0;           // row tiles of 256 ahead of the 128s
+  int tile = 128, ksplit = 1;  // tile: 64, 128, 160 (128 x 160), 256
   double us = 1e30;
 };
 struct Rate {
@@ -98,11 +97,10 @@ struct Tile {
   int id, bm, bn, wgs;
   Rate rate[3];  // with 1, 2, 3 workgroups on the CU
 };
-constexpr Tile TILES[] = {{128, 128, 128, 2, {{0.30, 3.0, 1.0}, {0.62, 2.5, 0.5}}},
+constexpr Tile TILES[] = {{128, 128, 128, 2, {{0.30, 3.0, 1.0}, {0.54, 2.5, 0.5}}},
                           {64, 64, 64, 3, {{0.18, 2.5, 1.0}, {0.26, 2.0, 0.5}, {0.36, 2.0, 0.35}}},
-                          {160, 128, 160, 1, {{0.31, 3.0, 1.0}}},
-                          {416, 256, 160, 1, {{0.58, 4.0, 1.0}}},
-                          {256, 256, 256, 1, {{0.76, 5.0, 1.0}}}};
+                          {160, 128, 160, 1, {{0.35, 3.5, 1.0}}},
+                          {256, 256, 256, 1, {{0.73, 5.0, 0.7}}}};
 constexpr double CU_BYTES_PER_US = 19900.0;
 double rounds_cost(int64_t tiles, const Tile& t, double steps, double bytes) {
   const int64_t per = fz_per_xcd(tiles), slots = 32 * t.wgs, full = per / slots, rest = per % slots;
@@ -111,29 +109,24 @@ double rounds_cost(int64_t tiles, const Tile& t, double steps, double bytes) {
 }
 // eb: bytes the epilogue moves per output
 Plan plan_gemm(int64_t M, int64_t NO, double steps, bool gated, double eb) {
-  const int o = gated ? 2 : 1;
-  auto cost = [&](const Tile& t, int64_t rows, double st, double e, int parts) {
-    const int bno = t.id == 64 ? 64 : t.bn / o;
+  Plan best;
+  for (const Tile& t : TILES) {
+    if (gated && t.id == 160) continue;
     Tile u = t;
+    const int bno = !gated || t.id == 64 ? t.bn : t.bn / 2;
     if (gated)  // the activation's vector work, and 64 x 64 outputs take 128 rows of w
       for (Rate& r : u.rate) {
         r.tile += t.id == 256 ? 4.0 : t.id == 128 ? 1.0 : 2.0;
         if (t.id == 64) r.step *= 2.0;
       }
-    return rounds_cost(cdiv(rows, t.bm) * cdiv(NO, bno) * parts, u, st, (double)t.bm * bno * e);
-  };
-  Plan best;
-  auto offer = [&](int tile, int ks, int64_t whole, double us) {
-    if (us < best.us) best = Plan{tile, ks, whole, us};
-  };
-  for (const Tile& t : TILES) {
-    if (gated && (t.id == 160 || t.id == 416)) continue;
-    offer(t.id, 1, 0, cost(t, M, steps, eb, 1));
-    for (int ks = 2; !gated && ks <= 8 && steps / ks >= 12; ++ks)  // the sums are written, read and finished by a second launch
-      offer(t.id, ks, 0, cost(t, M, cdiv((int64_t)steps, ks), 4.0, ks) + 3.0 + (double)M * NO * (4.0 * ks + eb) / (256 * CU_BYTES_PER_US));
+    const int64_t tiles = cdiv(M, t.bm) * cdiv(NO, bno);
+    const double area = (double)t.bm * bno;
+    for (int ks = 1; ks == 1 || (!gated && ks <= 8 && steps / ks >= 12); ++ks) {
+      double us = rounds_cost(tiles * ks, u, ks == 1 ? steps : cdiv((int64_t)steps, ks), area * (ks == 1 ? eb : 4.0));
+      if (ks > 1) us += 4.0 + (double)M * NO * (4.0 * ks + eb) / (256 * CU_BYTES_PER_US);
+      if (us < best.us) best = Plan{t.id, ks, us};
+    }
   }
-  const int64_t tn = cdiv(NO, 256 / o), tm = cdiv(M, 256), whole = tm * tn / 256 * 256 / tn;
-  if (whole > 0 && whole < tm) offer(128, 1, whole, cost(TILES[4], whole * 256, steps, eb, 1) + cost(TILES[0], M - whole * 256, steps, eb, 1) + 4.0);
   return best;
 }
 template <typename E, int EPI>
@@ -146,47 +139,29 @@ int64_t part_bytes(const Plan& pl, int64_t M, int64_t N) { return pl.ksplit > 1 
 template <typename E, typename TO, bool A_KS, bool B_KS, int EPI>
 int launch_gemm(const Plan& pl, FzProb p, FzEpi ep, void* part, hipStream_t st) {
   constexpr bool G = EPI == FZ_GATED;
-  constexpr int O = G ? 2 : 1;  // B rows an output column takes
-  using K256 = FzKernel<E, TO, 256, 256, 2, 4, 5, A_KS, B_KS, EPI>;
-  using K128 = FzKernel<E, TO, 128, 128, 4, 2, 5, A_KS, B_KS, EPI>;
-  using K64 = FzKernel<E, TO, 64, 64 * O, 2, 2, 6, A_KS, B_KS, EPI>;
-  const int64_t NO = G ? ep.F : p.N;
+  // ring slots of 128 bytes of K (cold inputs), but 64 where neither operand's rows lie along K: 128 x 128 dw 5120 x 640, K = 8192: 101 us
+  // against 123, 256 x 256 dw 10240 x 1280, K = 4096: 104 against 110
+  constexpr int SB = A_KS && B_KS ? 64 : 128, D = A_KS && B_KS ? 5 : 2;
+  using K256 = FzKernel<E, TO, 256, 256, 2, 4, SB, D, A_KS, B_KS, EPI>;
+  using K128 = FzKernel<E, TO, 128, 128, 4, 2, SB, D, A_KS, B_KS, EPI>;
+  using K64 = FzKernel<E, TO, 64, G ? 128 : 64, 2, 2, 128, 3, A_KS, B_KS, EPI>;
   p.ksplit = pl.ksplit;
   ep.part = part;
-  if (pl.whole) {
-    const int64_t m = pl.whole * 256;
-    FzProb a = p, b = p;
-    a.M = (int)m;
-    b.M = (int)(p.M - m);
-    b.A = static_cast<const char*>(p.A) + (A_KS ? 2 * m : m * p.lda);
-    FzEpi e = ep;
-    e.out = static_cast<TO*>(ep.out) + m * NO;
-    if (ep.sa) e.sa = ep.sa + m;
-    if (ep.base) e.base = static_cast<const TO*>(ep.base) + m * NO * O;
-    e.pre_row = ep.pre_row + m;  // (p's two planes are addressed by row)
-    FZ_TRY((launch_tile<K256, 256>(a, ep, st)));
-    return launch_tile<K128, 128>(b, e, st);
+  switch (pl.tile) {
+    case 64: FZ_TRY((launch_tile<K64, 64>(p, ep, st))); break;
+    case 128: FZ_TRY((launch_tile<K128, 128>(p, ep, st))); break;
+    case 160:
+      if constexpr (!G) FZ_TRY((launch_tile<FzKernel<E, TO, 128, 160, 4, 2, 128, 4, A_KS, B_KS, EPI>, 128>(p, ep, st)));
+      break;
+    default: FZ_TRY((launch_tile<K256, 256>(p, ep, st)));
   }
   if constexpr (!G) {
-    using K160 = FzKernel<E, TO, 128, 160, 4, 2, 6, A_KS, B_KS, EPI>;
-    using K416 = FzKernel<E, TO, 256, 160, 4, 2, 5, A_KS, B_KS, EPI>;
-    switch (pl.tile) {
-      case 64: FZ_TRY((launch_tile<K64, 64>(p, ep, st))); break;
-      case 128: FZ_TRY((launch_tile<K128, 128>(p, ep, st))); break;
-      case 160: FZ_TRY((launch_tile<K160, 128>(p, ep, st))); break;
-      case 416: FZ_TRY((launch_tile<K416, 256>(p, ep, st))); break;
-      default: FZ_TRY((launch_tile<K256, 256>(p, ep, st)));
-    }
-    if (p.ksplit == 1) return LYC_OK;
-    hipLaunchKernelGGL((fz_reduce_kernel<E, TO>), dim3(grid_of((int64_t)p.M * cdiv(p.N, 8))), dim3(256), 0, st, p, ep);
-    return check_launch("fz_reduce");
-  } else {
-    switch (pl.tile) {
-      case 64: return launch_tile<K64, 64>(p, ep, st);
-      case 128: return launch_tile<K128, 128>(p, ep, st);
-      default: return launch_tile<K256, 256>(p, ep, st);
+    if (p.ksplit > 1) {
+      hipLaunchKernelGGL((fz_reduce_kernel<E, TO>), dim3(grid_of((int64_t)p.M * cdiv(p.N, 8))), dim3(256), 0, st, p, ep);
+      return check_launch("fz_reduce");
     }
   }
+  return LYC_OK;
 }
 
 // up to 32 rows: frozen_skinny.h.  x: the activations when the kernel quantises them itself, else null

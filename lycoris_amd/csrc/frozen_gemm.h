@@ -11,11 +11,11 @@
 // v_mfma_f32_16x16x32) run the same loop: a step is 64 bytes of K, a fragment 16 bytes of one row, an MFMA 16 cycles either way.
 //
 // What bounds the loop, measured inside it (256 x 256 tile, 8 waves, cycles per 64-byte step; the MFMAs alone are 1024): 1450 with the
-// descriptor and tail arithmetic of every step in line (~100 scalar instructions between the barrier and the first MFMA), 1250 with it
-// behind a branch that is taken at the end of a segment only, 1205 - 1250 with one barrier per two steps.  The clock then is 1.75 - 1.95
-// GHz: the matrix pipe is near what the card's power allows (1.68 PFLOP/s bf16, 2.7 POP/s int8 inside the loop).  Ring depth beyond what
-// the waits need, LDS bank conflicts (SQ_LDS_BANK_CONFLICT) and L2 order were not what bounded it at 4096 rows; at 8192^3 the order was
-// (tiles in flight on an XCD as a block: 988 -> 872 us).
+// descriptor and tail arithmetic of every step in line (~100 scalar instructions between the barrier and the first MFMA), 1250 with a
+// handful.  The clock then is 1.75 - 1.95 GHz: the matrix pipe is near what the card's power allows (1.68 PFLOP/s bf16, 2.4 - 2.7 POP/s int8
+// inside the loop).  The LDS pipe is a quarter busy and the L2 order matters at 8192^3 only (988 -> 872 us).  On inputs out of HBM the
+// granularity of the DMA counts: with slots of 64 bytes of K every row is asked for in half cache lines, with 128 bytes in whole ones, and a
+// product like dx 8192 x 640 x 5120 takes 64 instead of 76 us (55 with its inputs in the caches).
 //
 //   * the buffer descriptor is rebased on every K step: an operand may be larger than 4 GiB;
 //   * rows, columns and K outside the operand are masked in the DMA's lane offsets, 16 bytes at a time (both operands: 0 times a stray NaN
@@ -121,77 +121,86 @@ struct FzEpi {
   const float *sa, *sw;  // 8-bit: scales of A's rows, of B's rows
   const void* bias;    // [N] (GATED: [2 F]) or null; fp32 when bias_f32, else the output's type
   const void* base;    // [M, N] (GATED: [M, 2 F]) in the output's type, or null
-  int64_t pre_total, pre_row;  // elements of the whole p; its row that this launch's first row is
+  int64_t pre_total;   // elements of p
   int bias_f32, act, gate_first, F;
 };
 
-// One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A K step is 64 bytes of K: one MFMA deep.
+// what the DMA pieces of one operand's K step need
+struct FzStep {
+  __amdgpu_buffer_rsrc_t rs;
+  unsigned mask;
+};
+
+// One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A ring slot holds SB = 64 or 128 bytes of K:
+// one or two MFMA steps.
 //   ROWS: tile extent; W: waves along it; NW: waves in all; KS: K-strided in memory; PAIRED: the n operand (paired tile order; with an odd
 //   number of 16-row tiles a wave, as in 160 rows over two waves, the last one is in natural order)
-// K-contiguous: LDS rows of 64 bytes, their four 16-byte chunks XOR-permuted on the DMA's source address -- by bits 2, 3 of the row in
-// natural order, 3, 4 in paired order -- so that the 16 rows of a fragment read fall on the 16 slots of a 256-byte bank row.
+// K-contiguous: LDS rows of SB bytes, their 16-byte chunks XOR-permuted on the DMA's source address so that a fragment read falls on
+// different slots of the 256-byte bank row.  The hardware serves ds_read_b128 in groups of lanes 0-3, 12-15, 20-27 and so on: with 64-byte
+// rows the permutation is 0 2 3 1 over bits 2, 3 of the row (3, 4 in paired order); 0 1 2 3 cost a conflict on every read.
 // K-strided (16-bit): the image in memory order, read transposed (gemm16d.h).
-template <int ROWS, int W, int NW, bool KS, bool PAIRED, bool GATED>
+template <int ROWS, int W, int NW, int SB, bool KS, bool PAIRED, bool GATED>
 struct FzOperand {
-  static constexpr int LROWS = KS && ROWS > 128 ? 256 : ROWS;  // KS: LDS rows of a power of two of bytes (the permutation is an XOR)
-  static constexpr int PIECES = LROWS / 16, PPW = (PIECES + NW - 1) / NW;  // 1 KiB DMA pieces of a K step; a wave without one fetches nothing
+  static constexpr int PIECES = ROWS * SB / 1024, PPW = (PIECES + NW - 1) / NW;  // 1 KiB DMA pieces of a K step; a wave without one fetches nothing
   static constexpr bool SPARE = PIECES % NW != 0;                          // ... into a spare piece of LDS: every wave's count is the same
   static constexpr int WEXT = ROWS / W, NT = WEXT / 16, NP = NT / 2;
   static constexpr bool ODD = PAIRED && NT % 2 != 0;
-  static constexpr int CH = LROWS / 8, PITCH = LROWS * 2;  // KS: chunks and bytes per k row
-  static constexpr int NADDR = KS ? (PAIRED ? NP + ODD : NT) : 1 + ODD;
-  static constexpr int SLOT = LROWS * 64;
+  static constexpr int CH = ROWS / 8, PITCH = ROWS * 2;  // KS: chunks and bytes per k row
+  static constexpr bool XOR = PITCH % 128 == 0;          // KS: 320-byte rows fall on different banks by themselves
+  static constexpr int HALVES = SB / 64, KROWS = SB / 2;  // MFMA steps a slot; KS: k rows a slot
+  static constexpr int NADDR = KS ? (PAIRED ? NP + ODD : NT) : HALVES * (1 + ODD);
+  static constexpr int SLOT = ROWS * SB;
   static_assert(WEXT % 16 == 0 && (!GATED || (PAIRED && !KS && NT % 4 == 0 && !SPARE)), "tile shape");
 
-  static constexpr unsigned BAD = 0xc0000000u;  // a lane whose row or column lies outside the operand; bit 31 alone: outside this step
-  unsigned voff[PPW], rd[NADDR];
-  const char *org, *cur;  // the tile's first byte in plane 0; the next K step's
-  unsigned kstep, kleft;  // bytes a step advances; K-contiguous: bytes, K-strided: rows, of the last step of a segment
-  __amdgpu_buffer_rsrc_t rs;
-
+  unsigned voff[PPW], rd[NADDR], beyond;  // beyond: K-contiguous: K4_OOB where this lane's chunk lies beyond K in the last step of a segment
+  const char *org, *cur;                  // the tile's first byte in plane 0; the next K step's
+  unsigned kstep, tail_bytes;             // bytes a step advances; K-strided: bytes of the rows that the last step of a segment has
   static __device__ __forceinline__ int swz(int r) {
+    if constexpr (SB == 128) return g16d_swz_kc<PAIRED>(r);
     const int j = (r >> (PAIRED ? 3 : 2)) & 3;
     return ((j << 1) & 3) ^ ((j >> 1) * 3);  // 0 2 3 1
   }
   static __device__ __forceinline__ int piece_row(int j) {  // row (KC) or k row (KS) of this lane in piece j of its wave
     const int wave = (int)(threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-    if constexpr (!KS) return 16 * (wave + NW * j) + (lane >> 2);
-    else return 1024 / PITCH * (wave + NW * j) + lane / CH;
+    if constexpr (!KS) return 1024 / SB * (wave + NW * j) + lane / (SB / 16);
+    else return (64 * (wave + NW * j) + lane) / CH;
   }
   static __device__ __forceinline__ int piece_chunk(int j) {
     const int lane = (int)threadIdx.x & 63;
-    if constexpr (!KS) return (lane & 3) ^ swz(piece_row(j));
-    else return (lane % CH) ^ g16d_swz_ks<PAIRED, CH>(piece_row(j));
+    if constexpr (!KS) return (lane % (SB / 16)) ^ swz(piece_row(j));
+    else return ((64 * (int)((threadIdx.x >> 6) + NW * j) + lane) % CH) ^ (XOR ? g16d_swz_ks<PAIRED, CH>(piece_row(j)) : 0);
   }
   __device__ __forceinline__ void setup(const void* base, int64_t ld, int r0, int ext, int kdim, int kb, int stage_off, int wsel, int second) {
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     if constexpr (!KS) {
       org = static_cast<const char*>(base) + (int64_t)r0 * ld;
-      kstep = 64;
-      kleft = ((kb - 1) & 63) + 1;
+      kstep = SB;
 #pragma unroll
       for (int j = 0; j < PPW; ++j) {
         const int r = piece_row(j);
         // GATED: rows 0 .. BN / 2 are the half whose first row is `base`, the others the half `second` rows further on
         const int gr = !GATED || r < ROWS / 2 ? r : second + r - ROWS / 2;
-        voff[j] = r0 + gr < ext && (!SPARE || r < ROWS) ? (unsigned)gr * (unsigned)ld + (unsigned)piece_chunk(j) * 16u : BAD;
+        voff[j] = r0 + gr < ext && (!SPARE || r < ROWS) ? (unsigned)gr * (unsigned)ld + (unsigned)piece_chunk(j) * 16u : K4_OOB;
       }
+      beyond = (unsigned)piece_chunk(0) * 16u > (unsigned)((kb - 1) & (SB - 1)) ? K4_OOB : 0u;  // (the chunk does not depend on the piece)
       const int r = wsel * (GATED ? WEXT / 2 : WEXT) + (PAIRED ? 8 * (li >> 2) + (li & 3) : li);
-      rd[0] = (unsigned)(stage_off + r * 64 + ((g ^ swz(r)) << 4));
-      if constexpr (ODD) {
-        const int o = wsel * WEXT + 32 * NP + li;
-        rd[1] = (unsigned)(stage_off + o * 64 + ((g ^ swz(o)) << 4));
+      const int o = wsel * WEXT + 32 * NP + li;  // ODD: the last tile's row
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        rd[h] = (unsigned)(stage_off + r * SB + (((4 * h + g) ^ swz(r)) << 4));
+        if constexpr (ODD) rd[HALVES + h] = (unsigned)(stage_off + o * SB + (((4 * h + g) ^ swz(o)) << 4));
       }
     } else {
       org = static_cast<const char*>(base) + (int64_t)r0 * 2;
-      kstep = 32u * (unsigned)ld;
-      kleft = ((kdim - 1) & 31) + 1;
+      kstep = (unsigned)KROWS * (unsigned)ld;
+      tail_bytes = (unsigned)((kdim - 1) & (KROWS - 1)) * (unsigned)ld + (unsigned)(((ext + 7) & ~7) - r0) * 2u;
+      beyond = 0;
 #pragma unroll
       for (int j = 0; j < PPW; ++j) {
         const int c = piece_chunk(j);
-        voff[j] = r0 + 8 * c < ext && 8 * c < ROWS && (!SPARE || piece_row(j) < 32) ? (unsigned)piece_row(j) * (unsigned)ld + (unsigned)c * 16u : BAD;
+        voff[j] = r0 + 8 * c < ext && (!SPARE || piece_row(j) < KROWS) ? (unsigned)piece_row(j) * (unsigned)ld + (unsigned)c * 16u : K4_OOB;
       }
-      const int rho = li >> 2, quad = li & 3, x = g16d_swz_ks<PAIRED, CH>(rho), krow = 8 * g + rho;
+      const int rho = li >> 2, quad = li & 3, x = XOR ? g16d_swz_ks<PAIRED, CH>(rho) : 0, krow = 8 * g + rho;
 #pragma unroll
       for (int t = 0; t < NADDR; ++t) {
         const int col = wsel * WEXT + (!PAIRED ? 16 * t + 4 * quad : ODD && t == NP ? 32 * NP + 4 * quad : 32 * t + 8 * quad);
@@ -200,53 +209,49 @@ struct FzOperand {
     }
   }
   __device__ __forceinline__ void seek(int64_t plane_off) { cur = org + plane_off; }
-  // what lies beyond K in the last step of a segment reads as zero: on for that step, off again behind it
-  __device__ __forceinline__ void tail(bool on) {
-#pragma unroll
-    for (int j = 0; j < PPW; ++j) {
-      const bool out = KS ? (unsigned)piece_row(j) >= kleft : (unsigned)piece_chunk(j) * 16u >= kleft;
-      if (on) voff[j] |= out ? K4_OOB : 0u;
-      else if (voff[j] < BAD) voff[j] &= ~K4_OOB;
-    }
-  }
-  // descriptor of the next K step (rebased: an operand may exceed 4 GiB; rows, columns and K are masked above, so any size will do, and
-  // none once nothing is left to fetch: the refills behind the last step store zeros)
-  __device__ __forceinline__ void open(int records) {
-    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(cur), 0, records, K4_RSRC_FLAGS);
+  // the next K step: the descriptor is rebased to it (an operand may exceed 4 GiB; rows and columns are masked in the lane offsets, so any
+  // size will do).  last: what lies beyond K reads as zero, by the lanes' chunks or by the descriptor's end; dead: nothing is left to fetch,
+  // the refills behind the last step store zeros
+  __device__ __forceinline__ FzStep next(bool last, bool dead) {
+    const unsigned bytes = dead ? 0u : KS && last ? tail_bytes : 0x7fffffffu;
+    const FzStep st{__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(cur), 0, (int)bytes, K4_RSRC_FLAGS), !KS && last ? beyond : 0u};
     cur += kstep;
+    return st;
   }
   template <int J>
-  __device__ __forceinline__ void issue_piece(char* slot_of_wave, char* spare) const {
+  __device__ __forceinline__ void issue_piece(const FzStep& st, char* slot_of_wave, char* spare) const {
     char* dst = slot_of_wave + NW * J * 1024;
     if constexpr (SPARE && (J + 1) * NW > PIECES) {
       if (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) + NW * J >= PIECES) dst = spare;
     }
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)dst, 16, (int)voff[J], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(st.rs, (k4_lds_ptr)dst, 16, (int)(KS ? voff[J] : voff[J] | st.mask), 0, 0, 0);
   }
   template <int... J>
-  __device__ __forceinline__ void issue(char* slot_of_wave, char* spare, std::integer_sequence<int, J...>) const {
-    (issue_piece<J>(slot_of_wave, spare), ...);
+  __device__ __forceinline__ void issue(const FzStep& st, char* slot_of_wave, char* spare, std::integer_sequence<int, J...>) const {
+    (issue_piece<J>(st, slot_of_wave, spare), ...);
   }
-  __device__ __forceinline__ void issue(char* slot_of_wave, char* spare) const { issue(slot_of_wave, spare, std::make_integer_sequence<int, PPW>{}); }
+  __device__ __forceinline__ void issue(const FzStep& st, char* slot_of_wave, char* spare) const {
+    issue(st, slot_of_wave, spare, std::make_integer_sequence<int, PPW>{});
+  }
 
   static constexpr int NRAW = KS ? 2 * NT : NT;
   using RawT = typename std::conditional<KS, u32x2, u32x4>::type;
   // LDS byte offset of tile TI behind rd[0]: K-contiguous tiles of 16 rows (natural) or pairs of 32 (paired); GATED: the second half of
   // the tiles lies BN / 2 rows further on
   static constexpr int kc_off(int ti) {
-    if (!PAIRED) return ti * 1024;
+    if (!PAIRED) return ti * 16 * SB;
     const int half = GATED && ti >= NT / 2, t = half ? ti - NT / 2 : ti;
-    return half * (ROWS / 2) * 64 + (t >> 1) * 2048 + (t & 1) * 256;
+    return (half * (ROWS / 2) + (t >> 1) * 32 + (t & 1) * 4) * SB;
   }
-  // read I of the NRAW that make up the wave's fragments of the step in the slot at LDS byte address sb
-  template <int I>
+  // read I of the NRAW that make up the wave's fragments of MFMA step H of the slot at LDS byte address sb
+  template <int H, int I>
   __device__ __forceinline__ void read(unsigned sb, RawT (&f)[NRAW]) const {
     if constexpr (!KS) {
-      if constexpr (ODD && I == NT - 1) f[I] = g16d_read128(sb + rd[1], 0);
-      else f[I] = g16d_read128(sb + rd[0], kc_off(I));
+      if constexpr (ODD && I == NT - 1) f[I] = g16d_read128(sb + rd[HALVES + H], 0);
+      else f[I] = g16d_read128(sb + rd[H], kc_off(I));
     } else {
       constexpr int TI = I / 2;
-      f[I] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], (PAIRED ? (TI & 1) * 8 : 0) + (I & 1) * 4 * PITCH);
+      f[I] = g16d_read_tr(sb + rd[PAIRED ? TI >> 1 : TI], H * 32 * PITCH + (PAIRED ? (TI & 1) * 8 : 0) + (I & 1) * 4 * PITCH);
     }
   }
   static __device__ __forceinline__ void tie(RawT (&f)[NRAW]) {
@@ -373,15 +378,15 @@ __device__ __forceinline__ bool fz_tile(int b, int tiles_m, int tiles_n, int& tm
 constexpr int fz_share(int q, int n, int over) { return over < 1 || q >= over ? n : (q * n + over - 1) / over; }
 
 // E: operand type; TO: type of out / base / pre; BM x BN tile, waves WR x WC; D: ring slots
-template <typename E, typename TO, int BM, int BN, int WR, int WC, int D, bool A_KS, bool B_KS, int EPI>
+template <typename E, typename TO, int BM, int BN, int WR, int WC, int SB, int D, bool A_KS, bool B_KS, int EPI>
 struct FzKernel {
   static constexpr int NW = WR * WC, BNO = EPI == FZ_GATED ? BN / 2 : BN;  // BNO: output columns of a tile
   static constexpr bool GATED = EPI == FZ_GATED;
-  using OA = FzOperand<BM, WR, NW, A_KS, false, false>;
-  using OB = FzOperand<BN, WC, NW, B_KS, true, GATED>;
+  using OA = FzOperand<BM, WR, NW, SB, A_KS, false, false>;
+  using OB = FzOperand<BN, WC, NW, SB, B_KS, true, GATED>;
   static constexpr int STAGE = OA::SLOT + OB::SLOT, LDS = D * STAGE + (OA::SPARE || OB::SPARE ? 1024 : 0);
   static constexpr int MI = OA::NT, NI = OB::NT, C = OA::PPW + OB::PPW;
-  static_assert(D >= 4 && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
+  static_assert(D >= (SB == 64 ? 4 : 2) && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
 
   static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b, int z) {
     const int NO = GATED ? ep.F : p.N;
@@ -401,55 +406,44 @@ struct FzKernel {
     // places in the tile instead of the offset becoming negative
     ob.setup(p.B, p.ldb, n0, p.N, p.K, p.kb, OA::SLOT, wc, GATED ? ep.F : 0);
 
-    constexpr int ES = FE<E>::SIZE, STEP = 64 / ES;
+    constexpr int ES = FE<E>::SIZE, STEP = SB / ES;
     const int nk = (p.K + STEP - 1) / STEP;
-    int steps = nk * p.nseg;
-    int seg = 0, left = nk, records = 0x7fffffff;  // of the next step to issue: its segment, the steps left in it
-    int todo = 0x40000000;                         // steps left to issue at all, where the range ends inside a segment
+    int slots = nk * p.nseg;
+    int seg = 0, left = nk;  // of the next slot to issue: its segment, the slots left in it
+    int todo = slots;        // slots left to issue at all
     auto plane = [](unsigned t, int s) { return (int64_t)((t >> (4 * s)) & 15u); };
     int first = 0;
     if constexpr (!GATED) {
       if (p.ksplit > 1) {
-        const int from = (int)((int64_t)steps * z / p.ksplit), to = (int)((int64_t)steps * (z + 1) / p.ksplit);
+        const int from = (int)((int64_t)slots * z / p.ksplit), to = (int)((int64_t)slots * (z + 1) / p.ksplit);
         seg = from / nk;
         first = from - seg * nk;
         left = nk - first;
-        steps = todo = to - from;
+        slots = todo = to - from;
       }
     }
     oa.seek(plane(p.pa, seg) * p.a_plane + (int64_t)first * oa.kstep);
     ob.seek(plane(p.pb, seg) * p.b_plane + (int64_t)first * ob.kstep);
-    auto open = [&]() {
-      if (left <= 1) {
-        if (left == 0) {
-          if (++seg < p.nseg && todo > 0) {
-            oa.seek(plane(p.pa, seg) * p.a_plane);
-            ob.seek(plane(p.pb, seg) * p.b_plane);
-            oa.tail(false);
-            ob.tail(false);
-            left = nk;
-          } else {
-            records = 0;
-            left = 0x40000000;
-          }
+    struct Steps {
+      FzStep a, b;
+    };
+    auto next = [&]() {
+      if (left == 0) {
+        if (++seg < p.nseg) {
+          oa.seek(plane(p.pa, seg) * p.a_plane);
+          ob.seek(plane(p.pb, seg) * p.b_plane);
         }
-        if (left == 1) {
-          oa.tail(true);
-          ob.tail(true);
-        }
+        left = nk;
       }
-      --left;
-      if constexpr (!GATED) {
-        if (todo-- == 0) records = 0;
-      }
-      oa.open(records);
-      ob.open(records);
+      const bool last = --left == 0, dead = todo-- <= 0;
+      return Steps{oa.next(last, dead), ob.next(last, dead)};
     };
     char *const wslot = smem + wave * 1024, *const spare = smem + D * STAGE;  // this wave's first DMA piece of slot 0
-    for (int s = 0; s < D - 1; ++s) {
-      open();
-      oa.issue(wslot + s * STAGE, spare);
-      ob.issue(wslot + s * STAGE + OA::SLOT, spare);
+    constexpr int AHEAD = D == 2 ? 2 : D - 1;  // slots filled before the loop
+    for (int s = 0; s < AHEAD; ++s) {
+      const Steps n = next();
+      oa.issue(n.a, wslot + s * STAGE, spare);
+      ob.issue(n.b, wslot + s * STAGE + OA::SLOT, spare);
     }
 
     using Acc = typename FE<E>::acc;
@@ -459,8 +453,8 @@ struct FzKernel {
 #pragma unroll
       for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = Acc{0, 0, 0, 0};
 
-    // Two steps between barriers.  When the waves meet before step s (even), its fragments are in everyone's registers and step s - 1 is
-    // done: both slots are free and take steps s - 1 + D and s + D, one in each half; steps s + 1 and s + 2 have landed (all DMA but the
+    // SB = 64: two steps between barriers.  When the waves meet before step s (even), its fragments are in everyone's registers and step s - 1 is
+    // done: both slots are free and take steps s - 1 + D and s + D; steps s + 1 and s + 2 have landed (all DMA but the
     // newest D - 4 steps').  The fragments of the next step are read and its refill is issued BETWEEN the MFMAs: reads over the first
     // 5/8 of the step, so that they have landed at its end, the DMA pieces evenly.
     constexpr int NH = MI * NI, RA = OA::NRAW, RB = OB::NRAW, R = RA + RB;
@@ -469,49 +463,89 @@ struct FzKernel {
       typename OA::RawT a[RA];
       typename OB::RawT b[RB];
     } f0, f1;
-    auto read_one = [&](auto ic, unsigned sb, Frags& f) {
-      constexpr int I = decltype(ic)::value;
-      if constexpr (I < RB) ob.template read<I>(sb, f.b);
-      else oa.template read<I - RB>(sb, f.a);
+    auto read_one = [&](auto hc, auto ic, unsigned sb, Frags& f) {
+      constexpr int H = decltype(hc)::value, I = decltype(ic)::value;
+      if constexpr (I < RB) ob.template read<H, I>(sb, f.b);
+      else oa.template read<H, I - RB>(sb, f.a);
     };
-    k4_wait_vm<(D - 2) * C>();
+    k4_wait_vm<(AHEAD - 1) * C>();
     __builtin_amdgcn_s_barrier();  // raw: __syncthreads() would drain the DMA queue
     asm volatile("" ::: "memory");
-    g16d_for_each([&](auto ic) { read_one(ic, sbase, f0); }, std::make_integer_sequence<int, R>{});
+    g16d_for_each([&](auto ic) { read_one(std::integral_constant<int, 0>{}, ic, sbase, f0); }, std::make_integer_sequence<int, R>{});
     int read_at = 0, fill_at = (D - 1) * STAGE;  // bytes
-    auto step = [&](Frags& now, Frags& then, auto meet) {
-      char* fill = wslot + fill_at;
-      fill_at = fill_at == (D - 1) * STAGE ? 0 : fill_at + STAGE;
-      read_at = read_at == (D - 1) * STAGE ? 0 : read_at + STAGE;
-      const unsigned sn = sbase + (unsigned)read_at;
-      open();
-      if constexpr (decltype(meet)::value) k4_wait_vm<(D - 4) * C>();
+    auto advance = [&](int at) { return at == (D - 1) * STAGE ? 0 : at + STAGE; };
+    // The MFMAs of the fragments `now`; between them the reads of the next step's (MFMA step H of the slot at sn) and DMA pieces FROM .. TO
+    // of the refill n
+    auto compute = [&](Frags& now, Frags& then, auto hc, unsigned sn, const Steps& n, char* fill, auto from, auto to) {
+      constexpr int F = decltype(from)::value, ND = decltype(to)::value - F;
       g16d_lgkm<0>();
       OB::tie(now.b);
       OA::tie(now.a);
-      if constexpr (decltype(meet)::value) __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       g16d_for_each([&](auto qc) {
         constexpr int Q = decltype(qc)::value;
         acc[Q % MI][Q / MI] = FE<E>::mma(OB::get(now.b, Q / MI), OA::get(now.a, Q % MI), acc[Q % MI][Q / MI]);
-        constexpr int r0 = fz_share(Q, R, NH * 5 / 8), r1 = fz_share(Q + 1, R, NH * 5 / 8), d0 = Q * C / NH, d1 = (Q + 1) * C / NH;
+        constexpr int r0 = fz_share(Q, R, NH * 5 / 8), r1 = fz_share(Q + 1, R, NH * 5 / 8), d0 = Q * ND / NH, d1 = (Q + 1) * ND / NH;
         if constexpr (r1 > r0 || d1 > d0) {
           __builtin_amdgcn_sched_barrier(0);
-          g16d_for_each([&](auto ic) { read_one(std::integral_constant<int, r0 + decltype(ic)::value>{}, sn, then); },
+          g16d_for_each([&](auto ic) { read_one(hc, std::integral_constant<int, r0 + decltype(ic)::value>{}, sn, then); },
                         std::make_integer_sequence<int, r1 - r0>{});
           g16d_for_each([&](auto ic) {
-            constexpr int P = d0 + decltype(ic)::value;
-            if constexpr (P < OA::PPW) oa.template issue_piece<P>(fill, spare);
-            else ob.template issue_piece<P - OA::PPW>(fill + OA::SLOT, spare);
+            constexpr int P = F + d0 + decltype(ic)::value;
+            if constexpr (P < OA::PPW) oa.template issue_piece<P>(n.a, fill, spare);
+            else ob.template issue_piece<P - OA::PPW>(n.b, fill + OA::SLOT, spare);
           }, std::make_integer_sequence<int, d1 - d0>{});
           __builtin_amdgcn_sched_barrier(0);
         }
       }, std::make_integer_sequence<int, NH>{});
     };
-    for (int s = 0; s < steps; s += 2) {  // an odd number of steps ends with one of zeros
-      step(f0, f1, std::true_type{});
-      step(f1, f0, std::false_type{});
+    auto meet = [&](auto outstanding) {  // the fragments that are about to be used have been read, and so many DMA operations may be in flight
+      k4_wait_vm<decltype(outstanding)::value>();
+      g16d_lgkm<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using IC = std::integral_constant<int, C>;
+    if constexpr (SB == 64) {
+      for (int s = 0; s < slots; s += 2) {  // an odd number of steps ends with one of zeros
+        auto step = [&](Frags& now, Frags& then, auto first) {
+          char* fill = wslot + fill_at;
+          fill_at = advance(fill_at);
+          read_at = advance(read_at);
+          const Steps n = next();
+          if constexpr (decltype(first)::value) meet(std::integral_constant<int, (D - 4) * C>{});
+          compute(now, then, I0{}, sbase + (unsigned)read_at, n, fill, I0{}, IC{});
+        };
+        step(f0, f1, std::true_type{});
+        step(f1, f0, std::false_type{});
+      }
+    } else if constexpr (D == 2) {
+      // SB = 128, two slots: the waves meet in the middle of slot k, when all of it is in registers; it takes slot k + 2 while slot k + 1,
+      // landed by then, is read
+      int at = 0;
+      for (int s = 0; s < slots; ++s) {
+        const Steps n = next();
+        compute(f0, f1, std::integral_constant<int, OA::HALVES - 1>{}, sbase + (unsigned)at, n, wslot, I0{}, I0{});
+        meet(I0{});
+        compute(f1, f0, I0{}, sbase + (unsigned)(STAGE - at), n, wslot + at, I0{}, IC{});
+        at = STAGE - at;
+      }
+    } else {
+      // SB = 128: one slot, two steps, between barriers.  When the waves meet before slot k, slot k - 1 is free and takes slot k - 1 + D, and
+      // slot k + 1 has landed (all DMA but the newest D - 3 slots').  (With D = 3 nothing may be in flight at a meeting: 140 -> 184 us for
+      // dx 4096 x 1280 x 10240 on 128 x 160; with D = 4: 117.)
+      for (int s = 0; s < slots; ++s) {
+        char* fill = wslot + fill_at;
+        fill_at = advance(fill_at);
+        const unsigned sb = sbase + (unsigned)read_at;
+        read_at = advance(read_at);
+        const Steps n = next();
+        meet(std::integral_constant<int, (D - 3) * C>{});
+        using IH = std::integral_constant<int, C / 2>;
+        compute(f0, f1, std::integral_constant<int, OA::HALVES - 1>{}, sb, n, fill, I0{}, IH{});
+        compute(f1, f0, I0{}, sbase + (unsigned)read_at, n, fill, IH{}, IC{});
+      }
     }
     // the reads and refills behind the last step have landed before their registers and LDS are given up
     g16d_lgkm<0>();
@@ -560,7 +594,7 @@ struct FzKernel {
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) sa[mi] = ep.sa && m0 + row0 + 16 * mi < p.M ? ep.sa[m0 + row0 + 16 * mi] : 1.f;
 
-    const int64_t rows = p.M - m0, prow = m0 + ep.pre_row;
+    const int64_t rows = p.M - m0;
     auto open_rows = [&](const void* base, int64_t row, int64_t pitch, bool have) {
       const int64_t bytes = have ? rows * pitch : 0;
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + row * pitch, 0,
@@ -568,8 +602,8 @@ struct FzKernel {
     };
     const int po = NO * TS, pb = po * H, ph = NO * (TS == 4 ? 8 : 4), pl = NO * 2;  // pitches: out, base, p and its 8-bit plane
     const __amdgpu_buffer_rsrc_t ro = open_rows(ep.out, m0, po, true), rb = open_rows(ep.base, m0, pb, ep.base != nullptr);
-    const __amdgpu_buffer_rsrc_t rh = open_rows(ep.pre, prow, ph, GATED && ep.pre),
-                                 rl = open_rows(static_cast<char*>(ep.pre) + 2 * ep.pre_total, prow, pl, GATED && ep.pre && TS == 2);
+    const __amdgpu_buffer_rsrc_t rh = open_rows(ep.pre, m0, ph, GATED && ep.pre),
+                                 rl = open_rows(static_cast<char*>(ep.pre) + 2 * ep.pre_total, m0, pl, GATED && ep.pre && TS == 2);
 
     // CN columns from n on, of every row tile; get(mi, e, half): their sums
     auto emit = [&](auto cn, int n, auto get) {
@@ -669,7 +703,7 @@ struct FzKernel {
                 keep(hoff, loff, vrow, v);
                 keep(hoff, loff, grow, t);
               } else {
-                const int64_t at = (m + ep.pre_row) * 2 * NO;
+                const int64_t at = m * 2 * NO;
                 fz_store_pre8<TO>(ep.pre, ep.pre_total, at + vrow + n, n, NO, v);
                 fz_store_pre8<TO>(ep.pre, ep.pre_total, at + grow + n, n, NO, t);
               }
