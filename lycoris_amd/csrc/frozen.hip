@@ -78,8 +78,8 @@ int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
 }
 
 // Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.
-//   256 x 256, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (three of 4 waves; gated: 64 x 128); where the tiles are few
-//   and K is long, K in parts whose sums a second launch joins.
+//   256 x 256, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (two of 4 waves; gated: 64 x 128, one); where the tiles are
+//   few and K is long, K in parts whose sums a second launch joins.
 // The tile of 160 columns is there for outputs of 320, 640 and 1280 channels, which it cuts into as many tiles as CUs: 4096 x 1280 are 256 (dx
 // with K = 10240, inputs out of HBM: 117 us, against 161 with 128 x 128 and 256 with 256 x 256); with whole rounds of the larger tile that wins
 // (dx 16384 x 5120, K = 1280: 213 us, against 240 with 128 x 128 and 289 with 128 x 160).
@@ -95,10 +95,10 @@ struct Rate {
 };
 struct Tile {
   int id, bm, bn, wgs;
-  Rate rate[3];  // with 1, 2, 3 workgroups on the CU
+  Rate rate[2];  // with 1, 2 workgroups on the CU
 };
 constexpr Tile TILES[] = {{128, 128, 128, 2, {{0.30, 3.0, 1.0}, {0.54, 2.5, 0.5}}},
-                          {64, 64, 64, 3, {{0.18, 2.5, 1.0}, {0.26, 2.0, 0.5}, {0.36, 2.0, 0.35}}},
+                          {64, 64, 64, 2, {{0.18, 2.5, 1.0}, {0.26, 2.0, 0.5}}},
                           {160, 128, 160, 1, {{0.35, 3.5, 1.0}}},
                           {256, 256, 256, 1, {{0.73, 5.0, 0.7}}}};
 constexpr double CU_BYTES_PER_US = 19900.0;
@@ -114,11 +114,13 @@ Plan plan_gemm(int64_t M, int64_t NO, double steps, bool gated, double eb) {
     if (gated && t.id == 160) continue;
     Tile u = t;
     const int bno = !gated || t.id == 64 ? t.bn : t.bn / 2;
-    if (gated)  // the activation's vector work, and 64 x 64 outputs take 128 rows of w
+    if (gated) {  // the activation's vector work, and 64 x 64 outputs take 128 rows of w
+      if (t.id == 64) u.wgs = 1;
       for (Rate& r : u.rate) {
         r.tile += t.id == 256 ? 4.0 : t.id == 128 ? 1.0 : 2.0;
-        if (t.id == 64) r.step *= 2.0;
+        if (t.id == 64) r.step *= 1.4;
       }
+    }
     const int64_t tiles = cdiv(M, t.bm) * cdiv(NO, bno);
     const double area = (double)t.bm * bno;
     for (int ks = 1; ks == 1 || (!gated && ks <= 8 && steps / ks >= 12); ++ks) {
@@ -144,7 +146,7 @@ int launch_gemm(const Plan& pl, FzProb p, FzEpi ep, void* part, hipStream_t st) 
   constexpr int SB = A_KS && B_KS ? 64 : 128, D = A_KS && B_KS ? 5 : 2;
   using K256 = FzKernel<E, TO, 256, 256, 2, 4, SB, D, A_KS, B_KS, EPI>;
   using K128 = FzKernel<E, TO, 128, 128, 4, 2, SB, D, A_KS, B_KS, EPI>;
-  using K64 = FzKernel<E, TO, 64, G ? 128 : 64, 2, 2, 128, 3, A_KS, B_KS, EPI>;
+  using K64 = FzKernel<E, TO, 64, G ? 128 : 64, 2, 2, 128, 4, A_KS, B_KS, EPI>;
   p.ksplit = pl.ksplit;
   ep.part = part;
   switch (pl.tile) {

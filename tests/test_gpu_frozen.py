@@ -514,3 +514,113 @@ def test_refusals_on_the_device():
     xl = x.clone().requires_grad_(True)
     with pytest.raises(RuntimeError, match="once only"):
         torch.autograd.grad(ops.int8_linear(xl, wq, sw).float().pow(2).sum(), xl, create_graph=True)
+
+
+def test_calls_from_two_threads():
+    import threading
+    gen = torch.Generator().manual_seed(21)
+    wq, sw = held(gen, 640, 320)
+    xs = [rnd(gen, (300 + 41 * i, 320), torch.bfloat16) for i in range(2)]
+    want = [ops.int8_linear(x, wq, sw) for x in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                got[i].append(ops.int8_linear(xs[i], wq, sw))
+        st.synchronize()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+def test_traced_block_equals_the_eager_one():
+    gen = torch.Generator().manual_seed(22)
+    wq, sw = held(gen, 128, 64)
+    w, b = rnd(gen, (96, 128), torch.bfloat16, 0.1), rnd(gen, (96,), torch.bfloat16)
+
+    def block(x, w):
+        h = torch.ops.lycoris_amd.int8_linear(x, wq, sw, None, None)
+        return torch.ops.lycoris_amd.gated_linear(h, w, None, b, None, 2, True)
+
+    x = rnd(gen, (5, 7, 64), torch.bfloat16)
+    g = rnd(gen, (5, 7, 48), torch.bfloat16)
+    outs = []
+    for f in (block, torch.compile(block, backend="aot_eager", fullgraph=True)):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = f(xl, wl)
+        outs.append([y.detach(), *torch.autograd.grad(y, [xl, wl], g)])
+    for a, c in zip(*outs):
+        assert torch.equal(a, c)
+
+
+# ---- together: a transformer block whose frozen layers are held in 8 bits, under adapters ------------------------------------------------
+class Block(torch.nn.Module):
+    def __init__(self, c, f):
+        super().__init__()
+        from lycoris_amd import GatedLinear
+        self.to_q, self.to_out = torch.nn.Linear(c, c, bias=False), torch.nn.Linear(f, c)
+        self.ff = GatedLinear(torch.nn.Linear(c, 2 * f))
+
+    def forward(self, x):
+        h = x + self.to_q(x)
+        return h + self.to_out(self.ff(h))
+
+
+@pytest.mark.parametrize("algo", ["locon", "lokr"])
+@pytest.mark.parametrize("dt,tol", [(torch.float32, 2e-3), (torch.bfloat16, 3e-2)], ids=["f32", "bf16"])
+def test_training_step_of_adapters_on_an_int8_block(algo, dt, tol):
+    """One step of adapters on Int8Linear layers and a GatedLinear block, against the same modules on the host in 64 bits.  Both sides
+    quantise their own activations: an element whose value differs by r of itself changes its integer with probability 127 r, by a step of
+    1/127 of the row's maximum (four times its rms, say).  fp32: r = 1e-6, so that one element in 1e4 moves by 3 % of the rms: 3e-4 norm-wise
+    a layer, three layers.  bf16: 2^-9 and more (the activations are rounded): a fifth of the elements, 1.4 % a layer."""
+    from lycoris_amd import LoConModule, LokrModule, NATIVE_ALGOS, quantize_frozen
+    assert NATIVE_ALGOS["locon"] is LoConModule
+    torch.manual_seed(3)
+    c, f = 320, 640
+    nets = [Block(c, f).requires_grad_(False) for _ in range(2)]
+    nets[1].load_state_dict(nets[0].state_dict())
+    x = torch.randn(2, 150, c).to(dt)
+    g = (torch.randn(2, 150, c) / c).to(dt)
+    results = []
+    for net, dev, ct in ((nets[0], DEV, dt), (nets[1], "cpu", torch.float64)):
+        names = quantize_frozen(net)  # the same integers on both sides
+        assert sorted(names) == ["ff.proj", "to_out", "to_q"]
+        net.to(dev)
+        layers = [net.to_q, net.ff.proj, net.to_out]
+        torch.manual_seed(4)
+        cls, kw = (LoConModule, dict(lora_dim=8, alpha=4.0)) if algo == "locon" else (LokrModule, dict(lora_dim=100000, factor=8))
+        mods = [cls(f"m{i}", l, **kw) for i, l in enumerate(layers)]
+        with torch.no_grad():
+            for m in mods:
+                for p in m.parameters():
+                    p.copy_(torch.randn(p.shape, generator=torch.Generator().manual_seed(p.numel())) * 0.1)
+        for m in mods:
+            m.to(dev)
+            if ct == torch.float64:
+                m.double()
+            m.apply_to()
+        for l in layers:
+            l.bias = None if l.bias is None else torch.nn.Parameter(l.bias.to(ct), requires_grad=False)
+            l.dtype = ct
+        xl = x.to(dev).to(ct).requires_grad_(True)
+        y = net(xl)
+        assert net.ff._adapters() == [mods[1]]
+        params = [p for m in mods for p in m.parameters()]
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        if dev == DEV:
+            ops.fused_grad_accumulation(True, None)
+        try:
+            y.backward(g.to(dev).to(ct))
+        finally:
+            ops.fused_grad_accumulation(False, None)
+        results.append([y.detach(), xl.grad] + [p.grad for p in params])
+        assert all(q.grad is None for l in layers for q in l.parameters())
+    for i, (a, b) in enumerate(zip(*results)):
+        a, b = f64(a), f64(b)
+        assert float((a - b).norm() / b.norm()) <= tol, i
