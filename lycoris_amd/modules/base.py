@@ -516,7 +516,8 @@ class LycorisBaseModule(nn.Module, metaclass=_TwinMeta):
         return p.device, p.dtype
 
     def _require_writable_weight(self, what):
-        if isinstance(getattr(type(self.org_module[0]), "weight", None), property):  # Int8Linear: `weight` is an expansion, not storage
+        from .frozen import Int8Linear
+        if isinstance(self.org_module[0], Int8Linear):  # its `weight` is an expansion, not storage
             raise _unsupported(f"{what} into a {type(self.org_module[0]).__name__} ({self.lora_name}): its 8-bit weight cannot take the sum; "
                                "merge into the unquantised layer, then quantise")
 
