@@ -233,6 +233,8 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
         for (int e = 0; e < 8; ++e) dv[e] *= sv[e], dt[e] *= st[e];
         fz_store8<E>(dps, m * lds + vo + k, k, F, full, dv);
         fz_store8<E>(dps, m * lds + go + k, k, F, full, dt);
+        if (k + 8 >= F)  // the product reads whole 16-byte chunks
+          for (int64_t c = N; c < lds; ++c) dps[m * lds + c] = (E)0.f;
       }
     }
   }

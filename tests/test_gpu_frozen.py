@@ -47,6 +47,12 @@ def quantize64(x):
     return q, (amax.float() / 127.0).double()
 
 
+def poison():
+    """leave NaNs in the memory that the next calls' outputs and workspaces come from"""
+    blocks = [torch.full((n,), float("nan"), device=DEV) for n in [1 << 17] * 24 + [1 << 22] * 4 + [1 << 25]]
+    del blocks
+
+
 def within(got, want, bound, what):
     sub = sub_of(got.dtype)
     got = f64(got).reshape(want.shape)
@@ -130,6 +136,7 @@ def test_linear_forward_and_dx(M, K, N, dt):
     base = rnd(gen, (*lead, N), dt, 0.3) if K % 3 else None
     xl = x.clone().requires_grad_(True)
     bl = None if base is None else base.clone().requires_grad_(True)
+    poison()
     y = ops.int8_linear(xl, wq, sw, bias, bl)
     assert y.shape == (*lead, N) and y.dtype == dt
     want, err = linear_reference(x, wq, sw, bias, base)
@@ -225,6 +232,7 @@ def test_matmul(M, K, N, dt):
     mag = p.abs() + (0 if bias is None else f64(bias).abs())
     want = p if bias is None else p + f64(bias)
     bound = 6 * E * mag + u_of(dt) * (want.abs() + 6 * E * mag)
+    poison()
     within(ops.int8_matmul(aq, sa, bq, sb, bias, dtype=dt), want, bound, "y")
     pitch = (K + 15) // 16 * 16 + 16
     wide = torch.full((M, pitch), -5, dtype=torch.int8, device=DEV)  # rows with values behind K
@@ -332,6 +340,7 @@ def test_gated_forward_and_gradients(M, K, F, dt, int8):
         w64 = f64(w)
     g = rnd(gen, (*lead, F), dt, 1 / math.sqrt(F))
     leaf = lambda t: None if t is None else t.clone().requires_grad_(True)  # noqa: E731
+    poison()
     leaves = {"dx": leaf(x), "dw": None if int8 else leaf(w), "dbias": leaf(bias), "dbase": leaf(base)}
     y = ops.gated_linear(leaves["dx"], w if int8 else leaves["dw"], leaves["dbias"], leaves["dbase"], act=act, gate_first=gate_first, weight_scale=sw)
     assert y.shape == (*lead, F) and y.dtype == dt
