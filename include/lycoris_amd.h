@@ -468,7 +468,7 @@ int lyc_rows_to_nchw(const void* rows, void* t, int64_t B, int64_t C, int64_t P,
  * The frozen nn.Linear under an adapter (the `org_forward(x)` of every lycoris/modules forward) with its weight kept as integers:
  *   w[n, k] ~= sw[n] wq[n, k],  sw[n] = max_k |w[n, k]| / 127,  wq = round-half-even(127 w / max|w|)   (lyc_int8_quantize on its rows)
  * and its input quantised the same way, one scale a row, on every call.  A row that holds an infinity or a NaN gets scale NaN.
- * Rows of 8-bit operands: 16-byte aligned base, pitch a multiple of 16.  K <= 2^17 (the int32 sums cannot overflow).
+ * Rows of 8-bit operands: 16-byte aligned base, pitch a multiple of 16.  K < 2^17 (the int32 sums cannot overflow), M <= 2^26.
  * `bias`: [N], fp32 when bias_f32, else `dtype`; `base`: [M, N] in `dtype` (an adapter's output), either may be NULL.
  * `ws`: device scratch of the *_workspace_bytes(...) bytes (-1: bad arguments), 16-byte aligned, no need to clear.        */
 int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int64_t K, int dtype, void* stream);

@@ -38,8 +38,9 @@ struct Carve {
 int check_dims(const char* who, int64_t M, int64_t N, int64_t K, int dtype) {
   if (dtype != LYC_F32 && dtype != LYC_F16 && dtype != LYC_BF16) return fail(LYC_ERR_ARG, "%s: unknown dtype %d", who, dtype);
   if (M < 0 || N < 1 || K < 1) return fail(LYC_ERR_ARG, "%s: bad dims M=%ld N=%ld K=%ld", who, (long)M, (long)N, (long)K);
-  if (M > (1 << 30) || N > (1 << 20) || K > (1 << 17))
-    return fail(LYC_ERR_UNSUPPORTED, "%s: M=%ld N=%ld K=%ld exceed 2^30 rows, 2^20 outputs or 2^17 inputs", who, (long)M, (long)N, (long)K);
+  // K: 2^17 products of -128 and -128 would sum to 2^31; M: launches stay below 2^32 threads, and 2 M bytes below 2^31 where rows are summed
+  if (M > (1 << 26) || N > (1 << 20) || K >= (1 << 17))
+    return fail(LYC_ERR_UNSUPPORTED, "%s: M=%ld N=%ld K=%ld exceed 2^26 rows, 2^20 outputs or 2^17 - 1 inputs", who, (long)M, (long)N, (long)K);
   return LYC_OK;
 }
 #define FZ_TRY(expr)                  \
@@ -192,6 +193,11 @@ inline bool skinny_fused(int64_t M, int64_t K) { return M <= SKINNY_ROWS && M * 
 
 template <typename T>
 int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int K, hipStream_t st) {
+  constexpr int64_t SLAB = 1 << 22;  // rows a launch: a workgroup a row stays below 2^32 threads
+  if (M > SLAB) {
+    FZ_TRY(launch_quant<T>(x, ldx, q, ldq, scale, SLAB, K, st));
+    return launch_quant<T>(x + SLAB * ldx, ldx, q + SLAB * ldq, ldq, scale + SLAB, M - SLAB, K, st);
+  }
   const int vec = fz_al16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0 && K % 8 == 0;
   const int64_t c = ldq / 8;  // chunks of 8 a row
   auto go = [&](auto tpr, auto nv) {
@@ -407,7 +413,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   const float* range = nullptr;
   if (scaled) FZ_TRY(launch_range<E>(q.sw, N, 7, f, &range, st));  // the largest sw f[0] near 1
   const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp);
-  hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)cdiv(q.F, DG_COLS), (unsigned)parts), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
+  hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)(cdiv(q.F, DG_COLS) * parts)), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
                      (int)q.F, q.act, q.gate_first, vec, rows);
   FZ_TRY(check_launch("gated backward"));
   if (want_dw || (want_dx && !scaled)) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));

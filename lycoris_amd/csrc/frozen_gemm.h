@@ -75,21 +75,23 @@ __device__ __forceinline__ void fz_phi(float t, float& phi, float& e) {
 __device__ __forceinline__ float fz_sigmoid(float t) { return __builtin_amdgcn_rcpf(1.f + __expf(-t)); }
 
 // act(t) and its derivative in fp32
-__device__ __forceinline__ float fz_act(int act, float t) {
-  if (act == FZ_ACT_SILU) return t * fz_sigmoid(t);
-  if (act == FZ_ACT_GELU) {
+template <int ACT>
+__device__ __forceinline__ float fz_act(float t) {
+  if constexpr (ACT == FZ_ACT_SILU) return t * fz_sigmoid(t);
+  if constexpr (ACT == FZ_ACT_GELU) {
     float phi, e;
     fz_phi(t, phi, e);
     return t * phi;
   }
   return t * fz_sigmoid(1.5957691216057308f * (t + 0.044715f * t * t * t));  // 0.5 t (1 + tanh u) = t sigmoid(2 u)
 }
-__device__ __forceinline__ void fz_act_grad(int act, float t, float& a, float& da) {
-  if (act == FZ_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ void fz_act_grad(float t, float& a, float& da) {
+  if constexpr (ACT == FZ_ACT_SILU) {
     const float s = fz_sigmoid(t);
     a = t * s;
     da = s + a * (1.f - s);
-  } else if (act == FZ_ACT_GELU) {
+  } else if constexpr (ACT == FZ_ACT_GELU) {
     float phi, e;
     fz_phi(t, phi, e);
     a = t * phi;
@@ -97,8 +99,15 @@ __device__ __forceinline__ void fz_act_grad(int act, float t, float& a, float& d
   } else {
     const float s = fz_sigmoid(1.5957691216057308f * (t + 0.044715f * t * t * t));
     a = t * s;
-    da = s + a * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * t * t);
+    da = s + a * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * fminf(t * t, 1e30f));  // (0 times infinity would be NaN)
   }
+}
+// f(the activation as a constant): one branch for as many values as f works on (a branch for each keeps the compiler from interleaving them)
+template <typename F>
+__device__ __forceinline__ void fz_for_act(int act, F f) {
+  if (act == FZ_ACT_SILU) f(std::integral_constant<int, FZ_ACT_SILU>{});
+  else if (act == FZ_ACT_GELU) f(std::integral_constant<int, FZ_ACT_GELU>{});
+  else f(std::integral_constant<int, FZ_ACT_GELU_TANH>{});
 }
 
 // One product.  lda / ldb in bytes.  kb: bytes of K along a K-contiguous operand, rounded up to 16 (what the operand's rows hold up to
@@ -347,8 +356,8 @@ __device__ __forceinline__ void fz_load_pre8(const void* pre, int64_t total, int
       const u32x4 h = *reinterpret_cast<const u32x4*>(hi);
       const u32x2 l = *reinterpret_cast<const u32x2*>(lo);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = __uint_as_float(((h[e >> 1] >> (16 * (e & 1))) << 16) | (((l[e >> 2] >> (8 * (e & 3))) & 0xffu) << 8));
+      for (int e = 0; e < 8; ++e)  // bytes: two of h, one of l, a zero
+        v[e] = __uint_as_float(__builtin_amdgcn_perm(h[e >> 1], l[e >> 2], (e & 1 ? 0x07060000u : 0x05040000u) | ((e & 3) << 8) | 0x0cu));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = n + e < N ? __uint_as_float(((unsigned)hi[e] << 16) | ((unsigned)lo[e] << 8)) : 0.f;
@@ -708,8 +717,10 @@ struct FzKernel {
                 fz_store_pre8<TO>(ep.pre, ep.pre_total, at + grow + n, n, NO, t);
               }
             }
+            fz_for_act(ep.act, [&](auto ac) {
 #pragma unroll
-            for (int e = 0; e < CN; ++e) v[e] *= fz_act(ep.act, t[e]);
+              for (int e = 0; e < CN; ++e) v[e] *= fz_act<decltype(ac)::value>(t[e]);
+            });
           }
         }
         if (vec) {

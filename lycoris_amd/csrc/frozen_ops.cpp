@@ -116,7 +116,8 @@ std::tuple<Tensor, Tensor> int8_quantize(const Tensor& x) {
   const int64_t K = x.size(-1), M = x.numel() / K, ldq = (K + 127) / 128 * 128;
   Tensor r = x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= K ? x : x.reshape({M, K}).contiguous();
   Tensor q = at::empty({M, ldq}, x.options().dtype(at::kChar)), scale = at::empty({M}, x.options().dtype(at::kFloat));
-  check_rc(lyc_int8_quantize(r.const_data_ptr(), r.stride(0), q.mutable_data_ptr<int8_t>(), ldq, scale.mutable_data_ptr<float>(), M, K,
+  // (the pitch of a single row means nothing and may be anything)
+  check_rc(lyc_int8_quantize(r.const_data_ptr(), M > 1 ? r.stride(0) : K, q.mutable_data_ptr<int8_t>(), ldq, scale.mutable_data_ptr<float>(), M, K,
                              code_of(x.scalar_type()), stream_of(x)), "int8_quantize");
   auto lead = x.sizes().vec();
   lead.pop_back();

@@ -192,8 +192,9 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
                                                        int act, int gate_first, int vec, int rows) {
   __shared__ float sums[2][DG_COLS];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int k = blockIdx.x * DG_COLS + tx * 8;
-  const int64_t m0 = (int64_t)blockIdx.y * rows;
+  const int across = (F + DG_COLS - 1) / DG_COLS, slab = (int)(blockIdx.x / across), c0 = ((int)blockIdx.x - slab * across) * DG_COLS;
+  const int k = c0 + tx * 8;
+  const int64_t m0 = (int64_t)slab * rows;
   const int vo = gate_first ? F : 0, go = gate_first ? 0 : F;
   const bool full = vec && k + 8 <= F;
   const int64_t N = 2 * (int64_t)F, lds = (N + 7) & ~7;
@@ -207,37 +208,40 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
 #pragma unroll
     for (int e = 0; e < 8; ++e) sv[e] *= scale, st[e] *= scale;
   }
-  if (k < F) {
+  auto each = [&](auto ac, auto fc) {
+    constexpr bool FULL = decltype(fc)::value;
 #pragma unroll 2
     for (int r = ty; r < rows && m0 + r < M; r += 8) {
       const int64_t m = m0 + r;
       float gv[8], v[8], t[8], dv[8], dt[8];
-      fz_load8<T>(g, m * F + k, k, F, full, gv);
-      fz_load_pre8<T>(pre, M * N, m * N + vo + k, k, F, full, v);
-      fz_load_pre8<T>(pre, M * N, m * N + go + k, k, F, full, t);
+      fz_load8<T>(g, m * F + k, k, F, FULL, gv);
+      fz_load_pre8<T>(pre, M * N, m * N + vo + k, k, F, FULL, v);
+      fz_load_pre8<T>(pre, M * N, m * N + go + k, k, F, FULL, t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float a, da;
-        fz_act_grad(act, t[e], a, da);
+        fz_act_grad<decltype(ac)::value>(t[e], a, da);
         dv[e] = gv[e] * a;
         dt[e] = gv[e] * v[e] * da;
         cv[e] += dv[e];
         ct[e] += dt[e];
       }
       if (dp) {
-        fz_store8<T>(dp, m * N + vo + k, k, F, full, dv);
-        fz_store8<T>(dp, m * N + go + k, k, F, full, dt);
+        fz_store8<T>(dp, m * N + vo + k, k, F, FULL, dv);
+        fz_store8<T>(dp, m * N + go + k, k, F, FULL, dt);
       }
       if (dps) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) dv[e] *= sv[e], dt[e] *= st[e];
-        fz_store8<E>(dps, m * lds + vo + k, k, F, full, dv);
-        fz_store8<E>(dps, m * lds + go + k, k, F, full, dt);
-        if (k + 8 >= F)  // the product reads whole 16-byte chunks
+        fz_store8<E>(dps, m * lds + vo + k, k, F, FULL, dv);
+        fz_store8<E>(dps, m * lds + go + k, k, F, FULL, dt);
+        if (!FULL && k + 8 >= F)  // the product reads whole 16-byte chunks
           for (int64_t c = N; c < lds; ++c) dps[m * lds + c] = (E)0.f;
       }
     }
-  }
+  };
+  if (full) fz_for_act(act, [&](auto ac) { each(ac, std::true_type{}); });
+  else if (k < F) fz_for_act(act, [&](auto ac) { each(ac, std::false_type{}); });
   if (!part) return;
   for (int i = 0; i < 8; ++i) {  // rows of threads one after the other
     if (ty == i) {
@@ -250,8 +254,8 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
     __syncthreads();
   }
   for (int h = 0; h < 2; ++h) {
-    const int c = blockIdx.x * DG_COLS + threadIdx.x;
-    if (c < F) part[(int64_t)blockIdx.y * N + (h ? go : vo) + c] = sums[h][threadIdx.x];
+    const int c = c0 + (int)threadIdx.x;
+    if (c < F) part[(int64_t)slab * N + (h ? go : vo) + c] = sums[h][threadIdx.x];
   }
 }
 // the partial rows' sum: 8 threads a column, joined in a fixed order

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(W * 64) void fz_skinny_kernel(const TI* __restrict_
       }
     }
     float y = v[0];
-    if constexpr (GATED) y *= fz_act(ep.act, v[H - 1]);
+    if constexpr (GATED) fz_for_act(ep.act, [&](auto ac) { y *= fz_act<decltype(ac)::value>(v[H - 1]); });
     static_cast<TO*>(ep.out)[(int64_t)m * NO + n] = (TO)y;
   }
 }

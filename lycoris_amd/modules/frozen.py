@@ -18,6 +18,11 @@ def _stock(layer, forward):
     return getattr(forward, "__func__", None) is type(layer).forward and getattr(forward, "__self__", None) is layer
 
 
+def _hooked(layer):
+    """does calling the layer do more than its forward?"""
+    return any(getattr(layer, n, None) for n in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
+
+
 class Int8Linear(nn.Linear):
     """nn.Linear with its weight as 8-bit integers and one scale an output channel; frozen.
 
@@ -78,7 +83,7 @@ class GatedLinear(nn.Module):
 
     ``proj`` is an nn.Linear or Int8Linear with 2 F outputs; the value half comes first unless ``gate_first``.  Adapters on ``proj`` (it
     keeps that name, which is also diffusers') are evaluated as its `base` operand when they are plain -- no dropout active, no weight
-    decomposition -- and by calling proj itself otherwise; the result is the same function."""
+    decomposition, no hooks on proj -- and by calling proj itself otherwise; the result is the same function."""
 
     def __init__(self, proj: nn.Linear, act: str = "gelu", gate_first: bool = False):
         super().__init__()
@@ -103,7 +108,8 @@ class GatedLinear(nn.Module):
 
     def forward(self, x):
         proj, held = self.proj, isinstance(self.proj, Int8Linear)
-        adapters = self._adapters() if type(proj) in (nn.Linear, Int8Linear) and not getattr(proj, "parametrizations", None) else None
+        plain = type(proj) in (nn.Linear, Int8Linear) and not _hooked(proj) and not getattr(proj, "parametrizations", None)
+        adapters = self._adapters() if plain else None
         if adapters is None:
             first, second = proj(x).chunk(2, -1)
             value, gate = (second, first) if self.gate_first else (first, second)
@@ -119,12 +125,14 @@ class GatedLinear(nn.Module):
 
 def quantize_frozen(model: nn.Module, where=None) -> list:
     """Replace every plain nn.Linear of `model` (those for which ``where(name, layer)`` holds) by the Int8Linear it becomes; returns the
-    names.  To be called before the network's adapters are created; a layer that already carries one is refused."""
+    names.  To be called before the network's adapters are created; a layer that already carries one, or hooks, is refused."""
     from .base import _STACK
     found = [(name, layer) for name, layer in model.named_modules() if name and type(layer) is nn.Linear and (where is None or where(name, layer))]
     for name, layer in found:
         if hasattr(layer, _STACK) or not _stock(layer, layer.forward) or getattr(layer, "parametrizations", None):
             raise RuntimeError(f"quantize_frozen: {name} already carries an adapter; quantise the model before the network is created")
+        if _hooked(layer):
+            raise RuntimeError(f"quantize_frozen: {name} carries hooks, which its replacement would lose; register them afterwards")
     made = {}  # a layer shared under several names stays shared
     for name, layer in found:
         made.setdefault(id(layer), None)

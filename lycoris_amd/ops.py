@@ -915,7 +915,7 @@ def int8_linear(x, wq, w_scale, bias=None, base=None):
 
     Differentiable in x and base.  The gradient is not quantised: dx = g (w_scale wq), the derivative of the layer with its weight as it is
     held, with the rounding of x passed straight through.  The weight, its scale and the bias are frozen (a bias or scale that requires a
-    gradient is refused).  K is limited to 2^17."""
+    gradient is refused).  K is below 2^17, and x has at most 2^26 rows."""
     x = _amp(x)
     if base is not None and base.dtype != x.dtype:
         base = base.to(x.dtype)
@@ -930,8 +930,8 @@ def gated_linear(x, weight, bias=None, base=None, act="gelu", gate_first=False, 
     comes first (diffusion feed-forwards) unless `gate_first` (stacked gate / up projections).
 
     weight in x's dtype, trainable or frozen, or int8 with `weight_scale` [2 F] (int8_quantize of its rows): x is then quantised row by row
-    as in int8_linear.  Differentiable in x, base, bias and an unquantised weight; the backward pass reads p, kept rounded to x's dtype, and
-    an 8-bit weight's gradient dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products (24 bits)."""
+    as in int8_linear.  Differentiable in x, base, bias and an unquantised weight.  The backward pass reads p in 24 bits (fp32: as it is),
+    3 M 2 F bytes kept from the forward; over an 8-bit weight dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products (24 bits)."""
     if act not in ACTIVATIONS:
         raise ValueError(f"gated_linear: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     x = _amp(x)

@@ -91,6 +91,8 @@ def test_c_abi_refuses_before_any_launch():
            ("lyc_int8_quantize", (None, 8, p, 16, p, 2, 8, bf, None), "null"), ("lyc_int8_quantize", (p, 4, p, 16, p, 2, 8, bf, None), "pitch of x"),
            ("lyc_int8_quantize", (p, 8, p, 24, p, 2, 8, bf, None), "multiple of 16"), ("lyc_int8_quantize", (p, 8, p + 8, 16, p, 2, 8, bf, None), "aligned"),
            ("lyc_int8_quantize", (p, 1 << 18, p, 1 << 18, p, 2, 1 << 18, bf, None), "exceed"),
+           ("lyc_int8_quantize", (p, 8, p, 16, p, (1 << 26) + 1, 8, bf, None), "exceed"),
+           ("lyc_int8_matmul", (p, 1 << 17, p, p, 1 << 17, p, None, 0, None, p, p, 2, 3, 1 << 17, bf, None), "exceed"),  # 2^17 (-128)^2 = 2^31
            ("lyc_int8_matmul", (p, 16, p, p, 8, p, None, 0, None, p, p, 2, 3, 8, bf, None), "multiple of 16"),
            ("lyc_int8_matmul", (p, 16, None, p, 16, p, None, 0, None, p, p, 2, 3, 8, bf, None), "null"),
            ("lyc_int8_linear_fwd", (p, p, 16, p, None, 0, None, p, None, 64, 3, 8, bf, None), "workspace"),
@@ -232,6 +234,13 @@ def test_gated_layer_falls_back_to_the_projection_itself():
     assert torch.allclose(got, v * nn.functional.silu(t), atol=1e-5) and not torch.allclose(got, want, atol=1e-3)
     m.restore()
     assert layer._adapters() == [] and torch.equal(layer(x), want)
+    seen = []
+    hook = proj.register_forward_hook(lambda mod, args, out: seen.append(out) or out + 1)
+    t, v = proj(x).chunk(2, -1)
+    assert torch.allclose(layer(x), v * nn.functional.silu(t), atol=1e-6) and len(seen) == 2
+    with pytest.raises(RuntimeError, match="hooks"):
+        quantize_frozen(layer)
+    hook.remove()
     proj.forward = lambda x: nn.functional.linear(x, proj.weight * 2, proj.bias)  # somebody else's patch
     t, v = proj(x).chunk(2, -1)
     assert torch.allclose(layer(x), v * nn.functional.silu(t), atol=1e-6)

@@ -4,8 +4,8 @@ the formulas in 64 bits on the same inputs.
 Bounds are elementwise and come from the arithmetic.  u = eps / 2 of the activation type is one rounding to it, e = 2^-24 one rounding to
 fp32.  A sum of n fp32 terms is off by at most n e times the sum of their magnitudes S.  8-bit products are exact integers below 2^31, so
 the 8-bit forward has no n: converting, two scales, bias and base are five roundings.  fp32 operands run as six bf16 products per term
-(what is left out is below 3 e of a term): 6 n e S.  The backward pass reads p rounded to the activation type (u |p|) and, from an 8-bit
-weight, sw q rounded to it (u S)."""
+(what is left out is below 3 e of a term): 6 n e S.  The backward pass reads p cut to its upper 24 bits (2^-15 |p|; fp32: as it is) and, over
+an 8-bit weight, sw q or sw dp rounded to the activation type (u S)."""
 import math
 
 import pytest
@@ -103,6 +103,9 @@ def test_quantize_halves_zeros_extremes_and_non_finite_rows(dt):
 def test_quantize_strided_and_misaligned_rows():
     gen = torch.Generator().manual_seed(5)
     big = rnd(gen, (40, 300), torch.bfloat16)
+    column = rnd(gen, (300, 1), torch.bfloat16)
+    q, s = ops.int8_quantize(column.t())  # one row whose pitch is 1
+    assert torch.equal(q.cpu().double(), quantize64(column.t())[0])
     for x in (big[:, 3:203], big[::2, :128], big.t(), big[:, ::2], big[5:6].expand(4, 300), big[:, 8:264]):
         q, s = ops.int8_quantize(x)
         q64, s64 = quantize64(x)
@@ -292,7 +295,8 @@ def gated_reference(x, w64, bias, base, act, gate_first, g, dt, held_weight, p_o
     if g is None:
         return out
     g64 = f64(g).reshape(-1, F)
-    ev, et = ev + u * (v.abs() + ev) + sub_of(dt), et + u * (t.abs() + et) + sub_of(dt)
+    cut = 0.0 if dt == torch.float32 else 2.0 ** -15  # 24 bits: sign, 8 of exponent, 15 of the fraction
+    ev, et = ev + cut * (v.abs() + ev), et + cut * (t.abs() + et)
     dv, dt_ = g64 * a, g64 * v * da
     edv = g64.abs() * (1.2 * et + afp + E * a.abs())
     edt = g64.abs() * ((da.abs() + afp) * ev + (v.abs() + ev) * (1.0 * et + afp) + 3 * E * (v * da).abs())
@@ -402,6 +406,11 @@ def test_gated_large_gates_and_non_finite_rows():
             within(y, 2 * ref[0], ACT_ERR * 2 * ref[0].abs() + u_of(dt) * 2.01 * ref[0].abs() + 1e-18, act)
             d, = torch.autograd.grad(y, base, torch.ones_like(y))
             within(d[:, 8:], 2 * ref[1], 1e-4 * ref[1].abs() + u_of(dt) * 2.01 * ref[1].abs() + 1e-15, act)
+            if dt != torch.float16:  # t^2 and t^3 beyond fp32: the derivative is 1 or 0
+                far = torch.tensor([1e20, -1e20, 1e30, -1e30], dtype=dt, device=DEV).repeat(4, 2)
+                far = torch.cat((torch.ones_like(far), far), 1).requires_grad_(True)
+                d, = torch.autograd.grad(ops.gated_linear(x, w, base=far, act=act).float().sum(), far)
+                assert torch.equal(d[:, 8:].float(), (far[:, 8:] > 0).float()), act
     gen = torch.Generator().manual_seed(1)
     x, w = rnd(gen, (20, 64), torch.bfloat16), rnd(gen, (64, 64), torch.bfloat16, 0.1)
     want = ops.gated_linear(x, w)
@@ -484,6 +493,27 @@ def test_outputs_past_32_bit_offsets():
     g[rows] = 1.0
     dx, dw = torch.autograd.grad(h, [xl, wl], g)
     want = gated_reference(x[rows], f64(w), None, None, "silu", False, g[rows], torch.bfloat16, False)
+    within(h[rows], *want["y"], "h")
+    within(dx[rows], *want["dx"], "dx")
+    within(dw, *want["dw"], "dw")  # the other rows' gradient is zero
+
+
+def test_many_rows():
+    """more rows than a launch of a workgroup a row, or a grid's second dimension, would take"""
+    M, K, F = (1 << 22) + 101, 16, 8
+    gen = torch.Generator().manual_seed(21)
+    x = torch.randn(M, K, dtype=torch.bfloat16, device=DEV)
+    rows = torch.tensor([0, (1 << 22) - 1, 1 << 22, M - 1], device=DEV)
+    q, s = ops.int8_quantize(x)
+    q64, s64 = quantize64(x[rows])
+    assert torch.equal(f64(q[rows]), q64) and torch.equal(f64(s[rows]), s64[:, 0])
+    w = rnd(gen, (2 * F, K), torch.bfloat16, 0.25)
+    xl, wl = x.requires_grad_(True), w.requires_grad_(True)
+    h = ops.gated_linear(xl, wl, act="gelu_tanh")
+    g = torch.zeros_like(h)
+    g[rows] = 1.0
+    dx, dw = torch.autograd.grad(h, [xl, wl], g)
+    want = gated_reference(x[rows], f64(w), None, None, "gelu_tanh", False, g[rows], torch.bfloat16, False)
     within(h[rows], *want["y"], "h")
     within(dx[rows], *want["dx"], "dx")
     within(dw, *want["dw"], "dw")  # the other rows' gradient is zero
