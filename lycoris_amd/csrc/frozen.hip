@@ -1,6 +1,7 @@
 // frozen.hip -- C ABI of the 8-bit frozen layer and the gated projection (include/lycoris_amd.h).  gfx950 only.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/lycoris_amd.h"
@@ -217,14 +218,6 @@ int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, 
   return check_launch("int8_quantize");
 }
 
-// x [rows, cols] contiguous -> NP planes of [rows, up(cols, 8)]
-template <typename TI, typename TO, int NP>
-int launch_stage(const TI* x, const float* col, TO* out, int64_t rows, int64_t cols, hipStream_t st) {
-  const int64_t ldo = up(cols, 8);
-  const int vec = fz_al16(x) && cols % 8 == 0;
-  hipLaunchKernelGGL((fz_stage_kernel<TI, TO, NP>), dim3(grid_of(rows * ldo / 8)), dim3(256), 0, st, x, col, out, ldo, rows, (int)cols, vec);
-  return check_launch("stage");
-}
 template <typename T>
 int launch_plane(const int8_t* q, int64_t ldq, const float* sw, const float* f, T* out, int64_t O, int64_t I, hipStream_t st) {
   const int rows = 4;
@@ -241,10 +234,27 @@ int launch_range(const float* sw, int64_t n, int top, float* f, const float** ou
   return check_launch("scale range");
 }
 
+// The operands of a pass that have to be staged, and their one launch
+template <typename T>
+struct Stages {
+  using E = typename std::conditional<sizeof(T) == 4, __bf16, T>::type;
+  FzStage list;
+  int n = 0;
+  int64_t most = 0;
+  void add(const T* x, const float* col, void* out, int64_t rows, int64_t cols) {
+    list.job[n++] = FzStageJob{x, col, out, rows, (int)cols, fz_al16(x) && cols % 8 == 0};
+    most = std::max(most, rows * cdiv(cols, 8));
+  }
+  int run(hipStream_t st) {
+    if (!n) return LYC_OK;
+    hipLaunchKernelGGL((fz_stage_kernel<T, E, sizeof(T) == 4 ? 3 : 1>), dim3(grid_of(most), n), dim3(256), 0, st, list);
+    return check_launch("stage");
+  }
+};
 // One operand of a product in the type the matrix cores take: the tensor itself, its staged copy, or its three bf16 planes.
 template <typename T>
 struct Operand {
-  using E = typename std::conditional<sizeof(T) == 4, __bf16, T>::type;
+  using E = typename Stages<T>::E;
   const void* p = nullptr;
   int64_t ld = 0, plane = 0;  // bytes
   void* room = nullptr;
@@ -253,16 +263,12 @@ struct Operand {
   Operand(Carve& ws, int64_t rows_, int64_t cols_, bool wanted) : rows(rows_), cols(cols_), own(sizeof(T) == 4 || cols_ % 8 != 0) {
     if (wanted && own) room = ws.take<E>((sizeof(T) == 4 ? 3 : 1) * rows * up(cols, 8));
   }
-  int fill(const T* x, const float* col, hipStream_t st) {
-    if (!own) {
-      p = x;
-      ld = cols * (int64_t)sizeof(T);
-      return LYC_OK;
-    }
-    p = room;
-    ld = up(cols, 8) * 2;
-    plane = rows * ld;
-    return launch_stage<T, E, sizeof(T) == 4 ? 3 : 1>(x, col, static_cast<E*>(room), rows, cols, st);
+  // x [rows, cols], contiguous; to be read after `stages` has run
+  void fill(const T* x, const float* col, Stages<T>& stages) {
+    p = own ? room : x;
+    ld = own ? up(cols, 8) * 2 : cols * (int64_t)sizeof(T);
+    plane = own ? rows * ld : 0;
+    if (own) stages.add(x, col, room, rows, cols);
   }
 };
 // segments: 16-bit 1; fp32 x fp32 6; fp32 x exact bf16 (an 8-bit weight's integers) 3.  The small terms come first.
@@ -320,7 +326,9 @@ int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve
   const float* range;
   FZ_TRY(launch_range<E>(sw, N, 14, f, &range, st));
   FZ_TRY(launch_plane<E>(wq, ldw, F32 ? nullptr : sw, range, plane, N, K, st));
-  FZ_TRY(a.fill(g, F32 ? sw : nullptr, st));
+  Stages<T> stages;
+  a.fill(g, F32 ? sw : nullptr, stages);
+  FZ_TRY(stages.run(st));
   FzProb p = prob(a.p, a.ld, a.plane, plane, up(K, 8) * 2, 0, M, K, N, 2);
   segments(p, F32 ? 3 : 1);
   FzEpi ep{};
@@ -369,8 +377,10 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
     *bytes = ws.used;
     return LYC_OK;
   }
-  FZ_TRY(a.fill(x, nullptr, st));
-  FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
+  Stages<T> stages;
+  a.fill(x, nullptr, stages);
+  b.fill(static_cast<const T*>(q.w), nullptr, stages);
+  FZ_TRY(stages.run(st));
   FzProb p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, 2 * q.F, q.I, 2);
   segments(p, sizeof(T) == 4 ? 6 : 1);
   if constexpr (sizeof(T) == 2) {
@@ -416,7 +426,11 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)(cdiv(q.F, DG_COLS) * parts)), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
                      (int)q.F, q.act, q.gate_first, vec, rows);
   FZ_TRY(check_launch("gated backward"));
-  if (want_dw || (want_dx && !scaled)) FZ_TRY(a.fill(dp, F32 && held ? q.sw : nullptr, st));
+  Stages<T> stages;
+  if (want_dw || (want_dx && !scaled)) a.fill(dp, F32 && held ? q.sw : nullptr, stages);
+  if (want_dx && !held) b.fill(static_cast<const T*>(q.w), nullptr, stages);
+  if (want_dw) xo.fill(x, nullptr, stages);
+  FZ_TRY(stages.run(st));
   if (want_dx) {
     FzEpi ep{};
     ep.out = dx;
@@ -427,14 +441,12 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
       else p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
       ep.alpha = range ? range + 1 : nullptr;
     } else {
-      FZ_TRY(b.fill(static_cast<const T*>(q.w), nullptr, st));
       p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, q.I, N, 2);
     }
     segments(p, F32 ? (held ? 3 : 6) : 1);
     FZ_TRY((launch_gemm<E, T, false, true, FZ_PLAIN>(pdx, p, ep, sums, st)));
   }
   if (want_dw) {
-    FZ_TRY(xo.fill(x, nullptr, st));
     FzProb p = prob(a.p, a.ld, a.plane, xo.p, xo.ld, xo.plane, N, q.I, q.M, 2);
     segments(p, F32 ? 6 : 1);
     FzEpi ep{};

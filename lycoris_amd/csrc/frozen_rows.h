@@ -153,18 +153,30 @@ __global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict_
 // ---- staging: a row matrix into 16-byte aligned rows of 16-bit elements, NP planes -----------------------------------------------------
 // NP = 1: a copy (rows whose length or base is not a multiple of 16 bytes).  NP = 3, fp32: x = h + m + l in bf16, each the rounding of
 // what the ones before left; `col` scales the columns first.  Columns cols .. ldo are zeros.
+// One launch stages up to three operands, one per blockIdx.y.
+struct FzStageJob {
+  const void* x;
+  const float* col;
+  void* out;
+  int64_t rows;
+  int cols, vec;
+};
+struct FzStage {
+  FzStageJob job[3];
+};
 template <typename TI, typename TO, int NP>
-__global__ __launch_bounds__(256) void fz_stage_kernel(const TI* __restrict__ x, const float* __restrict__ col, TO* __restrict__ out, int64_t ldo, int64_t rows,
-                                                       int cols, int vec) {
-  const int64_t chunks = ldo >> 3, n = rows * chunks, plane = rows * ldo;
+__global__ __launch_bounds__(256) void fz_stage_kernel(FzStage jobs) {
+  const FzStageJob& j = jobs.job[blockIdx.y];
+  const TI* x = static_cast<const TI*>(j.x);
+  const int64_t chunks = (j.cols + 7) >> 3, ldo = chunks * 8, n = j.rows * chunks, plane = j.rows * ldo;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / chunks;
     const int k = (int)(i - r * chunks) * 8;
     float v[8];
-    fz_row8<TI>(x + r * cols, k, cols, vec, v);
-    if (col) {
+    fz_row8<TI>(x + r * j.cols, k, j.cols, j.vec, v);
+    if (j.col) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= k + e < cols ? col[k + e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] *= k + e < j.cols ? j.col[k + e] : 0.f;
     }
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
@@ -175,7 +187,7 @@ __global__ __launch_bounds__(256) void fz_stage_kernel(const TI* __restrict__ x,
         const float h = (float)t[e];
         v[e] = fabsf(h) <= 3.4e38f ? v[e] - h : 0.f;
       }
-      *reinterpret_cast<u32x4*>(out + p * plane + r * ldo + k) = *reinterpret_cast<u32x4*>(t);
+      *reinterpret_cast<u32x4*>(static_cast<TO*>(j.out) + p * plane + r * ldo + k) = *reinterpret_cast<u32x4*>(t);
     }
   }
 }
