@@ -767,16 +767,24 @@ __global__ __launch_bounds__(256) void fz_reduce_kernel(FzProb p, FzEpi ep) {
     S s[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = 0;
-    for (int z = 0; z < p.ksplit; ++z, src += plane) {
-      if (pitch8) {
-        const u32x4 a = reinterpret_cast<const u32x4*>(src)[0], b = reinterpret_cast<const u32x4*>(src)[1];
+    for (int z0 = 0; z0 < p.ksplit; z0 += 4) {  // four parts' loads in flight: what lies beyond the last part or column is read again, not used
+      S part[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += __builtin_bit_cast(S, e < 4 ? a[e & 3] : b[e & 3]);
-      } else {
+      for (int z = 0; z < 4; ++z) {
+        const S* at = src + min(z0 + z, p.ksplit - 1) * plane;
+        if (pitch8) {
+          const u32x4 a = reinterpret_cast<const u32x4*>(at)[0], b = reinterpret_cast<const u32x4*>(at)[1];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < N) s[e] += src[e];
+          for (int e = 0; e < 8; ++e) part[z][e] = __builtin_bit_cast(S, e < 4 ? a[e & 3] : b[e & 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part[z][e] = at[min(e, N - 1 - n)];
+        }
       }
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += z0 + z < p.ksplit ? part[z][e] : 0;
     }
     float v[8], t[8];
 #pragma unroll
