@@ -8,6 +8,9 @@
 //
 // FUSED (8-bit, few activations): every workgroup quantises the rows itself into LDS while its first weight pieces are in flight -- one
 // launch instead of two.  The rows are read by all workgroups, out of the L2, so this pays while they are small beside the weight slice.
+//
+// Measured: 1 x 1280 -> 1280 in 5.3 us and gated 1 x 1280 -> 2 x 5120 (13 MB) in 7.1, quantisation included; 16 x 4096 -> 4096 (17 MB) in 5.4 - 6.8
+// behind a quantisation of 3.7.  An empty launch takes about 4.
 #pragma once
 #include "frozen_rows.h"
 
