@@ -61,11 +61,12 @@ class Int8Linear(nn.Linear):
         return (self.wq.float() * self.weight_scale[:, None]).to(self.dtype)
 
     def _apply(self, fn, recurse=True):
-        # .half() / .to(dtype) set the dtype the layer stands for; the scales stay fp32
+        # .half() / .to(dtype) set the dtype the layer stands for; the scales stay the fp32 they were
+        scale = self.weight_scale
         super()._apply(fn, recurse)
         self.dtype = fn(torch.zeros((), dtype=self.dtype, device=self.weight_q.device)).dtype
         if self.weight_scale.dtype != torch.float32:
-            self.weight_scale = self.weight_scale.float()
+            self.weight_scale = scale.to(self.weight_scale.device)
         return self
 
     def reset_parameters(self):

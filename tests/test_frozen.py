@@ -212,6 +212,16 @@ def test_adapters_on_an_int8_gated_block(algo):
         assert torch.allclose(a, b, atol=1e-4 * float(b.detach().abs().max()) + 1e-6)
 
 
+def test_casting_an_int8_layer_keeps_its_scales():
+    layer = Int8Linear.from_linear(nn.Linear(40, 24))
+    scale, q = layer.weight_scale.clone(), layer.weight_q.clone()
+    for cast in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.float(), lambda m: m.to("cpu"), lambda m: m.double()):
+        cast(layer)
+        assert torch.equal(layer.weight_scale, scale) and layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_q, q)
+        assert layer.weight.dtype == layer.bias.dtype == layer.dtype
+    assert layer.to(device="meta").weight_scale.device.type == "meta"
+
+
 def test_gated_layer_falls_back_to_the_projection_itself():
     torch.manual_seed(4)
     proj = nn.Linear(8, 12)
