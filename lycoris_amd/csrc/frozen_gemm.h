@@ -217,6 +217,15 @@ struct FzOperand {
       }
     }
   }
+  // the byte offset of line part + S i of the tile's K step (K-strided: 128 bytes of a k row, of whole steps only), beyond the tile: K4_OOB
+  template <int S>
+  __device__ __forceinline__ unsigned ahead(int part, int i, int64_t ld, int r0, int ext) const {
+    const int l = part + S * i;
+    if constexpr (!KS) return l < ROWS && r0 + l < ext ? (unsigned)l * (unsigned)ld : K4_OOB;
+    constexpr int LINES = (PITCH + 127) / 128;
+    const int kr = l / LINES, c = l % LINES;
+    return kr < KROWS && r0 + 64 * c < ext ? (unsigned)kr * (unsigned)ld + 128u * c : K4_OOB;
+  }
   __device__ __forceinline__ void seek(int64_t plane_off) { cur = org + plane_off; }
   // the next K step: the descriptor is rebased to it (an operand may exceed 4 GiB; rows and columns are masked in the lane offsets, so any
   // size will do).  last: what lies beyond K reads as zero, by the lanes' chunks or by the descriptor's end; dead: nothing is left to fetch,
@@ -393,9 +402,16 @@ struct FzKernel {
   static constexpr bool GATED = EPI == FZ_GATED;
   using OA = FzOperand<BM, WR, NW, SB, A_KS, false, false>;
   using OB = FzOperand<BN, WC, NW, SB, B_KS, true, GATED>;
-  static constexpr int STAGE = OA::SLOT + OB::SLOT, LDS = D * STAGE + (OA::SPARE || OB::SPARE ? 1024 : 0);
+  static constexpr int STAGE = OA::SLOT + OB::SLOT, SPARE = OA::SPARE || OB::SPARE ? 1024 : 0;
+  // Two slots of 64 KiB are the whole LDS, and what HBM takes to deliver the next one shows.  The 256 x 256 tile's waves therefore ask for one
+  // word of every cache line of the slot PFD ahead of the one they fill (into spare LDS: nobody reads it), so that the lines are in the
+  // L2 when their turn comes.  The workgroups of an XCD that share rows share them out: 8 row tiles those of B, 4 columns of tiles
+  // those of A, one instruction a wave and slot.  dx 4096 x 1280, K = 10240 in three parts: 124 -> 105 us.  Not for other tiles (deeper
+  // rings or a second workgroup hide the same: 0 to 3 % slower with it), and not for K of fewer than FAR slots (16384 x 5120, K = 1280: 190 -> 195).
+  static constexpr int PF = SB == 128 && BM * BN == 256 * 256 && !GATED, PFD = 2, FAR = 32;
+  static constexpr int LDS = D * STAGE + SPARE + (PF ? 256 : 0);
   static constexpr int MI = OA::NT, NI = OB::NT, C = OA::PPW + OB::PPW;
-  static_assert(D >= (SB == 64 ? 4 : 2) && (D - 1) * C <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
+  static_assert(D >= (SB == 64 ? 4 : 2) && (D - 1) * (C + 1) <= 63 && (FE<E>::SIZE == 2 || (!A_KS && !B_KS)), "ring");
 
   static __device__ __forceinline__ void run(const FzProb& p, const FzEpi& ep, char* smem, int b, int z) {
     const int NO = GATED ? ep.F : p.N;
@@ -447,12 +463,27 @@ struct FzKernel {
       const bool last = --left == 0, dead = todo-- <= 0;
       return Steps{oa.next(last, dead), ob.next(last, dead)};
     };
+    const bool far = PF && slots >= FAR, ofb = wave & 1;  // odd waves: B's lines
+    unsigned line = K4_OOB;
+    if constexpr (PF) {
+      const int i = (wave >> 1) + NW / 2 * lane;
+      line = ofb ? ob.template ahead<8>(tm & 7, i, p.ldb, n0, p.N) : oa.template ahead<4>(tn & 3, i, p.lda, m0, p.M);
+    }
+    auto fetch_ahead = [&]() {  // behind the slot that next() has just given; an operation in any case, the waits count it
+      if constexpr (PF) {
+        const char *const la = oa.cur + (int64_t)(PFD - 1) * oa.kstep, *const lb = ob.cur + (int64_t)(PFD - 1) * ob.kstep;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(ofb ? lb : la), 0,
+                                                                            far && todo >= 0 && left > PFD ? 0x7fffffff : 0, K4_RSRC_FLAGS);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (k4_lds_ptr)(smem + D * STAGE + SPARE), 4, (int)line, 0, 0, 0);
+      }
+    };
     char *const wslot = smem + wave * 1024, *const spare = smem + D * STAGE;  // this wave's first DMA piece of slot 0
     constexpr int AHEAD = D == 2 ? 2 : D - 1;  // slots filled before the loop
     for (int s = 0; s < AHEAD; ++s) {
       const Steps n = next();
       oa.issue(n.a, wslot + s * STAGE, spare);
       ob.issue(n.b, wslot + s * STAGE + OA::SLOT, spare);
+      fetch_ahead();
     }
 
     using Acc = typename FE<E>::acc;
@@ -477,7 +508,7 @@ struct FzKernel {
       if constexpr (I < RB) ob.template read<H, I>(sb, f.b);
       else oa.template read<H, I - RB>(sb, f.a);
     };
-    k4_wait_vm<(AHEAD - 1) * C>();
+    k4_wait_vm<(AHEAD - 1) * (C + PF) + PF>();  // (PF: of the operations behind a slot's own, fetch_ahead's)
     __builtin_amdgcn_s_barrier();  // raw: __syncthreads() would drain the DMA queue
     asm volatile("" ::: "memory");
     g16d_for_each([&](auto ic) { read_one(std::integral_constant<int, 0>{}, ic, sbase, f0); }, std::make_integer_sequence<int, R>{});
@@ -536,8 +567,9 @@ struct FzKernel {
       for (int s = 0; s < slots; ++s) {
         const Steps n = next();
         compute(f0, f1, std::integral_constant<int, OA::HALVES - 1>{}, sbase + (unsigned)at, n, wslot, I0{}, I0{});
-        meet(I0{});
+        meet(std::integral_constant<int, PF>{});
         compute(f1, f0, I0{}, sbase + (unsigned)(STAGE - at), n, wslot + at, I0{}, IC{});
+        fetch_ahead();
         at = STAGE - at;
       }
     } else {
@@ -550,10 +582,11 @@ struct FzKernel {
         const unsigned sb = sbase + (unsigned)read_at;
         read_at = advance(read_at);
         const Steps n = next();
-        meet(std::integral_constant<int, (D - 3) * C>{});
+        meet(std::integral_constant<int, (D - 3) * (C + PF) + PF>{});
         using IH = std::integral_constant<int, C / 2>;
         compute(f0, f1, std::integral_constant<int, OA::HALVES - 1>{}, sb, n, fill, I0{}, IH{});
         compute(f1, f0, I0{}, sbase + (unsigned)read_at, n, fill, IH{}, IC{});
+        fetch_ahead();
       }
     }
     // the reads and refills behind the last step have landed before their registers and LDS are given up

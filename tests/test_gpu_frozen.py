@@ -161,6 +161,28 @@ def test_linear_forward_and_dx(M, K, N, dt):
         assert torch.equal(ops.int8_linear(x, wq, sw, bias, base), y)
 
 
+@pytest.mark.parametrize("M,K,N,dt", [(3850, 5130, 3900, torch.bfloat16), (4090, 1276, 10250, torch.bfloat16), (4090, 1276, 10250, torch.float32)],
+                         ids=["large", "long", "long_f32"])
+def test_long_ragged_products(M, K, N, dt):
+    """the largest tiles over many K steps, in one part and in several, with rows, columns and K that end inside a tile"""
+    gen = torch.Generator(device=DEV).manual_seed(M)
+    x, g = (torch.randn(M, n, generator=gen, device=DEV).to(dt) for n in (K, N))
+    wq, sw = ops.int8_quantize(torch.randn(N, K, generator=gen, device=DEV) / math.sqrt(K))
+    poison()
+    xl = x.clone().requires_grad_(True)
+    y = ops.int8_linear(xl, wq, sw)
+    dx, = torch.autograd.grad(y, xl, g)
+    assert torch.isfinite(y).all() and torch.isfinite(dx).all()
+    rows = torch.cat((torch.arange(0, M, 97), torch.tensor([255, 256, M - 2, M - 1]))).to(DEV)
+    want, err = linear_reference(x[rows], wq, sw, None, None)
+    within(y[rows], want, err + u_of(dt) * (want.abs() + err), "y")
+    w64, g64 = f64(wq) * f64(sw)[:, None], f64(g[rows])
+    want, S = g64 @ w64, g64.abs() @ w64.abs()
+    u = u_of(dt)
+    rel = (u + (N + 2) * E) if dt != torch.float32 else (3 * N + 8) * E
+    within(dx[rows], want, rel * S * 1.01 + u * want.abs(), "dx")
+
+
 def test_linear_operands_of_other_layouts():
     gen = torch.Generator().manual_seed(3)
     M, K, N = 50, 203, 96
