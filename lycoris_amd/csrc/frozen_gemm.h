@@ -664,17 +664,17 @@ struct FzKernel {
           if (GATED) fz_bias<TO, CN>(ep, grow + n, n, NO, vec, c2);
         }
       }
-      auto fetch = [&](const __amdgpu_buffer_rsrc_t& r, unsigned off, float (&x)[CN]) {  // adds
-        TO t[CN];
+      struct Row {
+        TO x[CN];
+      };
+      auto fetch = [&](const __amdgpu_buffer_rsrc_t& r, unsigned off, Row& t) {
         if constexpr (TS * CN == 8) {
-          reinterpret_cast<u32x2*>(t)[0] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+          reinterpret_cast<u32x2*>(t.x)[0] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
         } else {
 #pragma unroll
           for (int i = 0; i < TS * CN / 16; ++i)
-            reinterpret_cast<u32x4*>(t)[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, 0));
+            reinterpret_cast<u32x4*>(t.x)[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, 0));
         }
-#pragma unroll
-        for (int e = 0; e < CN; ++e) x[e] += (float)t[e];
       };
       auto store = [&](const __amdgpu_buffer_rsrc_t& r, unsigned off, const float (&x)[CN]) {
         TO t[CN];
@@ -700,10 +700,21 @@ struct FzKernel {
           }
         }
       };
+      // the base operand of GR row tiles is asked for at once: behind a store the next load would wait for itself
+      constexpr int GR = TS == 2 ? (MI < 4 ? MI : 4) : 2;
+      Row bv[GR], bt[GR];
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) {
         const int r = row0 + 16 * mi;
         const int64_t m = m0 + r;
+        if (EPI != FZ_PLAIN && vec && ep.base && mi % GR == 0) {
+#pragma unroll
+          for (int j = 0; j < GR; ++j) {
+            const unsigned off = in ? (unsigned)((r + 16 * j) * pb + n * TS) : K4_OOB;
+            fetch(rb, off + vrow * TS, bv[j]);
+            if (GATED) fetch(rb, off + grow * TS, bt[j]);
+          }
+        }
         if (!vec && (m >= p.M || !in)) continue;
         float v[CN], t[CN];
 #pragma unroll
@@ -723,9 +734,11 @@ struct FzKernel {
           }
           if (ep.base) {
             if (vec) {
-              const unsigned off = in ? (unsigned)(r * pb + n * TS) : K4_OOB;
-              fetch(rb, off + vrow * TS, v);
-              if (GATED) fetch(rb, off + grow * TS, t);
+#pragma unroll
+              for (int e = 0; e < CN; ++e) {
+                v[e] += (float)bv[mi % GR].x[e];
+                if (GATED) t[e] += (float)bt[mi % GR].x[e];
+              }
             } else {
               float x[CN];
               fz_load<TO, CN>(ep.base, m * H * NO + vrow + n, n, NO, false, x);
