@@ -82,9 +82,10 @@ int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
 // Which tiles, and into how many parts of K, for a product of M x NO outputs and `steps` 64-byte steps of K.
 //   256 x 256, 128 x 160 (one workgroup of 8 waves a CU), 128 x 128 (two), 64 x 64 (two of 4 waves; gated: 64 x 128, one); where the tiles are
 //   few and K is long, K in parts whose sums a second launch joins.
-// The tile of 160 columns is there for outputs of 320, 640 and 1280 channels, which it cuts into as many tiles as CUs: 4096 x 1280 are 256 (dx
-// with K = 10240, inputs out of HBM: 117 us, against 161 with 128 x 128 and 256 with 256 x 256); with whole rounds of the larger tile that wins
-// (dx 16384 x 5120, K = 1280: 213 us, against 240 with 128 x 128 and 289 with 128 x 160).
+// The tile of 160 columns is there for outputs of 320, 640 and 1280 channels, which it cuts into as many tiles as CUs (dx 8192 x 640, K = 5120: 64
+// us, against 83 with 128 x 128 and 127 with 256 x 256); with whole rounds of the larger tile that wins (dx 16384 x 5120, K = 1280: 190 us,
+// against 247 and 283), and in parts of a long K (dx 4096 x 1280, K = 10240, three parts: 106 + 12 us, against 157 with 128 x 128 and 127 with
+// 128 x 160).
 // The rule compares estimates in microseconds, from sweeps of 30 shapes with inputs out of HBM: a round costs what a step costs times the
 // steps, plus what a tile's beginning and end leave exposed -- of its epilogue's bytes, at a CU's share of HBM, less where a second
 // workgroup computes meanwhile.
