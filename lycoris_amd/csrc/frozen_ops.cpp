@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -230,12 +231,30 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
 };
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return has(t) && t->requires_grad(); }
+// A leaf has one gradient accumulator for as long as any graph on it lives, bound to the stream of the first.  A backward pass captured on
+// another stream while such an eager graph lives makes the engine synchronise the two streams, which destroys the capture, and the process with
+// it when the capture ends.  Found out here, while it is still an error that can be caught.
+void capture_safe(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs) {
+    if (!t || !t->defined() || !t->is_cuda() || !t->requires_grad() || t->grad_fn()) continue;
+    const auto current = c10::hip::getCurrentHIPStream(t->device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream.has_value() || stream->id() == current.id(), what, ": a graph is being captured while an eager autograd graph on one of the "
+                "inputs, made on another stream, is alive; drop its outputs (or detach them) before the capture");
+  }
+}
+const Tensor* ref(const OptTensor& t) { return has(t) ? &*t : nullptr; }
 Tensor int8_linear_autograd(const Tensor& x, const Tensor& wq, const Tensor& sw, const OptTensor& bias, const OptTensor& base) {
   TORCH_CHECK(!wants(sw) && !wants(bias), "int8_linear: the layer is frozen, its scale and bias cannot require a gradient");
   if (eager(x) && !(c10::GradMode::is_enabled() && (wants(x) || wants(base)))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return int8_linear(x, wq, sw, bias, base);
   }
+  capture_safe({&x, ref(base)}, "int8_linear");
   return Int8LinearFn::apply(x, wq, sw, bias, base);
 }
 
@@ -384,6 +403,7 @@ Tensor gated_linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& 
                          .typed<Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool)>();
     return eager(x) ? gated_linear(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
   }
+  capture_safe({&x, &w, ref(bias), ref(base)}, "gated_linear");
   return GatedLinearFn::apply(x, w, sw, bias, base, act, gate_first);
 }
 

@@ -685,3 +685,103 @@ def test_training_step_of_adapters_on_an_int8_block(algo, dt, tol):
     for i, (a, b) in enumerate(zip(*results)):
         a, b = f64(a), f64(b)
         assert float((a - b).norm() / b.norm()) <= tol, i
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_one_tensor_in_two_places_broadcast_operands_and_recomputation(dt):
+    from torch.utils.checkpoint import checkpoint
+    gen = torch.Generator().manual_seed(31)
+    wq, sw = held(gen, 96, 96)
+    w = rnd(gen, (96, 96), dt, 0.1)
+    x, g, g2 = rnd(gen, (50, 96), dt), rnd(gen, (50, 96), dt), rnd(gen, (50, 48), dt)
+
+    def grads(f, leaves, grad):
+        leaves = [t.clone().requires_grad_(True) for t in leaves]
+        y = f(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+
+    for f, grad in ((lambda a, b: ops.int8_linear(a, wq, sw, base=b), g), (lambda a, b: ops.gated_linear(a, w, base=b), g2),
+                    (lambda a, b: ops.gated_linear(a, wq, base=b, weight_scale=sw, gate_first=True), g2)):
+        y, da, db = grads(f, [x, x], grad)  # two leaves of the same values
+        one, d = grads(lambda a: f(a, a), [x], grad)
+        assert torch.equal(one, y) and torch.equal(d, da + db)
+        again, dc = grads(lambda a: checkpoint(lambda t: f(t, t), a, use_reentrant=False), [x], grad)
+        assert torch.equal(again, y) and torch.equal(dc, d)
+        row = x[:1].clone()  # a base that every row shares
+        full, _, dfull = grads(f, [x, row.expand(50, 96).contiguous()], grad)
+        shared, _, drow = grads(lambda a, r: f(a, r.expand(50, 96)), [x, row], grad)
+        assert torch.equal(shared, full)
+        within(drow, f64(dfull).sum(0, keepdim=True), (u_of(dt) * 2 + 50 * E) * f64(dfull).abs().sum(0, keepdim=True) + 1e-30, "shared base")
+    wl = w.clone().requires_grad_(True)  # one weight in two calls
+    y = ops.gated_linear(x, wl) + ops.gated_linear(x, wl, act="silu")
+    dw, = torch.autograd.grad(y, wl, g2)
+    parts = [grads(lambda v: ops.gated_linear(x, v, act=act), [w], g2)[1] for act in ("gelu", "silu")]
+    assert torch.equal(dw, parts[0] + parts[1])
+
+
+def test_two_captured_graphs_replayed_side_by_side():
+    gen = torch.Generator().manual_seed(32)
+    wq, sw = held(gen, 640, 320)
+    inputs = [rnd(gen, (n, 320), torch.bfloat16).requires_grad_(True) for n in (700, 90)]
+    g = [rnd(gen, (t.shape[0], 320), torch.bfloat16) for t in inputs]
+
+    def step(x, grad):
+        y = ops.gated_linear(x, wq, weight_scale=sw)
+        z = ops.int8_linear(y, wq[:320], sw[:320])
+        return z.detach(), torch.autograd.grad(z, x, grad)[0]
+
+    want = [[t.clone() for t in step(x, grad)] for x, grad in zip(inputs, g)]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in inputs], [], []
+    for x, grad, st in zip(inputs, g, streams):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            step(x, grad)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(step(x, grad))
+        graphs.append(graph)
+    for _ in range(4):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+            for a in got:
+                a.zero_()
+        step(inputs[0], g[0])  # eager work between the replays
+
+
+def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
+    """(its backward pass would end the process when the capture ends: refused by the forward call)"""
+    gen = torch.Generator().manual_seed(33)
+    wq, sw = held(gen, 64, 64)
+    w = rnd(gen, (64, 64), torch.bfloat16, 0.1).requires_grad_(True)
+    x = rnd(gen, (40, 64), torch.bfloat16).requires_grad_(True)
+    alive = [ops.int8_linear(x, wq, sw), ops.gated_linear(x.detach(), w)]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        plain = x.detach() * 2
+        frozen = ops.int8_linear(x.detach(), wq, sw)  # nothing to differentiate: no matter
+        for call in (lambda: ops.int8_linear(x, wq, sw), lambda: ops.gated_linear(x, wq, weight_scale=sw), lambda: ops.gated_linear(x.detach(), w),
+                     lambda: ops.int8_linear(x.detach(), wq, sw, base=x)):
+            with pytest.raises(RuntimeError, match="eager autograd graph"):
+                call()
+    want = alive[0].detach().clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(frozen, want) and torch.equal(plain, x.detach() * 2)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):  # nothing lives: captured
+        y = ops.int8_linear(x, wq, sw)
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        y = y.detach()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
