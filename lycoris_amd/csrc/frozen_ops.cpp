@@ -231,6 +231,12 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
 };
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return has(t) && t->requires_grad(); }
+const Tensor* ref(const OptTensor& t) { return has(t) ? &*t : nullptr; }
+// A dual tensor need not require a gradient, so it has to be asked for by itself: passed below autograd, its tangent would be lost without a word.
+void no_tangent(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative; an input carries a tangent");
+}
 // A leaf has one gradient accumulator for as long as any graph on it lives, bound to the stream of the first.  A backward pass captured on
 // another stream while such an eager graph lives makes the engine synchronise the two streams, which destroys the capture, and the process with
 // it when the capture ends.  Found out here, while it is still an error that can be caught.
@@ -247,9 +253,9 @@ void capture_safe(std::initializer_list<const Tensor*> inputs, const char* what)
                 "inputs, made on another stream, is alive; drop its outputs (or detach them) before the capture");
   }
 }
-const Tensor* ref(const OptTensor& t) { return has(t) ? &*t : nullptr; }
 Tensor int8_linear_autograd(const Tensor& x, const Tensor& wq, const Tensor& sw, const OptTensor& bias, const OptTensor& base) {
   TORCH_CHECK(!wants(sw) && !wants(bias), "int8_linear: the layer is frozen, its scale and bias cannot require a gradient");
+  no_tangent({&x, &sw, ref(bias), ref(base)}, "int8_linear");
   if (eager(x) && !(c10::GradMode::is_enabled() && (wants(x) || wants(base)))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return int8_linear(x, wq, sw, bias, base);
@@ -397,6 +403,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
 };
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& sw, const OptTensor& bias, const OptTensor& base, int64_t act, bool gate_first) {
   TORCH_CHECK(!wants(sw), "gated_linear: an 8-bit weight is frozen, its scale cannot require a gradient");
+  no_tangent({&x, &w, ref(sw), ref(bias), ref(base)}, "gated_linear");
   if (!c10::GradMode::is_enabled() || !(wants(x) || wants(w) || wants(bias) || wants(base))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::gated_linear", "")

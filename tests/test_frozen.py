@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 import torch.nn as nn
 
 import lycoris_amd
@@ -259,3 +260,27 @@ def test_gated_layer_falls_back_to_the_projection_itself():
     with pytest.raises(ValueError):
         GatedLinear(nn.Linear(8, 6), act="relu")
     assert lycoris_amd.GatedLinear is GatedLinear
+
+
+def test_forward_mode_is_refused_and_not_dropped():
+    """the device operators have no jvp: a dual input, which need not require a gradient, is an error and not an output without its tangent"""
+    N.load_torch_ops()
+    ns, m = torch.ops.lycoris_amd, dict(device="meta")
+    wq, sw = torch.empty(12, 40, dtype=torch.int8, **m), torch.empty(12, **m)
+    x, w, bias, base = torch.empty(5, 40, **m), torch.empty(12, 40, **m), torch.empty(12, **m), torch.empty(5, 12, **m)
+    calls = [(lambda x, sw, bias, base: ns.int8_linear(x, wq, sw, bias, base), (x, sw, bias, base)),
+             (lambda x, sw, bias, base: ns.gated_linear(x, wq, sw, bias, base, 0, False), (x, sw, bias, base)),
+             (lambda x, w, bias, base: ns.gated_linear(x, w, None, bias, base, 0, False), (x, w, bias, base))]
+    for call, args in calls:
+        for i in range(len(args)):
+            for grad in (True, False):
+                with fwad.dual_level(), torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward"):
+                    call(*[fwad.make_dual(t, torch.empty_like(t)) if j == i else t for j, t in enumerate(args)])
+        assert call(*args).shape[0] == 5  # and without a tangent nothing is
+    # the host forms are differentiable either way
+    x = rnd(3, 12, dtype=torch.float64)
+    q, s = ops.int8_quantize(rnd(8, 12))
+    t = rnd(3, 12, dtype=torch.float64)
+    with fwad.dual_level():
+        got = fwad.unpack_dual(ops.int8_linear(fwad.make_dual(x, t), q, s)).tangent
+    assert torch.allclose(got, t @ (q.double() * s.double()[:, None]).t())
