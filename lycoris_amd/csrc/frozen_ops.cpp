@@ -98,11 +98,19 @@ void check_w8(const Tensor& wq, const char* what) {
   TORCH_CHECK(wq.dim() == 2 && wq.scalar_type() == at::kChar && wq.size(0) > 0 && wq.size(1) > 0, what, ": the 8-bit operand must be a non-empty int8 matrix, got ",
               wq.sizes(), " ", wq.scalar_type());
 }
-// a plain device tensor outside of tracing and batching: the device function can be called without another trip through the dispatcher
-bool eager(const Tensor& t) {
-  const c10::DispatchKeySet ks = t.key_set();
-  return t.is_cuda() && !ks.has(c10::DispatchKey::Python) && !ks.has(c10::DispatchKey::Functionalize) && !ks.has(c10::DispatchKey::FuncTorchBatched);
+// May the device function be called without another trip through the dispatcher?  Where the dispatcher would go there by itself: what is left
+// of the tensors' keys and the thread's, behind autograd and autocast, is the device.  Anything above it has to hear of the operator: an active
+// mode (TorchDispatchMode, functorch, the Python dispatcher), a tensor subclass, a functional or batched wrapper, a view with its negation pending.
+bool eager(std::initializer_list<const Tensor*> tensors) {
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  c10::DispatchKeySet ks = tls.included_;
+  for (const Tensor* t : tensors)
+    if (t && t->defined()) ks = ks | t->key_set();
+  ks = ks - tls.excluded_ - c10::autograd_dispatch_keyset_with_ADInplaceOrView - c10::autocast_dispatch_keyset -
+       c10::DispatchKeySet(c10::DispatchKey::BackendSelect);
+  return ks.highestPriorityTypeId() == c10::DispatchKey::CUDA;
 }
+const Tensor* tensor_of(const OptTensor& t) { return has(t) ? &*t : nullptr; }
 void once(const char* what) { TORCH_CHECK(!c10::GradMode::is_enabled(), what, " can be differentiated once only (create_graph is not supported)"); }
 
 // ---- int8_quantize --------------------------------------------------------------------------------------------------------------------
@@ -214,7 +222,7 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
     ctx->save_for_backward({wq, sw});  // not x: the layer is frozen
     ctx->saved_data["dt"] = (int64_t)x.scalar_type();
     ctx->saved_data["base"] = edge(base, 3 + has(bias));
-    return eager(x) ? int8_linear(x, wq, sw, bias, base) : op.call(x, wq, sw, bias, base);
+    return eager({&x, &wq, &sw, tensor_of(bias), tensor_of(base)}) ? int8_linear(x, wq, sw, bias, base) : op.call(x, wq, sw, bias, base);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("int8_linear");
@@ -224,14 +232,13 @@ struct Int8LinearFn : public torch::autograd::Function<Int8LinearFn> {
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::_int8_linear_backward", "")
                          .typed<Tensor(const Tensor&, const Tensor&, const Tensor&)>();
     Tensor g = grads[0].to((at::ScalarType)ctx->saved_data["dt"].toInt());
-    if (ctx->needs_input_grad(0)) out[0] = eager(g) ? int8_linear_bwd(g, s[0], s[1]) : op.call(g, s[0], s[1]);
+    if (ctx->needs_input_grad(0)) out[0] = eager({&g, &s[0], &s[1]}) ? int8_linear_bwd(g, s[0], s[1]) : op.call(g, s[0], s[1]);
     if (wanted(ctx, "base")) out[4] = g;
     return out;
   }
 };
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return has(t) && t->requires_grad(); }
-const Tensor* ref(const OptTensor& t) { return has(t) ? &*t : nullptr; }
 // A dual tensor need not require a gradient, so it has to be asked for by itself: passed below autograd, its tangent would be lost without a word.
 void no_tangent(std::initializer_list<const Tensor*> inputs, const char* what) {
   for (const Tensor* t : inputs)
@@ -255,12 +262,12 @@ void capture_safe(std::initializer_list<const Tensor*> inputs, const char* what)
 }
 Tensor int8_linear_autograd(const Tensor& x, const Tensor& wq, const Tensor& sw, const OptTensor& bias, const OptTensor& base) {
   TORCH_CHECK(!wants(sw) && !wants(bias), "int8_linear: the layer is frozen, its scale and bias cannot require a gradient");
-  no_tangent({&x, &sw, ref(bias), ref(base)}, "int8_linear");
-  if (eager(x) && !(c10::GradMode::is_enabled() && (wants(x) || wants(base)))) {
+  no_tangent({&x, &sw, tensor_of(bias), tensor_of(base)}, "int8_linear");
+  if (eager({&x, &wq, &sw, tensor_of(bias), tensor_of(base)}) && !(c10::GradMode::is_enabled() && (wants(x) || wants(base)))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     return int8_linear(x, wq, sw, bias, base);
   }
-  capture_safe({&x, ref(base)}, "int8_linear");
+  capture_safe({&x, tensor_of(base)}, "int8_linear");
   return Int8LinearFn::apply(x, wq, sw, bias, base);
 }
 
@@ -367,7 +374,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::_gated_linear_forward", "")
                          .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool)>();
-    auto [h, pre] = eager(x) ? gated_forward(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
+    auto [h, pre] = eager({&x, &w, tensor_of(sw), tensor_of(bias), tensor_of(base)}) ? gated_forward(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
     // x is read by dw alone
     ctx->save_for_backward({pre, w.requires_grad() ? x : Tensor(), w, has(sw) ? *sw : Tensor()});
     ctx->saved_data["bias"] = edge(bias, 2 + has(sw));
@@ -393,7 +400,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     const int64_t act = ctx->saved_data["act"].toInt();
     const bool gf = ctx->saved_data["gf"].toBool();
     const Tensor& xs = s[1].defined() ? s[1] : g;
-    auto [b, x, w, bi] = eager(g) ? gated_backward(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias) : op.call(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias);
+    auto [b, x, w, bi] = eager({&g, &s[0], &xs, &s[2], tensor_of(sw)}) ? gated_backward(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias) : op.call(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias);
     if (dx) out[0] = x;
     if (dw) out[1] = w;
     if (dbias) out[3] = bi.to((at::ScalarType)ctx->saved_data["bdt"].toInt());
@@ -403,14 +410,14 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
 };
 Tensor gated_linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& sw, const OptTensor& bias, const OptTensor& base, int64_t act, bool gate_first) {
   TORCH_CHECK(!wants(sw), "gated_linear: an 8-bit weight is frozen, its scale cannot require a gradient");
-  no_tangent({&x, &w, ref(sw), ref(bias), ref(base)}, "gated_linear");
+  no_tangent({&x, &w, tensor_of(sw), tensor_of(bias), tensor_of(base)}, "gated_linear");
   if (!c10::GradMode::is_enabled() || !(wants(x) || wants(w) || wants(bias) || wants(base))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::gated_linear", "")
                          .typed<Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool)>();
-    return eager(x) ? gated_linear(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
+    return eager({&x, &w, tensor_of(sw), tensor_of(bias), tensor_of(base)}) ? gated_linear(x, w, sw, bias, base, act, gate_first) : op.call(x, w, sw, bias, base, act, gate_first);
   }
-  capture_safe({&x, &w, ref(bias), ref(base)}, "gated_linear");
+  capture_safe({&x, &w, tensor_of(bias), tensor_of(base)}, "gated_linear");
   return GatedLinearFn::apply(x, w, sw, bias, base, act, gate_first);
 }
 
