@@ -55,15 +55,16 @@ int need16(const char* who, const char* what, const void* p, bool optional = fal
   return fz_al16(p) ? LYC_OK : fail(LYC_ERR_ARG, "%s: %s must be 16-byte aligned", who, what);
 }
 
-// dynamic LDS above 64 KiB is allowed per kernel AND device
-template <typename Kern>
-int allow_lds(Kern kern, int bytes) {
+// Dynamic LDS above 64 KiB is allowed per kernel AND device: the kernel is a template argument (of one type are all products), so that each
+// has its own flags.  Devices beyond the flags are set on every launch.
+template <auto Kern>
+int allow_lds(int bytes) {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return fail(LYC_ERR_LAUNCH, "hipGetDevice failed");
-  const uint64_t bit = 1ull << (dev & 63);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return LYC_OK;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return fail(LYC_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   done.fetch_or(bit, std::memory_order_relaxed);
   return LYC_OK;
@@ -74,7 +75,7 @@ int grid_of(int64_t chunks) { return (int)(cdiv(chunks, 256) < 16384 ? cdiv(chun
 template <typename K, int BM>
 int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
   const int per = fz_per_xcd(cdiv(p.M, BM) * cdiv(K::GATED ? ep.F : p.N, K::BNO));
-  FZ_TRY(allow_lds(&fz_gemm_kernel<K>, K::LDS));
+  FZ_TRY((allow_lds<&fz_gemm_kernel<K>>(K::LDS)));
   hipLaunchKernelGGL((fz_gemm_kernel<K>), dim3((unsigned)(8 * per), p.ksplit > 1 ? p.ksplit : 1), dim3(K::NW * 64), K::LDS, st, p, ep);
   return check_launch("fz_gemm");
 }
@@ -177,7 +178,7 @@ int launch_skinny2(const TI* x, const FzProb& p, const FzEpi& ep, hipStream_t st
     constexpr int W = decltype(wc)::value;
     const int red = (GATED ? 2 : 1) * MT * W * 16 * 20 * 4, rows = FUSED ? p.M * sk_pitch(p.K) : 0;
     const int lds = red > rows ? red : rows;
-    FZ_TRY(allow_lds(&fz_skinny_kernel<E, TI, TO, MT, W, GATED, FUSED>, 96 * 1024));
+    FZ_TRY((allow_lds<&fz_skinny_kernel<E, TI, TO, MT, W, GATED, FUSED>>(96 * 1024)));
     hipLaunchKernelGGL((fz_skinny_kernel<E, TI, TO, MT, W, GATED, FUSED>), dim3((unsigned)cdiv(NO, 16)), dim3(W * 64), lds, st, x, p, ep);
     return check_launch("fz_skinny");
   };

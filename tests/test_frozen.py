@@ -1,6 +1,9 @@
 """Host side of the 8-bit frozen layer and the gated projection: the forms for host tensors against the formulas in 64 bits, refusals,
 argument checks of the C ABI (before any launch), tracing shapes, and the modules under adapters."""
 import math
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -284,3 +287,13 @@ def test_forward_mode_is_refused_and_not_dropped():
     with fwad.dual_level():
         got = fwad.unpack_dual(ops.int8_linear(fwad.make_dual(x, t), q, s)).tangent
     assert torch.allclose(got, t @ (q.double() * s.double()[:, None]).t())
+
+
+def test_every_product_kernel_has_its_own_lds_limit_flags():
+    """the limit of dynamic LDS is raised per kernel and device, and remembered: one set of flags for all kernels of a type would leave it at
+    the default for all but the first one launched"""
+    nm = shutil.which("nm") or "/opt/rocm/llvm/bin/llvm-nm"
+    names = subprocess.run([nm, N.lib_path()], check=True, capture_output=True, text=True).stdout.split()
+    kernels = [n for n in names if re.search(r"__device_stub__fz_(gemm|skinny)_kernel", n)]
+    flags = [n for n in names if "allow_lds" in n and n.endswith("E4done")]
+    assert len(kernels) > 50 and len(set(flags)) == len(set(kernels))
