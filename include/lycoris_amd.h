@@ -47,14 +47,16 @@ enum { LYC_F32_ROWS = 0x100, LYC_DEFER_WGRAD = 0x200,
        LYC_KCONV_W4 = 0x40000,
        /* same entry points, round 6: keep the k loop of the 8-wave patch kernel in its serial form (one basic block per k step) instead of
         * the software-pipelined loop (next k step's fragments read before this one's MFMAs) -- the A/B and regression-test switch */
-       LYC_KCONV_SERIAL = 0x80000 };
+       LYC_KCONV_SERIAL = 0x80000,
+       /* lyc_gated_linear_bwd only: dbias is fp32, as the bias of the forward call was (bias_f32), not `dtype` */
+       LYC_F32_DBIAS = 0x100000 };
 /* The *_planes Conv2d entry points and lyc_lokr_conv2d_planes_ok / _dx_blocks: pin the patch kernel's row tile (mi = 2, 4 or 8: 64 * mi
  * stage-1 rows per workgroup) instead of letting the host plan it -- for tests, which otherwise reach only the smallest tile with
  * their small problems (rounds 2-3 read an environment variable for this). */
 #define LYC_KCONV_ROW_TILE(mi) (((mi) & 0xf) << 12)
 enum { LYC_OK = 0, LYC_ERR_ARG = 1, LYC_ERR_UNSUPPORTED = 2, LYC_ERR_LAUNCH = 3 };
 
-#define LYC_ABI_VERSION 14
+#define LYC_ABI_VERSION 15
 int lyc_abi_version(void);
 const char* lyc_last_error(void);
 
@@ -488,7 +490,8 @@ int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const floa
  * value and gate are the halves of p's columns (value first, or gate first with gate_first).  w [2 F, I] in `dtype`, contiguous, or 8-bit
  * rows of pitch ldw with scales sw (then x is quantised as above).  `pre` (training, 16-byte aligned): receives p for
  * bwd: fp32 in 32 bits; else 24 bits of each value, 3 * M * 2 F bytes.
- * bwd, each output optional: dbase = dp [M, 2 F], dx = dp w, dw = dp^T x (not with an 8-bit weight), dbias = sum_m dp.          */
+ * bwd, each output optional: dbase = dp [M, 2 F], dx = dp w, dw = dp^T x (not with an 8-bit weight), dbias = sum_m dp (in fp32 with
+ * dtype | LYC_F32_DBIAS).                                                                                                            */
 enum { LYC_ACT_GELU = 0, LYC_ACT_GELU_TANH = 1, LYC_ACT_SILU = 2 };
 enum { LYC_GATED_INT8 = 1, LYC_GATED_BACKWARD = 2, LYC_GATED_DBASE = 4, LYC_GATED_DX = 8, LYC_GATED_DW = 16, LYC_GATED_DBIAS = 32 };
 int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dtype, int flags);

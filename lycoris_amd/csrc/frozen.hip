@@ -401,7 +401,7 @@ int dgate_rows(int64_t M, int64_t F) {
 // dp is written once, by one elementwise pass.  dx over an 8-bit weight takes dp sw (16 bits: rounded once, from fp32; 32 bits: staged in
 // three planes) times the weight's integers, which 16 bits hold exactly; over a 16 / 32-bit weight it takes dp and the weight.
 template <typename T>
-int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T* dx, T* dw, T* dbias, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
+int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T* dx, T* dw, void* dbias, bool dbias_f32, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
   using E = typename Operand<T>::E;
   constexpr bool F32 = sizeof(T) == 4;
   const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
@@ -456,7 +456,9 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
     FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(pdw, p, ep, sums, st)));
   }
   if (part) {
-    hipLaunchKernelGGL((fz_join_kernel<T>), dim3((unsigned)cdiv(N, 32)), dim3(256), 0, st, part, dbias, parts, (int)N);
+    const dim3 grid((unsigned)cdiv(N, 32));
+    if (dbias_f32) hipLaunchKernelGGL((fz_join_kernel<float>), grid, dim3(256), 0, st, part, static_cast<float*>(dbias), parts, (int)N);
+    else hipLaunchKernelGGL((fz_join_kernel<T>), grid, dim3(256), 0, st, part, static_cast<T*>(dbias), parts, (int)N);
     FZ_TRY(check_launch("column sums"));
   }
   return LYC_OK;
@@ -558,7 +560,7 @@ int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dt
   const float one = 1.f;
   Carve ws{nullptr};
   if (flags & LYC_GATED_BACKWARD) {
-    FZ_DTYPE(dtype, (void)gated_bwd<T>(q, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, flags, ws, &n, nullptr));
+    FZ_DTYPE(dtype, (void)gated_bwd<T>(q, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, false, flags, ws, &n, nullptr));
   } else {
     q.sw = flags & LYC_GATED_INT8 ? &one : nullptr;
     FZ_DTYPE(dtype, (void)gated_fwd<T>(q, nullptr, nullptr, 0, nullptr, nullptr, nullptr, ws, &n, nullptr));
@@ -585,6 +587,8 @@ int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float*
 int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const void* w, int64_t ldw, const float* sw, void* dbase, void* dx, void* dw,
                          void* dbias, void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream) {
   const char* who = "gated_linear_bwd";
+  const bool dbias_f32 = dtype & LYC_F32_DBIAS;
+  dtype &= ~LYC_F32_DBIAS;
   const Gated q{w, ldw, sw, M, I, F, act, gate_first};
   FZ_TRY(check_gated(who, q, sw != nullptr, dtype));
   if (dw && sw) return fail(LYC_ERR_UNSUPPORTED, "%s: an 8-bit weight is frozen", who);
@@ -598,7 +602,7 @@ int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const vo
   const int flags = LYC_GATED_BACKWARD | (sw ? LYC_GATED_INT8 : 0) | (dbase ? LYC_GATED_DBASE : 0) | (dx ? LYC_GATED_DX : 0) | (dw ? LYC_GATED_DW : 0) |
                     (dbias ? LYC_GATED_DBIAS : 0);
   FZ_DTYPE(dtype, return gated_bwd<T>(q, static_cast<const T*>(g), pre, static_cast<const T*>(x), static_cast<T*>(dbase),
-                                      static_cast<T*>(dx), static_cast<T*>(dw), static_cast<T*>(dbias), flags, Carve{static_cast<char*>(ws)}, nullptr,
+                                      static_cast<T*>(dx), static_cast<T*>(dw), dbias, dbias_f32, flags, Carve{static_cast<char*>(ws)}, nullptr,
                                       static_cast<hipStream_t>(stream)));
   return LYC_OK;
 }

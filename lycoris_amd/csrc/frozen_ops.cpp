@@ -339,16 +339,17 @@ std::tuple<Tensor, Tensor> gated_forward_meta(const Tensor& x, const Tensor& w, 
 }
 // (dbase [M, 2 F], dx, dw, dbias); what is not asked for comes back empty
 std::tuple<Tensor, Tensor, Tensor, Tensor> gated_backward_meta(const Tensor& g, const Tensor& pre, const Tensor& x, const Tensor& w, const OptTensor& sw,
-                                                               int64_t act, bool gate_first, bool dbase, bool dx, bool dw, bool dbias) {
+                                                               int64_t act, bool gate_first, bool dbase, bool dx, bool dw, bool dbias, bool dbias_f32) {
   auto e = [&](bool want, at::IntArrayRef shape) { return want ? at::empty(shape, g.options()) : at::empty({0}, g.options()); };
-  return {e(dbase, with_last(g, w.size(0))), e(dx, with_last(g, w.size(1))), e(dw, w.sizes()), e(dbias, {w.size(0)})};
+  return {e(dbase, with_last(g, w.size(0))), e(dx, with_last(g, w.size(1))), e(dw, w.sizes()),
+          dbias ? at::empty({w.size(0)}, dbias_f32 ? g.options().dtype(at::kFloat) : g.options()) : e(false, {})};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& g, const Tensor& pre, const Tensor& x, const Tensor& w, const OptTensor& sw,
-                                                          int64_t act, bool gate_first, bool dbase, bool dx, bool dw, bool dbias) {
+                                                          int64_t act, bool gate_first, bool dbase, bool dx, bool dw, bool dbias, bool dbias_f32) {
   const c10::DeviceGuard guard(g.device());
   const int code = code_of(g.scalar_type());
   const int64_t F = w.size(0) / 2, I = w.size(1);
-  auto out = gated_backward_meta(g, pre, x, w, sw, act, gate_first, dbase, dx, dw, dbias);
+  auto out = gated_backward_meta(g, pre, x, w, sw, act, gate_first, dbase, dx, dw, dbias, dbias_f32);
   Tensor gr = rows_of(g, F);
   const int64_t M = gr.size(0);
   if (M == 0) {
@@ -364,7 +365,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_backward(const Tensor& g, const
   auto p = [](bool want, const Tensor& t) { return want ? t.mutable_data_ptr() : nullptr; };
   check_rc(lyc_gated_linear_bwd(gr.const_data_ptr(), pre.const_data_ptr(), dw ? xr.const_data_ptr() : nullptr, a.w.const_data_ptr(), a.ldw, a.sw,
                                 p(dbase, std::get<0>(out)), p(dx, std::get<1>(out)), p(dw, std::get<2>(out)), p(dbias, std::get<3>(out)),
-                                mptr(ws), M, I, F, (int)act, gate_first, code, stream_of(g)), "gated_linear backward");
+                                mptr(ws), M, I, F, (int)act, gate_first, code | (dbias_f32 ? LYC_F32_DBIAS : 0), stream_of(g)), "gated_linear backward");
   return out;
 }
 
@@ -392,7 +393,7 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     auto s = ctx->get_saved_variables();
     static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lycoris_amd::_gated_linear_backward", "")
                          .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, int64_t,
-                                                                           bool, bool, bool, bool, bool)>();
+                                                                           bool, bool, bool, bool, bool, bool)>();
     const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1), dbias = wanted(ctx, "bias"), dbase = wanted(ctx, "base");
     if (!(dx || dw || dbias || dbase)) return out;
     OptTensor sw = opt(s[3]);
@@ -400,10 +401,13 @@ struct GatedLinearFn : public torch::autograd::Function<GatedLinearFn> {
     const int64_t act = ctx->saved_data["act"].toInt();
     const bool gf = ctx->saved_data["gf"].toBool();
     const Tensor& xs = s[1].defined() ? s[1] : g;
-    auto [b, x, w, bi] = eager({&g, &s[0], &xs, &s[2], tensor_of(sw)}) ? gated_backward(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias) : op.call(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias);
+    const auto bdt = (at::ScalarType)ctx->saved_data["bdt"].toInt();
+    const bool df = bdt != g.scalar_type();  // the kernels read any other type of bias as fp32, and its gradient is the fp32 sum
+    auto [b, x, w, bi] = eager({&g, &s[0], &xs, &s[2], tensor_of(sw)}) ? gated_backward(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias, df)
+                                                                  : op.call(g, s[0], xs, s[2], sw, act, gf, dbase, dx, dw, dbias, df);
     if (dx) out[0] = x;
     if (dw) out[1] = w;
-    if (dbias) out[3] = bi.to((at::ScalarType)ctx->saved_data["bdt"].toInt());
+    if (dbias) out[3] = bi.to(bdt);
     if (dbase) out[4] = b;
     return out;
   }
@@ -431,7 +435,7 @@ TORCH_LIBRARY_FRAGMENT(lycoris_amd, m) {
   m.def("gated_linear(Tensor x, Tensor weight, Tensor? weight_scale, Tensor? bias, Tensor? base, int act, bool gate_first) -> Tensor");
   m.def("_gated_linear_forward(Tensor x, Tensor weight, Tensor? weight_scale, Tensor? bias, Tensor? base, int act, bool gate_first) -> (Tensor, Tensor)");
   m.def("_gated_linear_backward(Tensor g, Tensor pre, Tensor x, Tensor weight, Tensor? weight_scale, int act, bool gate_first, bool dbase, bool dx, bool dw, "
-        "bool dbias) -> (Tensor, Tensor, Tensor, Tensor)");
+        "bool dbias, bool dbias_f32) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(lycoris_amd, CUDA, m) {
   m.impl("int8_quantize", int8_quantize);
