@@ -324,13 +324,17 @@ __device__ __forceinline__ void fz_bias(const FzEpi& ep, int64_t at, int n, int 
   if (ep.bias_f32) fz_load<float, CN>(ep.bias, at, n, N, vec, v);
   else fz_load<T, CN>(ep.bias, at, n, N, vec, v);
 }
-// p for the backward pass: fp32 as it is; 16-bit types keep the upper 24 bits of the fp32 value (sign, exponent, 15 bits: off by less than
-// 2^-15, infinities and NaNs stay what they are), as a plane of its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p
-// alone would cost the gradients as much as their own rounding does.  total: elements of p
+// p for the backward pass: fp32 as it is; 16-bit types keep 24 bits of the fp32 value (sign, exponent, 15 bits) rounded to nearest, off by at
+// most 2^-16 of it, as a plane of its upper 16 bits and, behind it, one of the next 8.  Rounded to 16 bits, p alone would cost the gradients as
+// much as their own rounding does.  total: elements of p
+//
+// The bits of v with half a unit of the 24 added, whose upper 24 are the rounded value: a carry runs into the exponent as it should, and an
+// infinity stays one.  A NaN is left alone: the carry out of a full payload would run into the sign.
+__device__ __forceinline__ unsigned fz_near24(float v) { return __float_as_uint(v) + (v == v ? 0x80u : 0u); }
 __device__ __forceinline__ void fz_split24(const float (&v)[8], u32x4& hi, u32x2& lo) {
   unsigned u[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(v[e]);
+  for (int e = 0; e < 8; ++e) u[e] = fz_near24(v[e]);
 #pragma unroll
   for (int e = 0; e < 4; ++e) hi[e] = __builtin_amdgcn_perm(u[2 * e + 1], u[2 * e], 0x07060302u);
 #pragma unroll
@@ -349,8 +353,8 @@ __device__ __forceinline__ void fz_store_pre8(void* pre, int64_t total, int64_t 
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (n + e < N) {
-        hi[e] = (uint16_t)(__float_as_uint(v[e]) >> 16);
-        lo[e] = (uint8_t)(__float_as_uint(v[e]) >> 8);
+        hi[e] = (uint16_t)(fz_near24(v[e]) >> 16);
+        lo[e] = (uint8_t)(fz_near24(v[e]) >> 8);
       }
   }
 }

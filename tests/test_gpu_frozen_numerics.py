@@ -49,3 +49,44 @@ def test_the_gradient_of_an_fp32_bias_keeps_32_bits(M, F, dt, int8):
     assert (over <= 0).all(), float(over.max())
     if M == 1200:  # the mean of silu over a standard normal is 0.207: 0.207 * 400 * 1200 = 99e3
         assert float(want.abs().max()) > 65504
+
+
+def kept(pre, n):
+    """the fp32 bits of p as the backward pass reads them: a plane of the upper 16 bits, one of the next 8"""
+    raw = pre.cpu()
+    hi, lo = raw[:2 * n].view(torch.int16).long() & 0xffff, raw[2 * n:].long()
+    return (hi << 16) | (lo << 8)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["plain", "int8"])
+@pytest.mark.parametrize("dt", HALVES, ids=IDS)
+@pytest.mark.parametrize("M,F", [(1, 8), (20, 33), (40, 40), (300, 77), (300, 640), (4100, 2560)])
+def test_p_is_kept_in_24_bits_to_the_nearest(M, F, dt, int8):
+    """half a step of 16 significant bits at most, 2^-16 of the value, and no more below it than above; infinities and NaNs stay what they are"""
+    gen = torch.Generator().manual_seed(M + F)
+    x, w = torch.zeros(M, 16, dtype=dt, device=DEV), torch.zeros(2 * F, 16, dtype=dt, device=DEV)
+    sw = None
+    if int8:
+        w, sw = ops.int8_quantize(torch.randn(2 * F, 16, generator=gen).to(DEV))
+    bits = torch.randint(-2 ** 31, 2 ** 31, (2 * F,), generator=gen, dtype=torch.int64)
+    bits[:12] = torch.tensor([0x7f800000, 0xff800000, 0x7fc00000, 0x7fffffff, 0xffffffff, 0x7f800001, 0, 0x80000000, 0x3f800080, 0x3f80007f, 0xbf8000ff, 0x3fffffff])
+    bits = bits.remainder(2 ** 32)
+    bias = bits.sub((bits >= 2 ** 31).long() * 2 ** 32).to(torch.int32).view(torch.float32)
+    h, pre = torch.ops.lycoris_amd._gated_linear_forward(x, w, sw, bias.to(DEV), None, 2, False)
+    got = kept(pre, M * 2 * F).view(M, 2 * F)
+    assert (got == got[0]).all()  # every row alike, whichever lane and path wrote it
+    value = got[0].sub((got[0] >= 2 ** 31).long() * 2 ** 32).to(torch.int32).view(torch.float32)
+    nan = bias.isnan()
+    assert torch.equal(value.isnan(), nan)
+    tiny = bias.abs() < 2.0 ** -126  # below: a product with the scale may flush them
+    big = bias.abs() >= 2.0 ** 128 - 2.0 ** 111  # rounds to the power above: infinity
+    rest = ~(nan | tiny | big)
+    assert torch.equal(value[big], torch.copysign(torch.full_like(value[big], math.inf), bias[big]))
+    assert (value[tiny].abs() <= 2.0 ** -126).all()
+    b64, v64 = bias[rest].double(), value[rest].double()
+    step = 2.0 ** (torch.floor(torch.log2(b64.abs())) - 15)
+    off = (v64 - b64) / step
+    assert float(off.abs().max()) <= 0.5
+    if F >= 640:  # uniform on a step of 1 around 0: standard deviation 0.289 / sqrt(n); truncation would give a mean of -0.5 of the magnitude
+        toward = (off * torch.sign(b64)).mean()
+        assert abs(float(toward)) < 6 * 0.289 / math.sqrt(off.numel())
