@@ -1,6 +1,8 @@
 // frozen_rows.h -- the row kernels around the products of frozen_gemm.h: quantisation, weight planes, operand staging, the gated
 // backward's elementwise pass, column sums.  All of them are bound by HBM (or, for one row, by the launch).
 #pragma once
+#include <cfloat>
+
 #include "frozen_gemm.h"
 
 namespace lyc {
@@ -155,6 +157,8 @@ __global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict_
 // ---- staging: a row matrix into 16-byte aligned rows of 16-bit elements, NP planes -----------------------------------------------------
 // NP = 1: a copy (rows whose length or base is not a multiple of 16 bytes).  NP = 3, fp32: x = h + m + l in bf16, each the rounding of
 // what the ones before left; `col` scales the columns first.  Columns cols .. ldo are zeros.
+// At the ends of the range: above the largest bf16 (the upper 0.2 % of the last binade) h is that one and not infinity, and m takes the rest;
+// below 2^-108 the lower planes leave the normal numbers, and a term of a product is off by up to 2^-125 of its other factor.
 // One launch stages up to three operands, one per blockIdx.y: they are small where it is needed most, and a launch costs 4 us.
 struct FzStageJob {
   const void* x;
@@ -166,6 +170,7 @@ struct FzStageJob {
 struct FzStage {
   FzStageJob job[3];
 };
+constexpr float BF16_MAX = 0x1.fep127f;
 template <typename TI, typename TO, int NP>
 __global__ __launch_bounds__(256) void fz_stage_kernel(FzStage jobs) {
   const FzStageJob& j = jobs.job[blockIdx.y];
@@ -186,8 +191,9 @@ __global__ __launch_bounds__(256) void fz_stage_kernel(FzStage jobs) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         t[e] = (TO)v[e];
-        const float h = (float)t[e];
-        v[e] = fabsf(h) <= 3.4e38f ? v[e] - h : 0.f;
+        float h = (float)t[e];
+        if (NP == 3 && fabsf(h) > BF16_MAX && fabsf(v[e]) <= FLT_MAX) t[e] = (TO)(h = copysignf(BF16_MAX, h));
+        v[e] = fabsf(h) <= FLT_MAX ? v[e] - h : 0.f;
       }
       *reinterpret_cast<u32x4*>(static_cast<TO*>(j.out) + p * plane + r * ldo + k) = *reinterpret_cast<u32x4*>(t);
     }

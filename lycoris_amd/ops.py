@@ -931,7 +931,8 @@ def gated_linear(x, weight, bias=None, base=None, act="gelu", gate_first=False, 
 
     weight in x's dtype, trainable or frozen, or int8 with `weight_scale` [2 F] (int8_quantize of its rows): x is then quantised row by row
     as in int8_linear.  Differentiable in x, base, bias and an unquantised weight.  The backward pass reads p in 24 bits (fp32: as it is),
-    3 M 2 F bytes kept from the forward; over an 8-bit weight dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products (24 bits)."""
+    3 M 2 F bytes kept from the forward; over an 8-bit weight dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products
+    (24 bits; of magnitudes below 2^-108 fewer, 2^-125 of the other factor a term; a row that holds an infinity comes out NaN)."""
     if act not in ACTIVATIONS:
         raise ValueError(f"gated_linear: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     x = _amp(x)

@@ -90,3 +90,46 @@ def test_p_is_kept_in_24_bits_to_the_nearest(M, F, dt, int8):
     if F >= 640:  # uniform on a step of 1 around 0: standard deviation 0.289 / sqrt(n); truncation would give a mean of -0.5 of the magnitude
         toward = (off * torch.sign(b64)).mean()
         assert abs(float(toward)) < 6 * 0.289 / math.sqrt(off.numel())
+
+
+def spread(gen, shape, top):
+    """fp32 values of all magnitudes in (top / 4, top], every bit of the fraction in use"""
+    return ((torch.rand(*shape, generator=gen).double() * 0.75 + 0.25) * top * torch.sign(torch.randn(*shape, generator=gen).double())).float()
+
+
+@pytest.mark.parametrize("top", [float(torch.finfo(torch.float32).max), 2.0 ** -100, 2.0 ** -112, 2.0 ** -120], ids=["max", "2^-100", "2^-112", "2^-120"])
+@pytest.mark.parametrize("M,K,N", [(3, 9, 6), (70, 64, 40), (300, 128, 256)])
+def test_32_bit_products_at_both_ends_of_the_range(M, K, N, top):
+    """three bf16 planes hold 24 bits where all three are normal numbers.  A term is then off by 3 e of it, the sum by e of the magnitudes for each
+    of its 3 n or 6 n products.  A plane below 2^-126 may be lost: 2^-125 of the other factor at most; so may a sum of one matrix instruction
+    (32 terms) below 2^-126"""
+    gen = torch.Generator().manual_seed(M)
+    flush = 2.0 ** -125
+    # dx of an 8-bit layer: g is staged; small scales keep the other columns finite
+    q = torch.randint(-127, 128, (N, K), generator=gen, dtype=torch.int8)
+    q[:, 1], q[0, :] = 0, 0
+    q[0, 1] = 1  # column 1 is g's column 0 itself
+    s = torch.full((N,), 2.0 ** -8 / max(N, 64))
+    s[0] = 1.0
+    g = spread(gen, (M, N), top)
+    g[0, 0] = top
+    x = torch.zeros(M, K, device=DEV, requires_grad=True)
+    y = ops.int8_linear(x, q.to(DEV), s.to(DEV))
+    dx, = torch.autograd.grad(y, x, g.to(DEV))
+    w64 = q.double() * s.double()[:, None]
+    want, mag = g.double() @ w64, g.double().abs() @ w64.abs()
+    off = (dx.double().cpu() - want).abs()
+    assert torch.isfinite(dx).all() and (off <= (3 * N + 8) * E * mag + E * want.abs() + flush * q.double().abs().sum(0) + (3 * N / 32 + 1) * 2.0 ** -126).all(), float((off / mag.clamp_min(1e-300)).max())
+    # the gated forward: x is staged against a weight of 2^-10 / K; the gate half is the bias alone, act(1)
+    F = N // 2
+    w = spread(gen, (2 * F, K), 2.0 ** -10 / K)
+    w[F:] = 0
+    bias = torch.cat((torch.zeros(F), torch.ones(F)))
+    a = spread(gen, (M, K), top)
+    a[0, 0] = top
+    h = ops.gated_linear(a.to(DEV), w.to(DEV), bias.to(DEV), act="silu")
+    one = float(silu64(torch.ones((), dtype=torch.float64))[0])
+    p, mag = a.double() @ w[:F].double().t(), a.double().abs() @ w[:F].double().abs().t()
+    off = (h.double().cpu() - p * one).abs()
+    assert torch.isfinite(h).all()
+    assert (off <= (6 * K + 16) * E * mag + (2 * ACT_ERR + E) * p.abs() + 2 * flush * w[:F].double().abs().sum(1) + (6 * K / 32 + 1) * 2.0 ** -126).all(), float((off / mag.clamp_min(1e-300)).max())
