@@ -194,21 +194,11 @@ int launch_skinny(const TI* x, const FzProb& p, const FzEpi& ep, hipStream_t st)
 constexpr int64_t SKINNY_ROWS = 32;
 inline bool skinny_fused(int64_t M, int64_t K) { return M <= SKINNY_ROWS && M * K <= SK_FUSED_ELEMS; }
 
-template <typename T>
-int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int K, hipStream_t st) {
-  constexpr int64_t SLAB = 1 << 22;  // rows a launch: a workgroup a row stays below 2^32 threads
-  if (M > SLAB) {
-    FZ_TRY(launch_quant<T>(x, ldx, q, ldq, scale, SLAB, K, st));
-    return launch_quant<T>(x + SLAB * ldx, ldx, q + SLAB * ldq, ldq, scale + SLAB, M - SLAB, K, st);
-  }
-  const int vec = fz_al16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0 && K % 8 == 0;
-  const int64_t c = ldq / 8;  // chunks of 8 a row
-  auto go = [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-    hipLaunchKernelGGL((fz_quant_kernel<T, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
-  };
+// How a row of c chunks of 8 is spread over threads: go(threads a row, chunks a thread) while registers hold it -- a wave a row, rows of 2048 columns
+// and more over a workgroup -- else whole()
+template <typename Go, typename Whole>
+void row_shape(int64_t c, Go go, Whole whole) {
   using std::integral_constant;
-  // a wave a row while its registers hold it; rows of 2048 columns and more are spread over a workgroup
   if (c <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (c <= 128) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
   else if (c <= 192) go(integral_constant<int, 64>{}, integral_constant<int, 3>{});
@@ -216,14 +206,43 @@ int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, 
   else if (c <= 512) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
   else if (c <= 768) go(integral_constant<int, 256>{}, integral_constant<int, 3>{});
   else if (c <= 1024) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  else hipLaunchKernelGGL((fz_quant_long_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
+  else whole();
+}
+constexpr int64_t ROW_SLAB = 1 << 22;  // rows a launch: a workgroup a row stays below 2^32 threads
+
+template <typename T>
+int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int K, hipStream_t st) {
+  if (M > ROW_SLAB) {
+    FZ_TRY(launch_quant<T>(x, ldx, q, ldq, scale, ROW_SLAB, K, st));
+    return launch_quant<T>(x + ROW_SLAB * ldx, ldx, q + ROW_SLAB * ldq, ldq, scale + ROW_SLAB, M - ROW_SLAB, K, st);
+  }
+  const int vec = fz_al16(x) && (ldx * (int64_t)sizeof(T)) % 16 == 0 && K % 8 == 0;
+  row_shape(ldq / 8, [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+    hipLaunchKernelGGL((fz_quant_kernel<T, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec);
+  }, [&] { hipLaunchKernelGGL((fz_quant_long_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, x, ldx, q, ldq, scale, M, K, vec); });
   return check_launch("int8_quantize");
 }
 
+// g [M, N] times col into NP fp16 planes, `plane` elements apart, rows of up(N, 8)
+template <typename T, int NP>
+int launch_scale(const T* g, const float* col, _Float16* out, int64_t plane, float* scale, int64_t M, int64_t N, hipStream_t st) {
+  if (M > ROW_SLAB) {
+    FZ_TRY((launch_scale<T, NP>(g, col, out, plane, scale, ROW_SLAB, N, st)));
+    return launch_scale<T, NP>(g + ROW_SLAB * N, col, out + ROW_SLAB * up(N, 8), plane, scale + ROW_SLAB, M - ROW_SLAB, N, st);
+  }
+  const int vec = fz_al16(g) && N % 8 == 0, vcol = fz_al16(col) && N % 8 == 0;
+  row_shape(cdiv(N, 8), [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+    hipLaunchKernelGGL((fz_scale_kernel<T, NP, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec, vcol);
+  }, [&] { hipLaunchKernelGGL((fz_scale_long_kernel<T, NP>), dim3((unsigned)M), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec, vcol); });
+  return check_launch("scaled rows");
+}
+
 template <typename T>
-int launch_plane(const int8_t* q, int64_t ldq, const float* sw, const float* f, T* out, int64_t O, int64_t I, hipStream_t st) {
+int launch_plane(const int8_t* q, int64_t ldq, T* out, int64_t O, int64_t I, hipStream_t st) {
   const int rows = 4;
-  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, sw, f, out, up(I, 8), (int)O, (int)I, rows);
+  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, out, up(I, 8), (int)O, (int)I, rows);
   return check_launch("weight plane");
 }
 // fp16: f[0], f[1] (fz_range_kernel); other types need none
@@ -273,10 +292,10 @@ struct Operand {
     if (own) stages.add(x, col, room, rows, cols);
   }
 };
-// segments: 16-bit 1; fp32 x fp32 6; fp32 x exact bf16 (an 8-bit weight's integers) 3.  The small terms come first.
+// segments: of one plane each 1; of 2 or 3 planes of A 2 or 3; fp32 x fp32 6.  The small terms come first.
 void segments(FzProb& p, int n) {
   p.nseg = n;
-  p.pa = n == 6 ? 0x010120u : n == 3 ? 0x012u : 0u;
+  p.pa = n == 6 ? 0x010120u : n == 3 ? 0x012u : n == 2 ? 0x01u : 0u;
   p.pb = n == 6 ? 0x001102u : 0u;
 }
 
@@ -310,32 +329,36 @@ int check_q(const char* who, const char* what, const void* q, int64_t ld, int64_
   return LYC_OK;
 }
 
-// ---- dx of a frozen 8-bit layer: g [M, N] times (sw wq) [N, K].  16 bits: g as it is, times the plane of sw wq (one rounding each entry);
-//      32 bits: g sw in three planes times the integers, which are exact in bf16 ----------------------------------------------------------
+// ---- dx of a frozen 8-bit layer: (g sw) [M, N] times the integers wq [N, K], which 16 bits hold exactly.  g sw takes a power of two a row in fp16
+//      (fz_scale_kernel; fp16 gradients: two planes), for fp32 gradients three bf16 planes ---------------------------------------------
 template <typename T>
 int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve ws, int64_t* bytes, int64_t M, int64_t N, int64_t K, hipStream_t st) {
-  using E = typename Operand<T>::E;
   constexpr bool F32 = sizeof(T) == 4;
+  constexpr int NP = F32 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1;
+  using E = typename std::conditional<F32, __bf16, _Float16>::type;
+  const int64_t ld = up(N, 8);
   E* plane = ws.take<E>(N * up(K, 8));
-  float* f = ws.take<float>(2);
-  Operand<T> a(ws, M, N, true);
-  const Plan pl = plan_of<E, FZ_PLAIN>(M, K, N, F32 ? 3 : 1, sizeof(T));
+  E* rows = ws.take<E>(NP * M * ld);
+  float* scale = F32 ? nullptr : ws.take<float>(M);
+  const Plan pl = plan_of<E, FZ_PLAIN>(M, K, N, NP, sizeof(T));
   char* part = ws.take<char>(part_bytes(pl, M, K));
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
   }
-  const float* range;
-  FZ_TRY(launch_range<E>(sw, N, 14, f, &range, st));
-  FZ_TRY(launch_plane<E>(wq, ldw, F32 ? nullptr : sw, range, plane, N, K, st));
-  Stages<T> stages;
-  a.fill(g, F32 ? sw : nullptr, stages);
-  FZ_TRY(stages.run(st));
-  FzProb p = prob(a.p, a.ld, a.plane, plane, up(K, 8) * 2, 0, M, K, N, 2);
-  segments(p, F32 ? 3 : 1);
+  FZ_TRY(launch_plane<E>(wq, ldw, plane, N, K, st));
+  if constexpr (F32) {
+    Stages<T> stages;
+    stages.add(g, sw, rows, M, N);
+    FZ_TRY(stages.run(st));
+  } else {
+    FZ_TRY((launch_scale<T, NP>(g, sw, rows, M * ld, scale, M, N, st)));
+  }
+  FzProb p = prob(rows, ld * 2, M * ld * 2, plane, up(K, 8) * 2, 0, M, K, N, 2);
+  segments(p, NP);
   FzEpi ep{};
   ep.out = dx;
-  ep.alpha = range ? range + 1 : nullptr;
+  ep.sa = scale;
   return launch_gemm<E, T, false, true, FZ_PLAIN>(pl, p, ep, part, st);
 }
 
@@ -438,7 +461,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
     ep.out = dx;
     FzProb p;
     if (held) {
-      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, nullptr, nullptr, plane, N, q.I, st));
+      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, plane, N, q.I, st));
       if (scaled) p = prob(dps, up(N, 8) * 2, 0, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
       else p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
       ep.alpha = range ? range + 1 : nullptr;

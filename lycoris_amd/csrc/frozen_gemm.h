@@ -127,7 +127,7 @@ struct FzEpi {
   void* out;           // [M, N] (GATED: [M, F]), row pitch = N (F) elements
   void* pre;           // GATED: p [M, 2 F] for the backward pass (fz_store_pre8) or null
   const float* alpha;  // PLAIN: device scalar on the result, or null
-  const float *sa, *sw;  // 8-bit: scales of A's rows, of B's rows
+  const float *sa, *sw;  // scales of A's rows (PLAIN too), of B's rows (8-bit only), or null
   const void* bias;    // [N] (GATED: [2 F]) or null; fp32 when bias_f32, else the output's type
   const void* base;    // [M, N] (GATED: [M, 2 F]) in the output's type, or null
   int64_t pre_total;   // elements of p
@@ -729,7 +729,7 @@ struct FzKernel {
         }
         if constexpr (EPI == FZ_PLAIN) {
 #pragma unroll
-          for (int e = 0; e < CN; ++e) v[e] *= alpha;
+          for (int e = 0; e < CN; ++e) v[e] *= alpha * sa[mi];
         } else {
 #pragma unroll
           for (int e = 0; e < CN; ++e) {
@@ -838,13 +838,13 @@ __global__ __launch_bounds__(256) void fz_reduce_kernel(FzProb p, FzEpi ep) {
         for (int e = 0; e < 8; ++e) s[e] += z0 + z < p.ksplit ? part[z][e] : 0;
     }
     float v[8], t[8];
+    const float sa = ep.sa ? ep.sa[m] : 1.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)s[e] * alpha;
+    for (int e = 0; e < 8; ++e) v[e] = (float)s[e] * (alpha * sa);
     if (ep.sw) {
-      const float sa = ep.sa[m];
       fz_load8<float>(ep.sw, n, n, N, vs, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] * sa * t[e];
+      for (int e = 0; e < 8; ++e) v[e] *= t[e];
     }
     if (ep.bias) {
       fz_bias<TO, 8>(ep, n, n, N, vb, t);

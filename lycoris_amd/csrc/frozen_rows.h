@@ -43,6 +43,19 @@ __device__ __forceinline__ u32x2 fz_pack_q(const float (&v)[8], float amax) {
   return o;
 }
 
+// the largest of the TPR threads of a row, to each of them
+template <int TPR>
+__device__ __forceinline__ unsigned fz_row_max(unsigned bits, unsigned (&red)[4]) {
+#pragma unroll
+  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = bits;
+    __syncthreads();
+    bits = max(max(red[0], red[1]), max(red[2], red[3]));
+  }
+  return bits;
+}
+
 // TPR threads a row, each holding NV chunks of 8 elements in registers: x is read once.  Columns K .. ldq are written as zeros.
 // Bound by HBM: bf16 16384 x 5120 in 59 us (4.3 TB/s of reading and writing), 16384 x 640 out of the caches in 13; one row by the launch.
 template <typename T, int TPR, int NV>
@@ -61,13 +74,7 @@ __global__ __launch_bounds__(256) void fz_quant_kernel(const T* __restrict__ x, 
       for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[i][e]) & 0x7fffffffu);
     }
   }
-#pragma unroll
-  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
-  if constexpr (TPR > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = bits;
-    __syncthreads();
-    bits = max(max(red[0], red[1]), max(red[2], red[3]));
-  }
+  bits = fz_row_max<TPR>(bits, red);
   if (m >= M) return;
   float sc;
   const float amax = fz_amax_of(bits, &sc);
@@ -92,11 +99,7 @@ __global__ __launch_bounds__(256) void fz_quant_long_kernel(const T* __restrict_
 #pragma unroll
     for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[e]) & 0x7fffffffu);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = bits;
-  __syncthreads();
-  bits = max(max(red[0], red[1]), max(red[2], red[3]));
+  bits = fz_row_max<256>(bits, red);
   float sc;
   const float amax = fz_amax_of(bits, &sc);
   if (threadIdx.x == 0) scale[m] = sc;
@@ -106,9 +109,92 @@ __global__ __launch_bounds__(256) void fz_quant_long_kernel(const T* __restrict_
   }
 }
 
+// ---- rows to fp16, scaled: out = 2^e g[m, n] col[n], scale[m] = 2^-e, the operand of dx over an 8-bit weight ------------------------------
+// The largest of a row comes to [2^14, 2^15), so that fp16 holds it with 11 bits down to 2^-28 of it and with a fixed step of 2^-38 below.
+// For bf16 gradients one plane is enough: g col in bf16 instead (8 bits), or col in the weight's plane, costs dx 1.4 times the error of its own
+// rounding (2.35e-3 of its norm against 1.66e-3; this way 1.67e-3).  fp16 gradients take a second plane of what the first leaves.
+// A row that holds an infinity or a NaN is not scaled.  Columns N .. up(N, 8) are zeros.
+__device__ __forceinline__ float fz_up_of(unsigned bits, float* down) {
+  const int e = bits >= 0x7f800000u ? 0 : min(14 + 127 - (int)(bits >> 23), 126);
+  *down = __uint_as_float((unsigned)(127 - e) << 23);
+  return __uint_as_float((unsigned)(127 + e) << 23);
+}
+template <typename T>
+__device__ __forceinline__ void fz_scaled8(const T* row, const float* col, int k, int N, bool vec, bool vcol, float (&v)[8]) {
+  float c[8];
+  fz_row8<T>(row, k, N, vec, v);
+  fz_load8<float>(col, k, k, N, vcol && k < N, c);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= c[e];
+}
+template <int NP>
+__device__ __forceinline__ void fz_store_planes(_Float16* out, int64_t plane, float (&v)[8], float up) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= up;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    _Float16 t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[e] = (_Float16)v[e];
+      v[e] = fabsf((float)t[e]) <= FLT_MAX ? v[e] - (float)t[e] : 0.f;
+    }
+    *reinterpret_cast<u32x4*>(out + p * plane) = *reinterpret_cast<u32x4*>(t);
+  }
+}
+// the split over threads is fz_quant_kernel's
+template <typename T, int NP, int TPR, int NV>
+__global__ __launch_bounds__(256) void fz_scale_kernel(const T* __restrict__ g, const float* __restrict__ col, _Float16* __restrict__ out, int64_t plane,
+                                                       float* __restrict__ scale, int64_t M, int N, int vec, int vcol) {
+  __shared__ unsigned red[4];
+  const int t = threadIdx.x % TPR, ldo = (N + 7) & ~7;
+  const int64_t m = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  float v[NV][8];
+  unsigned bits = 0;
+  if (m < M) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      fz_scaled8<T>(g + m * N, col, (i * TPR + t) * 8, N, vec, vcol, v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[i][e]) & 0x7fffffffu);
+    }
+  }
+  bits = fz_row_max<TPR>(bits, red);
+  if (m >= M) return;
+  float down;
+  const float up = fz_up_of(bits, &down);
+  if (t == 0) scale[m] = down;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = (i * TPR + t) * 8;
+    if (k < ldo) fz_store_planes<NP>(out + m * ldo + k, plane, v[i], up);
+  }
+}
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void fz_scale_long_kernel(const T* __restrict__ g, const float* __restrict__ col, _Float16* __restrict__ out, int64_t plane,
+                                                            float* __restrict__ scale, int64_t M, int N, int vec, int vcol) {
+  __shared__ unsigned red[4];
+  const int64_t m = blockIdx.x, ldo = (N + 7) & ~7;
+  const T* row = g + m * N;
+  unsigned bits = 0;
+  float v[8];
+  for (int k = threadIdx.x * 8; k < N; k += 2048) {
+    fz_scaled8<T>(row, col, k, N, vec, vcol, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(v[e]) & 0x7fffffffu);
+  }
+  bits = fz_row_max<256>(bits, red);
+  float down;
+  const float up = fz_up_of(bits, &down);
+  if (threadIdx.x == 0) scale[m] = down;
+  for (int k = threadIdx.x * 8; k < N; k += 2048) {
+    fz_scaled8<T>(row, col, k, N, vec, vcol, v);
+    fz_store_planes<NP>(out + m * ldo + k, plane, v, up);
+  }
+}
+
 // ---- fp16 only: the power of two that brings an 8-bit weight's scales into its range --------------------------------------------------
-// The gradients' products take sw either inside the weight plane (sw q) or inside the other operand (sw dp).  fp16 has 5 exponent bits and
-// the scales of a weight may lie anywhere: they are multiplied by f[0] = 2^e, which brings 127 max|sw| to [2^-1, 1) 2^`top`, and the product's
+// The gated backward takes sw inside dx's other operand (sw dp).  fp16 has 5 exponent bits and the scales of a weight may lie anywhere: they are multiplied by f[0] = 2^e, which brings 127 max|sw| to [2^-1, 1) 2^`top`, and the product's
 // alpha, f[1] = 2^-e, takes it out again.
 __global__ __launch_bounds__(256) void fz_range_kernel(const float* __restrict__ sw, int n, int top, float* __restrict__ f) {
   __shared__ float red[4];
@@ -128,26 +214,25 @@ __global__ __launch_bounds__(256) void fz_range_kernel(const float* __restrict__
   f[1] = ldexpf(1.f, -e);
 }
 
-// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): out[o, i] = sw[o] f[0] q[o, i], one rounding; without sw the
-// integers themselves, which 16 bits hold exactly.  f: fz_range_kernel's, or null.  A workgroup takes four rows: 10240 x 1280 in 10 us (39 MB), and
-// 5 - 8 us, most of them the launch, for 1280 x 1280 and 1280 x 5120
+// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): its integers, which 16 bits hold exactly; the scales go to the other
+// operand.  Columns I .. ldo are zeros.  A workgroup takes four rows: 10240 x 1280 in 10 us (39 MB), and 5 - 8 us, most of them the launch,
+// for 1280 x 1280 and 1280 x 5120
 template <typename T>
-__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ sw, const float* __restrict__ f,
-                                                       T* __restrict__ out, int64_t ldo, int O, int I, int rows_per_wg) {
+__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, T* __restrict__ out, int64_t ldo, int O, int I,
+                                                       int rows_per_wg) {
   const int chunks = (int)(ldo >> 3);
   for (int r = 0; r < rows_per_wg; ++r) {
     const int o = blockIdx.x * rows_per_wg + r;
     if (o >= O) return;
-    const float s = sw ? sw[o] * (f ? f[0] : 1.f) : 1.f;
     for (int c = threadIdx.x; c < chunks; c += 256) {
       T t[8];
       if (8 * c + 8 <= I) {
         const u32x2 w = *reinterpret_cast<const u32x2*>(q + (int64_t)o * ldq + 8 * c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = (T)(s * (float)(int8_t)(w[e >> 2] >> (8 * (e & 3))));
+        for (int e = 0; e < 8; ++e) t[e] = (T)(float)(int8_t)(w[e >> 2] >> (8 * (e & 3)));
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = (T)(8 * c + e < I ? s * (float)q[(int64_t)o * ldq + 8 * c + e] : 0.f);
+        for (int e = 0; e < 8; ++e) t[e] = (T)(8 * c + e < I ? (float)q[(int64_t)o * ldq + 8 * c + e] : 0.f);
       }
       *reinterpret_cast<u32x4*>(out + (int64_t)o * ldo + 8 * c) = *reinterpret_cast<u32x4*>(t);
     }

@@ -133,3 +133,71 @@ def test_32_bit_products_at_both_ends_of_the_range(M, K, N, top):
     off = (h.double().cpu() - p * one).abs()
     assert torch.isfinite(h).all()
     assert (off <= (6 * K + 16) * E * mag + (2 * ACT_ERR + E) * p.abs() + 2 * flush * w[:F].double().abs().sum(1) + (6 * K / 32 + 1) * 2.0 ** -126).all(), float((off / mag.clamp_min(1e-300)).max())
+
+
+def held(gen, N, K):
+    w = torch.randn(N, K, generator=gen) / math.sqrt(K) * torch.exp(0.3 * torch.randn(N, 1, generator=gen))
+    return ops.int8_quantize(w.to(DEV))
+
+
+# terms of dx = (g sw) wq: in fp16 with a power of two a row, one rounding (2^-12) beside bf16 gradients; two planes (2^-22) beside fp16 ones.  Below 2^-14
+# of what fp16 holds the step is fixed: 2^-39 of the row's largest (half a step).  Sums: n e of the magnitudes.
+TERM = {torch.bfloat16: 2.0 ** -12, torch.float16: 2.0 ** -22}
+
+
+def check_dx(dx, g, wq, sw, dt):
+    w64 = wq.double().cpu() * sw.double().cpu()[:, None]
+    g64 = g.double().cpu()
+    N = g64.shape[-1]
+    want, mag = g64 @ w64, g64.abs() @ w64.abs()
+    top = (g64 * sw.double().cpu()).abs().amax(-1, keepdim=True)
+    planes = 1 if dt == torch.bfloat16 else 2
+    bound = (TERM[dt] + 2 * E + (planes * N + 4) * E) * mag * 1.01 + 2.0 ** -39 * top * wq.double().cpu().abs().sum(0)
+    u, f = torch.finfo(dt).eps / 2, torch.finfo(dt)
+    bound = bound + u * (want.abs() + bound) + f.smallest_normal * f.eps / 2
+    over = (dx.double().cpu() - want).abs() - bound
+    assert torch.isfinite(dx).all() and (over <= 0).all(), float(over.max())
+    return float((dx.double().cpu() - want).norm() / want.norm()), float((want.to(dt).double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("dt", HALVES, ids=IDS)
+@pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 640, 1280), (5, 200, 17), (33, 64, 600), (130, 136, 1100), (300, 77, 1600), (40, 96, 3000), (257, 320, 5000), (64, 80, 8000),
+                                   (20, 64, 8200), (2100, 1284, 1032)])
+def test_dx_over_an_8_bit_weight_is_rounded_once(M, K, N, dt):
+    """the operands keep more bits than the gradient's type: the error of dx is that of its own rounding"""
+    gen = torch.Generator().manual_seed(M + K + N)
+    wq, sw = held(gen, N, K)
+    g = (torch.randn(M, N, generator=gen) / math.sqrt(N)).to(dt).to(DEV)
+    x = torch.zeros(M, K, dtype=dt, device=DEV, requires_grad=True)
+    dx, = torch.autograd.grad(ops.int8_linear(x, wq, sw), x, g)
+    here, once = check_dx(dx, g, wq, sw, dt)
+    if M * K > 10000:
+        assert here < 1.03 * once, (here, once)
+
+
+@pytest.mark.parametrize("dt", HALVES, ids=IDS)
+def test_dx_of_rows_of_every_magnitude(dt):
+    """rows as small as the type has them and as large, rows of zeros, one entry that outweighs the others by all that fp16 can hold and more"""
+    gen = torch.Generator().manual_seed(31)
+    M, K, N = 48, 72, 200
+    wq, sw = held(gen, N, K)
+    wq = wq.clone()
+    wq[7, :40] = 0
+    sw[7] = 1.0
+    g = torch.randn(M, N, generator=gen)
+    small = 2.0 ** -30 if dt == torch.bfloat16 else 2.0 ** -12
+    g[:16] *= 2.0 ** torch.linspace(-20 if dt == torch.float16 else -130, 8 if dt == torch.float16 else 100, 16)[:, None]
+    g[16:32] *= small * 2.0 ** -torch.arange(16.0)[:, None]
+    g[16:32, 7] = 1.0  # columns below 40 see the small entries alone
+    g[32] = 0
+    g = g.to(dt).to(DEV)
+    x = torch.zeros(M, K, dtype=dt, device=DEV, requires_grad=True)
+    dx, = torch.autograd.grad(ops.int8_linear(x, wq, sw), x, g)
+    check_dx(dx, g, wq, sw, dt)
+    assert (dx[32] == 0).all()
+    bad = g.clone()
+    bad[40, 3], bad[41, 199] = float("nan"), float("inf")
+    x2 = x.detach().clone().requires_grad_(True)
+    d2, = torch.autograd.grad(ops.int8_linear(x2, wq, sw), x2, bad)
+    rest = [m for m in range(M) if m not in (40, 41)]
+    assert torch.equal(d2[rest], dx[rest]) and torch.isnan(d2[40]).all() and not torch.isfinite(d2[41]).any()
