@@ -245,16 +245,6 @@ int launch_plane(const int8_t* q, int64_t ldq, T* out, int64_t O, int64_t I, hip
   hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, out, up(I, 8), (int)O, (int)I, rows);
   return check_launch("weight plane");
 }
-// fp16: f[0], f[1] (fz_range_kernel); other types need none
-template <typename E>
-int launch_range(const float* sw, int64_t n, int top, float* f, const float** out, hipStream_t st) {
-  *out = nullptr;
-  if (!std::is_same<E, _Float16>::value) return LYC_OK;
-  hipLaunchKernelGGL(fz_range_kernel, dim3(1), dim3(256), 0, st, sw, (int)n, top, f);
-  *out = f;
-  return check_launch("scale range");
-}
-
 // The operands of a pass that have to be staged, and their one launch
 template <typename T>
 struct Stages {
@@ -421,61 +411,102 @@ int dgate_rows(int64_t M, int64_t F) {
   return rows;
 }
 
-// dp is written once, by one elementwise pass.  dx over an 8-bit weight takes dp sw (16 bits: rounded once, from fp32; 32 bits: staged in
-// three planes) times the weight's integers, which 16 bits hold exactly; over a 16 / 32-bit weight it takes dp and the weight.
+// The elementwise pass where products follow, 16 bits: rows of a slab.  512 slabs (of waves: 2048) are two workgroups a CU, whose rows follow each other
+// with the next one's loads in flight: 8192 x 2560 in 69 us, against 82 with 1024 slabs (and twice the partial column sums); 4096 x 5120 in 75, against 78.
+int dgate_slab_rows(int64_t M, int64_t F) { return (int)cdiv(M, (F <= 512 ? 4 : 1) * 512); }
+template <typename T, int NP, bool SUMS>
+int launch_dgate_rows(const FzDgate& a, int64_t slabs, hipStream_t st) {
+  const int64_t chunks = cdiv(a.F, 8);
+  const dim3 grid((unsigned)slabs), block((unsigned)std::min<int64_t>(1024, up(chunks, 64)));
+  if (chunks <= 64) hipLaunchKernelGGL((fz_dgate_rows_kernel<T, NP, 1, true, SUMS>), dim3((unsigned)cdiv(slabs, 4)), dim3(256), 0, st, a);
+  else if (chunks <= 1024) hipLaunchKernelGGL((fz_dgate_rows_kernel<T, NP, 1, false, SUMS>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((fz_dgate_rows_kernel<T, NP, 0, false, SUMS>), grid, block, 0, st, a);
+  return check_launch("gated backward");
+}
+
+// dp is formed once, by one elementwise pass.  The products' operands:
+//   16 bits   dp (over an 8-bit weight sw dp) in fp16 with a power of two a row (fp16 gradients: two planes); the weight's integers, which fp16 holds
+//             exactly, or the 16-bit weight and x in fp16 with one power of two each (fz_level_kernel)
+//   32 bits   three bf16 planes each of dp (sw dp), the weight and x
 template <typename T>
 int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T* dx, T* dw, void* dbias, bool dbias_f32, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
-  using E = typename Operand<T>::E;
   constexpr bool F32 = sizeof(T) == 4;
-  const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW;
-  const int rows = dgate_rows(q.M, q.F);
-  const int64_t N = 2 * q.F, parts = cdiv(q.M, rows);
-  const bool scaled = held && want_dx && !F32;  // dps
-  if (!(flags & LYC_GATED_DBASE)) dp = want_dw || (want_dx && !scaled) ? ws.take<T>(q.M * N) : nullptr;
-  E* dps = scaled ? ws.take<E>(q.M * up(N, 8)) : nullptr;
-  Operand<T> a(ws, q.M, N, want_dw || (want_dx && !scaled));  // dp as the products' operand (K-contiguous for dx, K-strided for dw)
-  Operand<T> b(ws, N, q.I, want_dx && !held), xo(ws, q.M, q.I, want_dw);
-  E* plane = want_dx && held ? ws.take<E>(N * up(q.I, 8)) : nullptr;
-  float* f = ws.take<float>(2);
-  float* part = flags & LYC_GATED_DBIAS ? ws.take<float>(parts * N) : nullptr;
-  const Plan pdx = plan_of<E, FZ_PLAIN>(q.M, q.I, N, F32 ? (held ? 3 : 6) : 1, sizeof(T)), pdw = plan_of<E, FZ_PLAIN>(N, q.I, q.M, F32 ? 6 : 1, sizeof(T));
-  const int64_t sdx = want_dx ? part_bytes(pdx, q.M, q.I) : 0, sdw = want_dw ? part_bytes(pdw, N, q.I) : 0;
-  char* sums = ws.take<char>(sdx > sdw ? sdx : sdw);
+  constexpr int NP = F32 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1, NB = F32 ? 3 : 1;  // planes of dp, of the weight and of x
+  using E = typename std::conditional<F32, __bf16, _Float16>::type;
+  const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW, want_db = flags & LYC_GATED_DBIAS;
+  const bool products = want_dx || want_dw, by_row = products && !F32, level = by_row && !held;
+  const int rows = by_row ? dgate_slab_rows(q.M, q.F) : dgate_rows(q.M, q.F);
+  const int64_t N = 2 * q.F, ld = up(N, 8), ldi = up(q.I, 8), parts = cdiv(q.M, rows);
+  if (!(flags & LYC_GATED_DBASE)) dp = products && F32 ? ws.take<T>(q.M * N) : nullptr;
+  E* a = products ? ws.take<E>(NP * q.M * ld) : nullptr;
+  float* scale = by_row ? ws.take<float>(q.M) : nullptr;
+  float* top = level && want_dw ? ws.take<float>(parts) : nullptr;
+  E* b = want_dx ? ws.take<E>((held ? 1 : NB) * N * ldi) : nullptr;
+  E* xo = want_dw ? ws.take<E>(NB * q.M * ldi) : nullptr;
+  unsigned* peaks = level ? ws.take<unsigned>(2 * FZ_PEAKS) : nullptr;
+  float* alpha = level ? ws.take<float>(2) : nullptr;
+  float* part = want_db ? ws.take<float>(parts * N) : nullptr;
+  const int sdx = F32 && !held ? 6 : NP, sdw = F32 ? 6 : NP;  // segments
+  const Plan pdx = plan_of<E, FZ_PLAIN>(q.M, q.I, N, sdx, sizeof(T)), pdw = plan_of<E, FZ_PLAIN>(N, q.I, q.M, sdw, sizeof(T));
+  char* sums = ws.take<char>(std::max(want_dx ? part_bytes(pdx, q.M, q.I) : 0, want_dw ? part_bytes(pdw, N, q.I) : 0));
   if (bytes) {
     *bytes = ws.used;
     return LYC_OK;
   }
-  const float* range = nullptr;
-  if (scaled) FZ_TRY(launch_range<E>(q.sw, N, 7, f, &range, st));  // the largest sw f[0] near 1
-  const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp);
-  hipLaunchKernelGGL((fz_dgate_kernel<T, E>), dim3((unsigned)(cdiv(q.F, DG_COLS) * parts)), dim3(256), 0, st, g, pre, dp, dps, q.sw, range, part, q.M,
-                     (int)q.F, q.act, q.gate_first, vec, rows);
-  FZ_TRY(check_launch("gated backward"));
-  Stages<T> stages;
-  if (want_dw || (want_dx && !scaled)) a.fill(dp, F32 && held ? q.sw : nullptr, stages);
-  if (want_dx && !held) b.fill(static_cast<const T*>(q.w), nullptr, stages);
-  if (want_dw) xo.fill(x, nullptr, stages);
-  FZ_TRY(stages.run(st));
-  if (want_dx) {
-    FzEpi ep{};
-    ep.out = dx;
-    FzProb p;
-    if (held) {
-      FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, plane, N, q.I, st));
-      if (scaled) p = prob(dps, up(N, 8) * 2, 0, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
-      else p = prob(a.p, a.ld, a.plane, plane, up(q.I, 8) * 2, 0, q.M, q.I, N, 2);
-      ep.alpha = range ? range + 1 : nullptr;
-    } else {
-      p = prob(a.p, a.ld, a.plane, b.p, b.ld, b.plane, q.M, q.I, N, 2);
+  const int vec = q.F % 8 == 0 && fz_al16(g) && fz_al16(pre) && fz_al16(dp) && (!held || fz_al16(q.sw));
+  FzProb p;
+  FzEpi ep{};
+  if constexpr (F32) {
+    hipLaunchKernelGGL((fz_dgate_kernel<T>), dim3((unsigned)(cdiv(q.F, DG_COLS) * parts)), dim3(256), 0, st, g, pre, dp, part, q.M, (int)q.F, q.act,
+                       q.gate_first, vec, rows);
+    FZ_TRY(check_launch("gated backward"));
+    Stages<T> stages;
+    if (products) stages.add(dp, held ? q.sw : nullptr, a, q.M, N);
+    if (want_dx && !held) stages.add(static_cast<const T*>(q.w), nullptr, b, N, q.I);
+    if (want_dw) stages.add(x, nullptr, xo, q.M, q.I);
+    FZ_TRY(stages.run(st));
+  } else if (!products) {
+    hipLaunchKernelGGL((fz_dgate_kernel<T>), dim3((unsigned)(cdiv(q.F, DG_COLS) * parts)), dim3(256), 0, st, g, pre, dp, part, q.M, (int)q.F, q.act,
+                       q.gate_first, vec, rows);
+    FZ_TRY(check_launch("gated backward"));
+  } else {
+    FzLevel jobs;
+    int n = 0;
+    int64_t most = 0;
+    auto add = [&](const void* v, E* out, const float* row, int64_t r) {
+      jobs.job[n] = FzLevelJob{v, out, row, row ? top : nullptr, peaks + n * FZ_PEAKS, alpha + n, r, (int)q.I, fz_al16(v) && q.I % 8 == 0, row ? (int)parts : 0};
+      most = std::max(most, r * cdiv(q.I, 8));
+      ++n;
+    };
+    if (level && want_dx) add(q.w, b, nullptr, N);
+    if (level && want_dw) add(x, xo, scale, q.M);
+    const int spread = (int)std::min<int64_t>(FZ_PEAKS, cdiv(most, 256));
+    if (level) {
+      hipLaunchKernelGGL((fz_peak_kernel<T>), dim3(spread, n), dim3(256), 0, st, jobs);
+      FZ_TRY(check_launch("operand range"));
     }
-    segments(p, F32 ? (held ? 3 : 6) : 1);
+    const FzDgate d{g, pre, dp, a, held ? q.sw : nullptr, scale, top, part, q.M, q.M * ld, (int)q.F, q.act, q.gate_first, vec, rows};
+    FZ_TRY((part ? launch_dgate_rows<T, NP, true>(d, parts, st) : launch_dgate_rows<T, NP, false>(d, parts, st)));
+    if (level) {
+      hipLaunchKernelGGL((fz_level_kernel<T>), dim3((unsigned)std::min<int64_t>(2048, cdiv(most, 256)), n), dim3(256), 0, st, jobs, spread);
+      FZ_TRY(check_launch("operands"));
+    }
+  }
+  if (want_dx) {
+    if (held) FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, b, N, q.I, st));
+    p = prob(a, ld * 2, q.M * ld * 2, b, ldi * 2, N * ldi * 2, q.M, q.I, N, 2);
+    segments(p, sdx);
+    ep.out = dx;
+    ep.sa = scale;
+    ep.alpha = alpha;
     FZ_TRY((launch_gemm<E, T, false, true, FZ_PLAIN>(pdx, p, ep, sums, st)));
   }
   if (want_dw) {
-    FzProb p = prob(a.p, a.ld, a.plane, xo.p, xo.ld, xo.plane, N, q.I, q.M, 2);
-    segments(p, F32 ? 6 : 1);
-    FzEpi ep{};
+    p = prob(a, ld * 2, q.M * ld * 2, xo, ldi * 2, q.M * ldi * 2, N, q.I, q.M, 2);
+    segments(p, sdw);
     ep.out = dw;
+    ep.sa = nullptr;
+    ep.alpha = alpha ? alpha + want_dx : nullptr;
     FZ_TRY((launch_gemm<E, T, true, true, FZ_PLAIN>(pdw, p, ep, sums, st)));
   }
   if (part) {
@@ -621,9 +652,9 @@ int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const vo
   else if (dx) FZ_TRY(need16(who, "w", w));
   if (dw) FZ_TRY(need16(who, "x", x));
   FZ_TRY(need16(who, "dbase", dbase, true));
-  FZ_TRY(need16(who, "workspace", ws));
   const int flags = LYC_GATED_BACKWARD | (sw ? LYC_GATED_INT8 : 0) | (dbase ? LYC_GATED_DBASE : 0) | (dx ? LYC_GATED_DX : 0) | (dw ? LYC_GATED_DW : 0) |
                     (dbias ? LYC_GATED_DBIAS : 0);
+  FZ_TRY(need16(who, "workspace", ws, lyc_gated_linear_workspace_bytes(M, I, F, dtype, flags) == 0));
   FZ_DTYPE(dtype, return gated_bwd<T>(q, static_cast<const T*>(g), pre, static_cast<const T*>(x), static_cast<T*>(dbase),
                                       static_cast<T*>(dx), static_cast<T*>(dw), dbias, dbias_f32, flags, Carve{static_cast<char*>(ws)}, nullptr,
                                       static_cast<hipStream_t>(stream)));

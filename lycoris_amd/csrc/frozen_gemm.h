@@ -358,6 +358,12 @@ __device__ __forceinline__ void fz_store_pre8(void* pre, int64_t total, int64_t 
       }
   }
 }
+// 8 values of the two planes
+__device__ __forceinline__ void fz_join24(const u32x4& h, const u32x2& l, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)  // bytes: two of h, one of l, a zero
+    v[e] = __uint_as_float(__builtin_amdgcn_perm(h[e >> 1], l[e >> 2], (e & 1 ? 0x07060000u : 0x05040000u) | ((e & 3) << 8) | 0x0cu));
+}
 template <typename TO>
 __device__ __forceinline__ void fz_load_pre8(const void* pre, int64_t total, int64_t at, int n, int N, bool vec, float (&v)[8]) {
   if constexpr (sizeof(TO) == 4) {
@@ -366,11 +372,7 @@ __device__ __forceinline__ void fz_load_pre8(const void* pre, int64_t total, int
     const uint16_t* hi = static_cast<const uint16_t*>(pre) + at;
     const uint8_t* lo = reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(pre) + total) + at;
     if (vec) {
-      const u32x4 h = *reinterpret_cast<const u32x4*>(hi);
-      const u32x2 l = *reinterpret_cast<const u32x2*>(lo);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)  // bytes: two of h, one of l, a zero
-        v[e] = __uint_as_float(__builtin_amdgcn_perm(h[e >> 1], l[e >> 2], (e & 1 ? 0x07060000u : 0x05040000u) | ((e & 3) << 8) | 0x0cu));
+      fz_join24(*reinterpret_cast<const u32x4*>(hi), *reinterpret_cast<const u32x2*>(lo), v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = n + e < N ? __uint_as_float(((unsigned)hi[e] << 16) | ((unsigned)lo[e] << 8)) : 0.f;
@@ -729,7 +731,7 @@ struct FzKernel {
         }
         if constexpr (EPI == FZ_PLAIN) {
 #pragma unroll
-          for (int e = 0; e < CN; ++e) v[e] *= alpha * sa[mi];
+          for (int e = 0; e < CN; ++e) v[e] = v[e] * alpha * sa[mi];
         } else {
 #pragma unroll
           for (int e = 0; e < CN; ++e) {
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(256) void fz_reduce_kernel(FzProb p, FzEpi ep) {
     float v[8], t[8];
     const float sa = ep.sa ? ep.sa[m] : 1.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)s[e] * (alpha * sa);
+    for (int e = 0; e < 8; ++e) v[e] = (float)s[e] * alpha * sa;
     if (ep.sw) {
       fz_load8<float>(ep.sw, n, n, N, vs, t);
 #pragma unroll

@@ -193,27 +193,6 @@ __global__ __launch_bounds__(256) void fz_scale_long_kernel(const T* __restrict_
   }
 }
 
-// ---- fp16 only: the power of two that brings an 8-bit weight's scales into its range --------------------------------------------------
-// The gated backward takes sw inside dx's other operand (sw dp).  fp16 has 5 exponent bits and the scales of a weight may lie anywhere: they are multiplied by f[0] = 2^e, which brings 127 max|sw| to [2^-1, 1) 2^`top`, and the product's
-// alpha, f[1] = 2^-e, takes it out again.
-__global__ __launch_bounds__(256) void fz_range_kernel(const float* __restrict__ sw, int n, int top, float* __restrict__ f) {
-  __shared__ float red[4];
-  float mx = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const float a = fabsf(sw[i]);
-    if (a <= 3.4e38f) mx = fmaxf(mx, a);
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
-  __syncthreads();
-  if (threadIdx.x) return;
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int e = mx > 1e-30f && mx < 1e30f ? top - 8 - ilogbf(mx) : 0;  // 127 mx < 2^(ilogb + 8)
-  f[0] = ldexpf(1.f, e);
-  f[1] = ldexpf(1.f, -e);
-}
-
 // ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): its integers, which 16 bits hold exactly; the scales go to the other
 // operand.  Columns I .. ldo are zeros.  A workgroup takes four rows: 10240 x 1280 in 10 us (39 MB), and 5 - 8 us, most of them the launch,
 // for 1280 x 1280 and 1280 x 5120
@@ -285,17 +264,62 @@ __global__ __launch_bounds__(256) void fz_stage_kernel(FzStage jobs) {
   }
 }
 
+// the gated backward's 8 columns from k on of row m: the value half's and the gate half's part of dp
+template <int ACT>
+__device__ __forceinline__ void fz_dgate_of(const float (&gv)[8], const float (&v)[8], const float (&t)[8], float (&dv)[8], float (&dt)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float a, da;
+    fz_act_grad<ACT>(t[e], a, da);
+    dv[e] = gv[e] * a;
+    dt[e] = gv[e] * v[e] * da;
+  }
+}
+template <typename T, int ACT>
+__device__ __forceinline__ void fz_dgate8(const T* g, const void* pre, int64_t m, int64_t M, int k, int F, int vo, int go, bool full, float (&dv)[8],
+                                          float (&dt)[8]) {
+  const int64_t N = 2 * (int64_t)F;
+  float gv[8], v[8], t[8];
+  fz_load8<T>(g, m * F + k, k, F, full, gv);
+  fz_load_pre8<T>(pre, M * N, m * N + vo + k, k, F, full, v);
+  fz_load_pre8<T>(pre, M * N, m * N + go + k, k, F, full, t);
+  fz_dgate_of<ACT>(gv, v, t, dv, dt);
+}
+// what is read for it, 16 bits and whole chunks, as it lies in memory (loads that are in flight while another row is worked on)
+struct FzDgateRaw {
+  u32x4 g, v, t;
+  u32x2 vl, tl;
+  template <typename T>
+  __device__ __forceinline__ void load(const T* gp, const void* pre, int64_t m, int64_t M, int k, int F, int vo, int go) {
+    const int64_t N = 2 * (int64_t)F;
+    const uint16_t* hi = static_cast<const uint16_t*>(pre) + m * N + k;
+    const uint8_t* lo = reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(pre) + M * N) + m * N + k;
+    g = *reinterpret_cast<const u32x4*>(gp + m * F + k);
+    v = *reinterpret_cast<const u32x4*>(hi + vo);
+    t = *reinterpret_cast<const u32x4*>(hi + go);
+    vl = *reinterpret_cast<const u32x2*>(lo + vo);
+    tl = *reinterpret_cast<const u32x2*>(lo + go);
+  }
+  template <typename T, int ACT>
+  __device__ __forceinline__ void use(float (&dv)[8], float (&dt)[8]) const {
+    float gv[8], vv[8], tv[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gv[e] = (float)reinterpret_cast<const T*>(&g)[e];
+    fz_join24(v, vl, vv);
+    fz_join24(t, tl, tv);
+    fz_dgate_of<ACT>(gv, vv, tv, dv, dt);
+  }
+};
+
 // ---- gated backward, elementwise: dp = (g act(gate), g value act'(gate)) in the order of p's halves -----------------------------------
-// One pass over g and p writes what the rest of the backward pass reads: dp (rounded to the activation type: a gradient, and the operand of
-// dw and dx), dps = sw f[0] dp (one rounding; dx over an 8-bit weight whose plane is its integers, [M, up(2 F, 8)]), and the column sums of
-// dp before rounding, as one partial row per workgroup row (fixed order: the same bits every time).
+// One pass over g and p writes what the rest of the backward pass reads.  fz_dgate_kernel, where dp itself is all that is wanted, and for 32 bits:
+// dp, rounded to the activation type (it is the gradient of `base`), and the column sums of dp before rounding, as one partial row per
+// workgroup row (fixed order: the same bits every time).
 // A workgroup takes DG_COLS columns of each half and `rows` rows; a thread 8 columns of every 8th row, two rows in flight.
-// Bound by HBM, at the rate of a copy: bf16 8192 x 2560 in 48 us (252 MB), 4096 x 5120 with dp and dps in 65 (336 MB).
 constexpr int DG_COLS = 256;
-template <typename T, typename E>
-__global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const void* __restrict__ pre, T* __restrict__ dp, E* __restrict__ dps,
-                                                       const float* __restrict__ sw, const float* __restrict__ f, float* __restrict__ part, int64_t M, int F,
-                                                       int act, int gate_first, int vec, int rows) {
+template <typename T>
+__global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, const void* __restrict__ pre, T* __restrict__ dp, float* __restrict__ part,
+                                                       int64_t M, int F, int act, int gate_first, int vec, int rows) {
   __shared__ float sums[2][DG_COLS];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int across = (F + DG_COLS - 1) / DG_COLS, slab = (int)(blockIdx.x / across), c0 = ((int)blockIdx.x - slab * across) * DG_COLS;
@@ -303,46 +327,22 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
   const int64_t m0 = (int64_t)slab * rows;
   const int vo = gate_first ? F : 0, go = gate_first ? 0 : F;
   const bool full = vec && k + 8 <= F;
-  const int64_t N = 2 * (int64_t)F, lds = (N + 7) & ~7;
-  float sv[8], st[8], cv[8], ct[8];
+  const int64_t N = 2 * (int64_t)F;
+  float cv[8], ct[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) cv[e] = ct[e] = 0.f;
-  if (dps && k < F) {
-    fz_load8<float>(sw, vo + k, k, F, false, sv);
-    fz_load8<float>(sw, go + k, k, F, false, st);
-    const float scale = f ? f[0] : 1.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sv[e] *= scale, st[e] *= scale;
-  }
   auto each = [&](auto ac, auto fc) {
     constexpr bool FULL = decltype(fc)::value;
 #pragma unroll 2
     for (int r = ty; r < rows && m0 + r < M; r += 8) {
       const int64_t m = m0 + r;
-      float gv[8], v[8], t[8], dv[8], dt[8];
-      fz_load8<T>(g, m * F + k, k, F, FULL, gv);
-      fz_load_pre8<T>(pre, M * N, m * N + vo + k, k, F, FULL, v);
-      fz_load_pre8<T>(pre, M * N, m * N + go + k, k, F, FULL, t);
+      float dv[8], dt[8];
+      fz_dgate8<T, decltype(ac)::value>(g, pre, m, M, k, F, vo, go, FULL, dv, dt);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float a, da;
-        fz_act_grad<decltype(ac)::value>(t[e], a, da);
-        dv[e] = gv[e] * a;
-        dt[e] = gv[e] * v[e] * da;
-        cv[e] += dv[e];
-        ct[e] += dt[e];
-      }
+      for (int e = 0; e < 8; ++e) cv[e] += dv[e], ct[e] += dt[e];
       if (dp) {
         fz_store8<T>(dp, m * N + vo + k, k, F, FULL, dv);
         fz_store8<T>(dp, m * N + go + k, k, F, FULL, dt);
-      }
-      if (dps) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dv[e] *= sv[e], dt[e] *= st[e];
-        fz_store8<E>(dps, m * lds + vo + k, k, F, FULL, dv);
-        fz_store8<E>(dps, m * lds + go + k, k, F, FULL, dt);
-        if (!FULL && k + 8 >= F)  // the product reads whole 16-byte chunks
-          for (int64_t c = N; c < lds; ++c) dps[m * lds + c] = (E)0.f;
       }
     }
   };
@@ -364,6 +364,235 @@ __global__ __launch_bounds__(256) void fz_dgate_kernel(const T* __restrict__ g, 
     if (c < F) part[(int64_t)slab * N + (h ? go : vo) + c] = sums[h][threadIdx.x];
   }
 }
+
+// The same where products follow, 16 bits: beside dp (or without it) their operand, 2^e c[n] dp[m, n] in NP fp16 planes with a power of two a
+// row as in fz_scale_kernel, and scale[m] = 2^-e.  c: the scales of an 8-bit weight, or null.  dp rounded to bf16 as an operand cost dx and
+// dw 1.4 times the error of their own rounding each (2.34e-3 of the norm against 1.66e-3; this way 1.67e-3).
+// The largest of a row is known when all of it has been computed, so a row stays in the registers of its threads: a wave's where it has up to
+// 512 columns a half (WAVE: four waves a workgroup, each with rows of its own), else a workgroup's, a chunk of 8 columns a thread; rows of more than 8192
+// columns are computed twice, the second time out of the caches (NV = 0; two chunks a thread do not fit the 128 registers of 1024 threads).  `rows` rows follow each other; the column sums stay with the threads of their columns.
+// top: the largest scale of the slab's rows, for the other operand of dw.
+// Bound by HBM, short of a copy's rate by the meeting for each row's largest: bf16 4096 x 5120 with dp 75 us (336 MB), 8192 x 2560 without, with column sums, 69.
+struct FzDgate {
+  const void *g, *pre;
+  void* dp;
+  _Float16* out;
+  const float* c;
+  float *scale, *top, *part;
+  int64_t M, plane;
+  int F, act, gate_first, vec, rows;
+};
+template <typename T, int NP, int NV, bool WAVE, bool SUMS>
+__global__ __launch_bounds__(WAVE ? 256 : 1024) void fz_dgate_rows_kernel(FzDgate a) {
+  __shared__ unsigned red[2][16];
+  const int F = a.F, nt = WAVE ? 64 : (int)blockDim.x, t = WAVE ? (int)threadIdx.x & 63 : (int)threadIdx.x;
+  const int64_t slab = WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x, m0 = slab * a.rows;
+  const int vo = a.gate_first ? F : 0, go = a.gate_first ? 0 : F;
+  const int64_t N = 2 * (int64_t)F, lds = (N + 7) & ~7;
+  const T* g = static_cast<const T*>(a.g);
+  float top = 0.f;
+  int at = 0;
+  auto largest = [&](unsigned bits) {  // of the row, to each of its threads
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o));
+    if constexpr (!WAVE) {
+      if ((threadIdx.x & 63) == 0) red[at][threadIdx.x >> 6] = bits;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the LDS write; __syncthreads() might wait for the next row's loads too
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      bits = 0;
+      for (int w = 0; w < nt / 64; ++w) bits = max(bits, red[at][w]);
+      at ^= 1;  // the next row's go where nobody reads this row's any more
+    }
+    return bits;
+  };
+  auto peak = [](const float (&v)[8], unsigned bits) {  // of the finite ones
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned u = __float_as_uint(v[e]) & 0x7fffffffu;
+      bits = u < 0x7f800000u ? max(bits, u) : bits;
+    }
+    return bits;
+  };
+  auto put = [&](int64_t m, int k, bool full, const float (&dv)[8], const float (&dt)[8]) {
+    if (a.dp) {
+      fz_store8<T>(a.dp, m * N + vo + k, k, F, full, dv);
+      fz_store8<T>(a.dp, m * N + go + k, k, F, full, dt);
+    }
+  };
+  auto times_c = [&](int k, bool full, float (&dv)[8], float (&dt)[8]) {
+    if (!a.c) return;
+    float cv[8], ct[8];
+    fz_load8<float>(a.c, vo + k, k, F, full, cv);
+    fz_load8<float>(a.c, go + k, k, F, full, ct);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dv[e] *= cv[e], dt[e] *= ct[e];
+  };
+  auto planes = [&](int64_t m, int k, bool full, float up, float (&v)[8], int half) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= up;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      _Float16* out = a.out + p * a.plane;
+      fz_store8<_Float16>(out, m * lds + half + k, k, F, full, v);
+      if (p + 1 < NP) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float h = (float)(_Float16)v[e];
+          v[e] = fabsf(h) <= FLT_MAX ? v[e] - h : 0.f;
+        }
+      }
+      if (!full && k + 8 >= F)  // the products read whole 16-byte chunks
+        for (int64_t c = N; c < lds; ++c) out[m * lds + c] = (_Float16)0.f;
+    }
+  };
+  fz_for_act(a.act, [&](auto ac) {
+    constexpr int ACT = decltype(ac)::value;
+    if constexpr (NV == 1) {
+      const int k = t * 8;
+      const bool in = k < F;
+      float sv[8], st[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sv[e] = st[e] = 0.f;
+      FzDgateRaw raw;
+      if (a.vec && in && m0 < a.M) raw.template load<T>(g, a.pre, m0, a.M, k, F, vo, go);
+      for (int r = 0; r < a.rows && m0 + r < a.M; ++r) {
+        const int64_t m = m0 + r;
+        float dv[8], dt[8];
+        unsigned bits = 0;
+        if (in) {
+          if (a.vec) {
+            const FzDgateRaw now = raw;
+            if (r + 1 < a.rows && m + 1 < a.M) raw.template load<T>(g, a.pre, m + 1, a.M, k, F, vo, go);  // in flight while this row is worked on
+            now.template use<T, ACT>(dv, dt);
+          } else {
+            fz_dgate8<T, ACT>(g, a.pre, m, a.M, k, F, vo, go, false, dv, dt);
+          }
+          if constexpr (SUMS) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sv[e] += dv[e], st[e] += dt[e];
+          }
+          put(m, k, a.vec, dv, dt);
+          times_c(k, a.vec, dv, dt);
+          bits = peak(dv, peak(dt, 0));
+        }
+        float down;
+        const float up = fz_up_of(largest(bits), &down);
+        if (t == 0) a.scale[m] = down;
+        top = fmaxf(top, down);
+        if (in) {
+          planes(m, k, a.vec, up, dv, vo);
+          planes(m, k, a.vec, up, dt, go);
+        }
+      }
+      if (SUMS && in && m0 < a.M) {
+        fz_store8<float>(a.part, slab * N + vo + k, k, F, a.vec, sv);
+        fz_store8<float>(a.part, slab * N + go + k, k, F, a.vec, st);
+      }
+    } else {
+      for (int r = 0; r < a.rows && m0 + r < a.M; ++r) {
+        const int64_t m = m0 + r;
+        float dv[8], dt[8];
+        unsigned bits = 0;
+        for (int k = t * 8; k < F; k += nt * 8) {
+          fz_dgate8<T, ACT>(g, a.pre, m, a.M, k, F, vo, go, a.vec, dv, dt);
+          put(m, k, a.vec, dv, dt);
+          if constexpr (SUMS) {  // the slab's partial sums, each the same thread's in every row
+            float s[8];
+            const int64_t pv = slab * N + vo + k, pt = slab * N + go + k;
+            fz_load8<float>(a.part, pv, k, r ? F : 0, r && a.vec, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += dv[e];
+            fz_store8<float>(a.part, pv, k, F, a.vec, s);
+            fz_load8<float>(a.part, pt, k, r ? F : 0, r && a.vec, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += dt[e];
+            fz_store8<float>(a.part, pt, k, F, a.vec, s);
+          }
+          times_c(k, a.vec, dv, dt);
+          bits = peak(dv, peak(dt, bits));
+        }
+        float down;
+        const float up = fz_up_of(largest(bits), &down);
+        if (t == 0) a.scale[m] = down;
+        top = fmaxf(top, down);
+        for (int k = t * 8; k < F; k += nt * 8) {
+          fz_dgate8<T, ACT>(g, a.pre, m, a.M, k, F, vo, go, a.vec, dv, dt);
+          times_c(k, a.vec, dv, dt);
+          planes(m, k, a.vec, up, dv, vo);
+          planes(m, k, a.vec, up, dt, go);
+        }
+      }
+    }
+  });
+  if (a.top && t == 0 && m0 < a.M) a.top[slab] = top;
+}
+
+// ---- the 16-bit weight and x as fp16 operands of dx and dw, 16 bits ---------------------------------------------------------------------
+// Each takes one power of two: the weight 2^f that brings its largest entry to [2^14, 2^15); x 2^f scale[m] (the row scales of dp's operand come
+// back in here, along the K of dw), its f from the largest of x and the largest scale.  What fp16 loses of bf16 values that way lies 2^-28 and more
+// below the largest.  fz_peak_kernel takes the largest finite entries, one partial a workgroup; fz_level_kernel joins the partials, writes the
+// operands, and 2^-f for the products' alpha.  blockIdx.y: the operand.
+constexpr int FZ_PEAKS = 1024;
+struct FzLevelJob {
+  const void* x;
+  _Float16* out;
+  const float *row, *top;  // row scales and their largest a slab, or null
+  unsigned* part;
+  float* alpha;
+  int64_t rows;
+  int cols, vec, tops;
+};
+struct FzLevel {
+  FzLevelJob job[2];
+};
+template <typename T>
+__global__ __launch_bounds__(256) void fz_peak_kernel(FzLevel jobs) {
+  __shared__ unsigned red[4];
+  const FzLevelJob& j = jobs.job[blockIdx.y];
+  const T* x = static_cast<const T*>(j.x);
+  const int64_t n = j.rows * j.cols;
+  const bool vec = fz_al16(x);
+  unsigned bits = 0;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+    float v[8];
+    fz_load8<T>(x, i, 0, n - i < 8 ? (int)(n - i) : 8, vec && n - i >= 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned u = __float_as_uint(v[e]) & 0x7fffffffu;
+      bits = u < 0x7f800000u ? max(bits, u) : bits;
+    }
+  }
+  bits = fz_row_max<256>(bits, red);
+  if (threadIdx.x == 0) j.part[blockIdx.x] = bits;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void fz_level_kernel(FzLevel jobs, int peaks) {
+  __shared__ unsigned red[2][4];
+  const FzLevelJob& j = jobs.job[blockIdx.y];
+  const T* x = static_cast<const T*>(j.x);
+  unsigned bits = 0, top = 0;
+  for (int i = threadIdx.x; i < peaks; i += 256) bits = max(bits, j.part[i]);
+  for (int i = threadIdx.x; i < j.tops; i += 256) top = max(top, __float_as_uint(j.top[i]));  // powers of two: ordered like their bits
+  bits = fz_row_max<256>(bits, red[0]);
+  top = fz_row_max<256>(top, red[1]);
+  const int f = max(-126, min(126, 14 - ((int)(bits >> 23) - 127) - (j.tops ? (int)(top >> 23) - 127 : 0)));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *j.alpha = __uint_as_float((unsigned)(127 - f) << 23);
+  const int64_t chunks = (j.cols + 7) >> 3, ldo = chunks * 8, n = j.rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int k = (int)(i - r * chunks) * 8;
+    const int e2 = f + (j.row ? (int)(__float_as_uint(j.row[r]) >> 23) - 127 : 0);
+    const float up = e2 < -126 ? 0.f : __uint_as_float((unsigned)(min(e2, 127) + 127) << 23);
+    float v[8];
+    _Float16 t[8];
+    fz_row8<T>(x + r * j.cols, k, j.cols, j.vec, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (_Float16)(v[e] * up);
+    *reinterpret_cast<u32x4*>(j.out + r * ldo + k) = *reinterpret_cast<u32x4*>(t);
+  }
+}
+
 // the partial rows' sum: 8 threads a column, joined in a fixed order (128 rows of 5120: 4 us, the launch)
 template <typename T>
 __global__ __launch_bounds__(256) void fz_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t parts, int N) {

@@ -140,9 +140,9 @@ def held(gen, N, K):
     return ops.int8_quantize(w.to(DEV))
 
 
-# terms of dx = (g sw) wq: in fp16 with a power of two a row, one rounding (2^-12) beside bf16 gradients; two planes (2^-22) beside fp16 ones.  Below 2^-14
+# terms of dx = (g sw) wq: in fp16 with a power of two a row, one rounding (eps / 2 = 2^-11: 11 significant bits) beside bf16 gradients; two planes (2^-22) beside fp16 ones.  Below 2^-14
 # of what fp16 holds the step is fixed: 2^-39 of the row's largest (half a step).  Sums: n e of the magnitudes.
-TERM = {torch.bfloat16: 2.0 ** -12, torch.float16: 2.0 ** -22}
+TERM = {torch.bfloat16: torch.finfo(torch.float16).eps / 2, torch.float16: 2.0 ** -22}
 
 
 def check_dx(dx, g, wq, sw, dt):
@@ -201,3 +201,117 @@ def test_dx_of_rows_of_every_magnitude(dt):
     d2, = torch.autograd.grad(ops.int8_linear(x2, wq, sw), x2, bad)
     rest = [m for m in range(M) if m not in (40, 41)]
     assert torch.equal(d2[rest], dx[rest]) and torch.isnan(d2[40]).all() and not torch.isfinite(d2[41]).any()
+
+
+def gated64(x, w64, wmag, bias, base, act_grad, g, dt, c, p=None):
+    """dp in 64 bits, and what an element of it may be off by before it is an operand: p in 24 bits, the activation, the sums of p"""
+    K, F = x.shape[-1], w64.shape[0] // 2
+    x64, g64 = x.double().cpu(), g.double().cpu()
+    Sp = x64.abs() @ wmag.t()
+    p = x64 @ w64.t() if p is None else p
+    for t in (bias, base):
+        if t is not None:
+            p, Sp = p + t.double().cpu(), Sp + t.double().cpu().abs()
+    ep = 2.0 ** -16 * p.abs() + (K + 8) * E * Sp
+    v, t = p.split(F, 1)
+    ev, et = ep.split(F, 1)
+    a, da = act_grad(t)
+    afp = ACT_ERR * (t.abs() + 1)
+    dv, d = g64 * a, g64 * v * da
+    edv = g64.abs() * (1.2 * et + afp + E * a.abs())
+    ed = g64.abs() * ((da.abs() + afp) * ev + (v.abs() + ev) * (et + afp) + 3 * E * (v * da).abs())
+    return torch.cat((dv, d), 1), torch.cat((edv, ed), 1)
+
+
+def check_gated(got, x, w64, dp, edp, c, dt, rows=None):
+    """dx and dw against dp in 64 bits: dp takes one rounding as an operand (TERM of it; c: an 8-bit weight's scales), 2^-39 of its row's largest at least;
+    the other operands are exact down to 2^-39 of their largest"""
+    u, f = torch.finfo(dt).eps / 2, torch.finfo(dt)
+    planes = 1 if dt == torch.bfloat16 else 2
+    x64, N, M = x.double().cpu(), dp.shape[1], dp.shape[0]
+    top = (dp * c).abs().amax(1, keepdim=True)
+    step = 2.0 ** -39
+    e = edp + (TERM[dt] + 2 * E) * (dp.abs() + edp) + step * top / c
+    stats = {}
+    wmax = w64.abs().max()
+    want, mag = dp @ w64, dp.abs() @ w64.abs()
+    bound = {"dx": e @ w64.abs() * 1.01 + (planes * N + 4) * E * mag * 1.01 + step * wmax * dp.abs().sum(1, keepdim=True)}
+    wants = {"dx": want}
+    if "dw" in got:
+        wants["dw"], mag = dp.t() @ x64, dp.abs().t() @ x64.abs()
+        lost = step * 2 * top.max() * x64.abs().max() * (dp.abs() / top.clamp_min(1e-300)).sum(0)[:, None]
+        bound["dw"] = e.t() @ x64.abs() * 1.01 + (planes * M + 4) * E * mag * 1.01 + lost
+    for n, want in wants.items():
+        b = bound[n] + u * (want.abs() + bound[n]) + f.smallest_normal * f.eps / 2
+        off = (got[n].double().cpu() - want).abs()
+        assert torch.isfinite(got[n]).all() and (off <= b).all(), (n, float((off - b).max()), float((off / b).max()))
+        stats[n] = float(off.norm() / want.norm()), float((want.to(dt).double() - want).norm() / want.norm())
+    return stats
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["plain", "int8"])
+@pytest.mark.parametrize("dt", HALVES, ids=IDS)
+@pytest.mark.parametrize("M,K,F", [(1, 16, 8), (3, 33, 5), (70, 64, 200), (300, 136, 512), (257, 72, 513), (130, 320, 1280), (64, 40, 2560), (50, 24, 8192), (33, 17, 8201), (9, 24, 16384),
+                                   (7, 16, 16392), (5, 9, 20003), (2100, 640, 264)])
+def test_gated_gradients_are_rounded_once(M, K, F, dt, int8):
+    gen = torch.Generator().manual_seed(M + K + F)
+    x = torch.randn(M, K, generator=gen).to(dt).to(DEV)
+    bias = (0.2 * torch.randn(2 * F, generator=gen)).to(dt).to(DEV)
+    g = (torch.randn(M, F, generator=gen) / math.sqrt(F)).to(dt).to(DEV)
+    sw, c, p = None, 1.0, None
+    if int8:
+        w, sw = held(gen, 2 * F, K)
+        c = sw.double().cpu()
+        w64 = w.double().cpu() * c[:, None]
+        q, s = ops.int8_quantize(x)
+        p = (q.double().cpu() @ w.double().cpu().t()) * s.double().cpu()[:, None] * c
+    else:
+        w = (torch.randn(2 * F, K, generator=gen) / math.sqrt(K)).to(dt).to(DEV)
+        w64 = w.double().cpu()
+    leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(not int8), bias.clone().requires_grad_(True)]
+    h = ops.gated_linear(*leaves, act="silu", weight_scale=sw)
+    names = ["dx", "dbias"] if int8 else ["dx", "dw", "dbias"]
+    got = dict(zip(names, torch.autograd.grad(h, [t for t in leaves if t.requires_grad], g)))
+    dp, edp = gated64(x, w64, w64.abs(), bias, None, silu64, g, dt, c, p)
+    stats = check_gated(got, x, w64, dp, edp, c, dt)
+    if M * K > 5000 and M > 100:
+        assert all(here < 1.03 * once for here, once in stats.values()), stats
+    u = torch.finfo(dt).eps / 2
+    eb = edp.sum(0) + (M + 8) * E * dp.abs().sum(0)
+    assert ((got["dbias"].double().cpu() - dp.sum(0)).abs() <= eb + u * (dp.sum(0).abs() + eb) + 2.0 ** -25).all()
+    for which in range(2 - int8):  # each gradient by itself: the same bits
+        one = [t.detach().clone().requires_grad_(i == which) for i, t in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(ops.gated_linear(*one, act="silu", weight_scale=sw), one[which], g)[0], got[names[which]])
+
+
+@pytest.mark.parametrize("F", [40, 700, 17000], ids=["wave", "workgroup", "twice"])
+@pytest.mark.parametrize("dt", HALVES, ids=IDS)
+def test_gated_gradients_of_rows_of_every_magnitude(dt, F):
+    """gradients from the type's smallest to large ones, rows and weight rows of zeros, rows that are not finite"""
+    gen = torch.Generator().manual_seed(17)
+    M, K = 64, 24
+    x, w = torch.randn(M, K, generator=gen).to(dt), (torch.randn(2 * F, K, generator=gen) / math.sqrt(K)).to(dt)
+    w[3], w[F + 5] = 0, 0  # dw of a zero row is not zero
+    g = torch.randn(M, F, generator=gen)
+    lo, hi = (-14, 4) if dt == torch.float16 else (-100, 60)
+    g *= 2.0 ** torch.linspace(lo, hi, M)[torch.randperm(M, generator=gen)][:, None]
+    g[11] = 0
+    x, w, g = x.to(DEV), w.to(DEV), g.to(dt).to(DEV)
+
+    def grads(x, g):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        return dict(zip(("dx", "dw"), torch.autograd.grad(ops.gated_linear(xl, wl, act="silu"), [xl, wl], g)))
+
+    got = grads(x, g)
+    dp, edp = gated64(x, w.double().cpu(), w.double().cpu().abs(), None, None, silu64, g, dt, 1.0)
+    check_gated(got, x, w.double().cpu(), dp, edp, 1.0, dt)
+    assert (got["dx"][11] == 0).all()
+    bad = g.clone()
+    bad[20, 7], bad[21, 0] = float("nan"), float("inf")
+    d = grads(x, bad)
+    rest = [m for m in range(M) if m not in (20, 21)]
+    assert torch.equal(d["dx"][rest], got["dx"][rest]) and torch.isnan(d["dx"][20]).all() and not torch.isfinite(d["dx"][21]).any()
+    clean = [o for o in range(2 * F) if o not in (7, F + 7, 0, F)]  # the other rows of dw see the finite entries alone
+    assert torch.isfinite(d["dw"][clean]).all() and ((d["dw"][clean].double() - got["dw"][clean].double()).norm() <= 2.0 ** -6 * got["dw"][clean].double().norm())
+    zero = torch.zeros_like(g)
+    assert all((t == 0).all() for t in grads(x, zero).values())
