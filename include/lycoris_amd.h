@@ -497,6 +497,11 @@ enum { LYC_GATED_INT8 = 1, LYC_GATED_BACKWARD = 2, LYC_GATED_DBASE = 4, LYC_GATE
 int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dtype, int flags);
 int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* h, void* pre,
                          void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream);
+/* How a product is run, for tools and tests: the tile's columns (64, 128, 160, 256; 32: the kernel for up to 32 rows) plus 2^16 times the
+ * parts its K is cut into; -1: bad arguments.  M, K, N: those of the layer (gated: I and F).  flags: LYC_GATED_INT8 (the weight), LYC_GATED_DBASE (a
+ * `base` is given), LYC_GATED_BACKWARD (p is kept): of the gated products.                                                           */
+enum { LYC_PRODUCT_INT8_FWD = 0, LYC_PRODUCT_INT8_DX = 1, LYC_PRODUCT_GATED_FWD = 2, LYC_PRODUCT_GATED_DX = 3, LYC_PRODUCT_GATED_DW = 4 };
+int lyc_frozen_plan(int product, int64_t M, int64_t K, int64_t N, int dtype, int flags);
 int lyc_gated_linear_bwd(const void* g, const void* pre, const void* x, const void* w, int64_t ldw, const float* sw, void* dbase, void* dx, void* dw,
                          void* dbias, void* ws, int64_t M, int64_t I, int64_t F, int act, int gate_first, int dtype, void* stream);
 

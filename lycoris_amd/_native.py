@@ -94,6 +94,7 @@ VALUE_SIGNATURES = {
     "lyc_int8_matmul_workspace_bytes": ([_i64, _i64, _i64, _i32], ctypes.c_int64),
     "lyc_int8_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
     "lyc_gated_linear_workspace_bytes": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_int64),
+    "lyc_frozen_plan": ([_i32, _i64, _i64, _i64, _i32, _i32], ctypes.c_int),  # tile + 2^16 parts, not an error code
     "lyc_loha_plane_cacheable": ([_fp, _fp, _fp, _fp, _i32, _i32, _i32, _i32], ctypes.c_int),
 }
 

@@ -319,18 +319,26 @@ int check_q(const char* who, const char* what, const void* q, int64_t ld, int64_
   return LYC_OK;
 }
 
+// the operand type of the backward pass's products, and the planes of the gradient's operand
+template <typename T>
+using GradE = typename std::conditional<sizeof(T) == 4, __bf16, _Float16>::type;
+template <typename T>
+constexpr int grad_planes() { return sizeof(T) == 4 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1; }
+template <typename T>
+Plan plan_dx8(int64_t M, int64_t K, int64_t N) { return plan_of<GradE<T>, FZ_PLAIN>(M, K, N, grad_planes<T>(), sizeof(T)); }
+
 // ---- dx of a frozen 8-bit layer: (g sw) [M, N] times the integers wq [N, K], which 16 bits hold exactly.  g sw takes a power of two a row in fp16
 //      (fz_scale_kernel; fp16 gradients: two planes), for fp32 gradients three bf16 planes ---------------------------------------------
 template <typename T>
 int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve ws, int64_t* bytes, int64_t M, int64_t N, int64_t K, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int NP = F32 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1;
-  using E = typename std::conditional<F32, __bf16, _Float16>::type;
+  constexpr int NP = grad_planes<T>();
+  using E = GradE<T>;
   const int64_t ld = up(N, 8);
   E* plane = ws.take<E>(N * up(K, 8));
   E* rows = ws.take<E>(NP * M * ld);
   float* scale = F32 ? nullptr : ws.take<float>(M);
-  const Plan pl = plan_of<E, FZ_PLAIN>(M, K, N, NP, sizeof(T));
+  const Plan pl = plan_dx8<T>(M, K, N);
   char* part = ws.take<char>(part_bytes(pl, M, K));
   if (bytes) {
     *bytes = ws.used;
@@ -361,13 +369,26 @@ struct Gated {
   int act, gate_first;
 };
 
+// eb: what the epilogue moves per output
+template <typename T>
+Plan plan_gated_fwd(int64_t M, int64_t I, int64_t F, bool held, bool base, bool keep) {
+  const double eb = (double)sizeof(T) * (base ? 3 : 1) + (keep ? sizeof(T) == 4 ? 8.0 : 6.0 : 0.0);
+  return held ? plan_of<int8_t, FZ_GATED>(M, F, I, 1, eb) : plan_of<typename Operand<T>::E, FZ_GATED>(M, F, I, sizeof(T) == 4 ? 6 : 1, eb);
+}
+template <typename T>
+int gated_segments(bool held) { return sizeof(T) == 4 && !held ? 6 : grad_planes<T>(); }
+template <typename T>
+Plan plan_gated_dx(int64_t M, int64_t I, int64_t F, bool held) { return plan_of<GradE<T>, FZ_PLAIN>(M, I, 2 * F, gated_segments<T>(held), sizeof(T)); }
+template <typename T>
+Plan plan_gated_dw(int64_t M, int64_t I, int64_t F) { return plan_of<GradE<T>, FZ_PLAIN>(2 * F, I, M, gated_segments<T>(false), sizeof(T)); }
+
 template <typename T>
 int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const T* base, T* h, void* pre, Carve ws, int64_t* bytes, hipStream_t st) {
   using E = typename Operand<T>::E;
   FzEpi ep{};
   ep.out = h; ep.pre = pre; ep.bias = bias; ep.bias_f32 = bias_f32; ep.base = base; ep.sw = q.sw; ep.act = q.act; ep.gate_first = q.gate_first; ep.F = (int)q.F;
   ep.pre_total = 2 * q.M * q.F;
-  const double eb = (double)sizeof(T) * (base ? 3 : 1) + (pre ? sizeof(T) == 4 ? 8.0 : 6.0 : 0.0);  // what the epilogue moves per output
+  const Plan pl = plan_gated_fwd<T>(q.M, q.I, q.F, q.sw != nullptr, base != nullptr, pre != nullptr);
   if (q.sw) {
     const int64_t ldq = up(q.I, 16);
     const bool fused = skinny_fused(q.M, q.I);
@@ -385,7 +406,7 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
     ep.sa = sa;
     FzProb p = prob(xq, ldq, 0, q.w, q.ldw, 0, q.M, 2 * q.F, q.I, 1);
     if (q.M <= SKINNY_ROWS) return launch_skinny<int8_t, T, T, true, false>(nullptr, p, ep, st);
-    return launch_gemm<int8_t, T, false, false, FZ_GATED>(plan_of<int8_t, FZ_GATED>(q.M, q.F, q.I, 1, eb), p, ep, nullptr, st);
+    return launch_gemm<int8_t, T, false, false, FZ_GATED>(pl, p, ep, nullptr, st);
   }
   Operand<T> a(ws, q.M, q.I, true), b(ws, 2 * q.F, q.I, true);
   if (bytes) {
@@ -401,7 +422,7 @@ int gated_fwd(const Gated& q, const T* x, const void* bias, int bias_f32, const 
   if constexpr (sizeof(T) == 2) {
     if (q.M <= SKINNY_ROWS) return launch_skinny<E, T, T, true, false>(nullptr, p, ep, st);
   }
-  return launch_gemm<E, T, false, false, FZ_GATED>(plan_of<E, FZ_GATED>(q.M, q.F, q.I, sizeof(T) == 4 ? 6 : 1, eb), p, ep, nullptr, st);
+  return launch_gemm<E, T, false, false, FZ_GATED>(pl, p, ep, nullptr, st);
 }
 
 // rows a workgroup of the elementwise pass takes: as many as leave 1024 workgroups (four a CU), 64 at most (fewer partial column sums)
@@ -431,8 +452,8 @@ int launch_dgate_rows(const FzDgate& a, int64_t slabs, hipStream_t st) {
 template <typename T>
 int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T* dx, T* dw, void* dbias, bool dbias_f32, int flags, Carve ws, int64_t* bytes, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int NP = F32 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1, NB = F32 ? 3 : 1;  // planes of dp, of the weight and of x
-  using E = typename std::conditional<F32, __bf16, _Float16>::type;
+  constexpr int NP = grad_planes<T>(), NB = F32 ? 3 : 1;  // planes of dp, of the weight and of x
+  using E = GradE<T>;
   const bool held = flags & LYC_GATED_INT8, want_dx = flags & LYC_GATED_DX, want_dw = flags & LYC_GATED_DW, want_db = flags & LYC_GATED_DBIAS;
   const bool products = want_dx || want_dw, by_row = products && !F32, level = by_row && !held;
   const int rows = by_row ? dgate_slab_rows(q.M, q.F) : dgate_rows(q.M, q.F);
@@ -446,8 +467,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   unsigned* peaks = level ? ws.take<unsigned>(2 * FZ_PEAKS) : nullptr;
   float* alpha = level ? ws.take<float>(2) : nullptr;
   float* part = want_db ? ws.take<float>(parts * N) : nullptr;
-  const int sdx = F32 && !held ? 6 : NP, sdw = F32 ? 6 : NP;  // segments
-  const Plan pdx = plan_of<E, FZ_PLAIN>(q.M, q.I, N, sdx, sizeof(T)), pdw = plan_of<E, FZ_PLAIN>(N, q.I, q.M, sdw, sizeof(T));
+  const Plan pdx = plan_gated_dx<T>(q.M, q.I, q.F, held), pdw = plan_gated_dw<T>(q.M, q.I, q.F);
   char* sums = ws.take<char>(std::max(want_dx ? part_bytes(pdx, q.M, q.I) : 0, want_dw ? part_bytes(pdw, N, q.I) : 0));
   if (bytes) {
     *bytes = ws.used;
@@ -495,7 +515,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   if (want_dx) {
     if (held) FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, b, N, q.I, st));
     p = prob(a, ld * 2, q.M * ld * 2, b, ldi * 2, N * ldi * 2, q.M, q.I, N, 2);
-    segments(p, sdx);
+    segments(p, gated_segments<T>(held));
     ep.out = dx;
     ep.sa = scale;
     ep.alpha = alpha;
@@ -503,7 +523,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
   }
   if (want_dw) {
     p = prob(a, ld * 2, q.M * ld * 2, xo, ldi * 2, q.M * ldi * 2, N, q.I, q.M, 2);
-    segments(p, sdw);
+    segments(p, gated_segments<T>(false));
     ep.out = dw;
     ep.sa = nullptr;
     ep.alpha = alpha ? alpha + want_dx : nullptr;
@@ -620,6 +640,22 @@ int64_t lyc_gated_linear_workspace_bytes(int64_t M, int64_t I, int64_t F, int dt
     FZ_DTYPE(dtype, (void)gated_fwd<T>(q, nullptr, nullptr, 0, nullptr, nullptr, nullptr, ws, &n, nullptr));
   }
   return n;
+}
+
+int lyc_frozen_plan(int product, int64_t M, int64_t K, int64_t N, int dtype, int flags) {
+  const bool gated = product >= LYC_PRODUCT_GATED_FWD, held = flags & LYC_GATED_INT8;
+  const Gated q{nullptr, 16, nullptr, M, K, N, 0, 0};
+  if (product < 0 || product > LYC_PRODUCT_GATED_DW || (gated ? check_gated("frozen_plan", q, true, dtype) : check_dims("frozen_plan", M, N, K, dtype)) != LYC_OK) return -1;
+  const bool few = M <= SKINNY_ROWS && (product == LYC_PRODUCT_INT8_FWD || (product == LYC_PRODUCT_GATED_FWD && (held || dtype != LYC_F32)));
+  Plan pl;
+  FZ_DTYPE(dtype, switch (product) {
+    case LYC_PRODUCT_INT8_FWD: pl = plan8(M, N, K, dtype); break;
+    case LYC_PRODUCT_INT8_DX: pl = plan_dx8<T>(M, K, N); break;
+    case LYC_PRODUCT_GATED_FWD: pl = plan_gated_fwd<T>(M, K, N, held, flags & LYC_GATED_DBASE, flags & LYC_GATED_BACKWARD); break;
+    case LYC_PRODUCT_GATED_DX: pl = plan_gated_dx<T>(M, K, N, held); break;
+    default: pl = plan_gated_dw<T>(M, K, N);
+  });
+  return few ? 32 + (1 << 16) : pl.tile + (pl.ksplit << 16);
 }
 
 int lyc_gated_linear_fwd(const void* x, const void* w, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* h, void* pre,
