@@ -472,7 +472,8 @@ int lyc_rows_to_nchw(const void* rows, void* t, int64_t B, int64_t C, int64_t P,
  * and its input quantised the same way, one scale a row, on every call.  A row that holds an infinity or a NaN gets scale NaN.
  * Rows of 8-bit operands: 16-byte aligned base, pitch a multiple of 16.  K < 2^17 (the int32 sums cannot overflow), M <= 2^26.
  * `bias`: [N], fp32 when bias_f32, else `dtype`; `base`: [M, N] in `dtype` (an adapter's output), either may be NULL.
- * `ws`: device scratch of the *_workspace_bytes(...) bytes (-1: bad arguments), 16-byte aligned, no need to clear.        */
+ * `ws`: device scratch of the *_workspace_bytes(...) bytes (-1: bad arguments), 16-byte aligned, no need to clear.
+ * M = 0 is no error: nothing is launched and nothing written (the sums over no rows, dw and dbias below, are the caller's to clear).  */
 int lyc_int8_quantize(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t M, int64_t K, int dtype, void* stream);
 /* y = (sa[m] sb[n]) sum_k aq[m, k] bq[n, k] + bias[n] + base[m, n].  aq's rows hold ZEROS from K up to the next multiple of 16. */
 int64_t lyc_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
@@ -481,7 +482,8 @@ int lyc_int8_matmul(const int8_t* aq, int64_t lda, const float* sa, const int8_t
 int64_t lyc_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int backward);
 int lyc_int8_linear_fwd(const void* x, const int8_t* wq, int64_t ldw, const float* sw, const void* bias, int bias_f32, const void* base, void* y, void* ws,
                         int64_t M, int64_t N, int64_t K, int dtype, void* stream);
-/* dx = g (sw wq): the gradient is not quantised; the weight is expanded to the activation type (32 bits: three bf16 products) */
+/* dx = g (sw wq): the gradient is not quantised.  Its operands: wq as it is; g sw in fp16 with a power of two a row (fp16: two planes; fp32: three
+ * bf16 planes) */
 int lyc_int8_linear_bwd(const void* g, const int8_t* wq, int64_t ldw, const float* sw, void* dx, void* ws, int64_t M, int64_t N, int64_t K, int dtype,
                         void* stream);
 

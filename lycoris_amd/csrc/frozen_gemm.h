@@ -55,8 +55,9 @@ struct FE<int8_t> {
 enum { FZ_ACT_GELU = 0, FZ_ACT_GELU_TANH = 1, FZ_ACT_SILU = 2 };
 
 // Phi(t) = erfc(-t / sqrt 2) / 2 with erfc(z) = w P(w) exp(-z^2), w = 1 / (1 + 0.45 z): P is the degree-7 polynomial of least largest
-// relative error on z = 0 .. 14 (3.5e-7, fitted to erfc in 64 bits); in fp32 Phi is off by 1.2e-6 of itself down to t = -6, where the
-// rounding of t^2 takes over.  About 20 operations, where the library's erfc takes three times that and a branch.
+// relative error on z = 0 .. 14 (3.5e-7, fitted to erfc in 64 bits).  Measured against 64 bits at two million points each, relative to Phi: 6.4e-7 on
+// [0, 8], 1.0e-6 on [-3, 0], 2.2e-6 on [-6, -3], 3.9e-6 on [-9, -6] (the rounding of t^2, which the exponential magnifies by t^2 / 2); it
+// underflows with exp(-t^2 / 2), below t = -13.  About 20 operations, where the library's erfc takes three times that and a branch.
 __device__ __forceinline__ void fz_phi(float t, float& phi, float& e) {
   const float z = 0.70710678f * fabsf(t);
   const float w = __builtin_amdgcn_rcpf(fmaf(0.45f, z, 1.f));
@@ -140,13 +141,12 @@ struct FzStep {
   unsigned mask;
 };
 
-// One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A ring slot holds SB = 64 or 128 bytes of K:
-// one or two MFMA steps.
+// One operand of one workgroup tile: DMA addressing (issue) and fragment addressing (read).  A ring slot holds SB = 64 (both operands
+// K-strided) or 128 bytes of K: one or two MFMA steps.
 //   ROWS: tile extent; W: waves along it; NW: waves in all; KS: K-strided in memory; PAIRED: the n operand (paired tile order; with an odd
 //   number of 16-row tiles a wave, as in 160 rows over two waves, the last one is in natural order)
-// K-contiguous: LDS rows of SB bytes, their 16-byte chunks XOR-permuted on the DMA's source address so that a fragment read falls on
-// different slots of the 256-byte bank row.  The hardware serves ds_read_b128 in groups of lanes 0-3, 12-15, 20-27 and so on: with 64-byte
-// rows the permutation is 0 2 3 1 over bits 2, 3 of the row (3, 4 in paired order); 0 1 2 3 cost a conflict on every read.
+// K-contiguous: LDS rows of 128 bytes, their 16-byte chunks XOR-permuted on the DMA's source address so that a fragment read falls on
+// different slots of the 256-byte bank row (gemm16d.h).
 // K-strided (16-bit): the image in memory order, read transposed (gemm16d.h).
 template <int ROWS, int W, int NW, int SB, bool KS, bool PAIRED, bool GATED>
 struct FzOperand {
@@ -159,16 +159,12 @@ struct FzOperand {
   static constexpr int HALVES = SB / 64, KROWS = SB / 2;  // MFMA steps a slot; KS: k rows a slot
   static constexpr int NADDR = KS ? (PAIRED ? NP + ODD : NT) : HALVES * (1 + ODD);
   static constexpr int SLOT = ROWS * SB;
+  static_assert(KS || SB == 128, "64-byte slots: K-strided operands");
   static_assert(WEXT % 16 == 0 && (!GATED || (PAIRED && !KS && NT % 4 == 0 && !SPARE)), "tile shape");
 
   unsigned voff[PPW], rd[NADDR], beyond;  // beyond: K-contiguous: K4_OOB where this lane's chunk lies beyond K in the last step of a segment
   const char *org, *cur;                  // the tile's first byte in plane 0; the next K step's
   unsigned kstep, tail_bytes;             // bytes a step advances; K-strided: bytes of the rows that the last step of a segment has
-  static __device__ __forceinline__ int swz(int r) {
-    if constexpr (SB == 128) return g16d_swz_kc<PAIRED>(r);
-    const int j = (r >> (PAIRED ? 3 : 2)) & 3;
-    return ((j << 1) & 3) ^ ((j >> 1) * 3);  // 0 2 3 1
-  }
   static __device__ __forceinline__ int piece_row(int j) {  // row (KC) or k row (KS) of this lane in piece j of its wave
     const int wave = (int)(threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
     if constexpr (!KS) return 1024 / SB * (wave + NW * j) + lane / (SB / 16);
@@ -176,7 +172,7 @@ struct FzOperand {
   }
   static __device__ __forceinline__ int piece_chunk(int j) {
     const int lane = (int)threadIdx.x & 63;
-    if constexpr (!KS) return (lane % (SB / 16)) ^ swz(piece_row(j));
+    if constexpr (!KS) return (lane % (SB / 16)) ^ g16d_swz_kc<PAIRED>(piece_row(j));
     else return ((64 * (int)((threadIdx.x >> 6) + NW * j) + lane) % CH) ^ (XOR ? g16d_swz_ks<PAIRED, CH>(piece_row(j)) : 0);
   }
   __device__ __forceinline__ void setup(const void* base, int64_t ld, int r0, int ext, int kdim, int kb, int stage_off, int wsel, int second) {
@@ -196,8 +192,8 @@ struct FzOperand {
       const int o = wsel * WEXT + 32 * NP + li;  // ODD: the last tile's row
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        rd[h] = (unsigned)(stage_off + r * SB + (((4 * h + g) ^ swz(r)) << 4));
-        if constexpr (ODD) rd[HALVES + h] = (unsigned)(stage_off + o * SB + (((4 * h + g) ^ swz(o)) << 4));
+        rd[h] = (unsigned)(stage_off + r * SB + (((4 * h + g) ^ g16d_swz_kc<PAIRED>(r)) << 4));
+        if constexpr (ODD) rd[HALVES + h] = (unsigned)(stage_off + o * SB + (((4 * h + g) ^ g16d_swz_kc<PAIRED>(o)) << 4));
       }
     } else {
       org = static_cast<const char*>(base) + (int64_t)r0 * 2;
@@ -409,7 +405,7 @@ struct FzKernel {
   using OA = FzOperand<BM, WR, NW, SB, A_KS, false, false>;
   using OB = FzOperand<BN, WC, NW, SB, B_KS, true, GATED>;
   static constexpr int STAGE = OA::SLOT + OB::SLOT, SPARE = OA::SPARE || OB::SPARE ? 1024 : 0;
-  // Two slots of 64 KiB are the whole LDS, and what HBM takes to deliver the next one shows.  The 256 x 256 tile's waves therefore ask for one
+  // A third slot of 64 KiB does not fit the LDS, and what HBM takes to deliver the next one shows.  The 256 x 256 tile's waves therefore ask for one
   // word of every cache line of the slot PFD ahead of the one they fill (into spare LDS: nobody reads it), so that the lines are in the
   // L2 when their turn comes.  The workgroups of an XCD that share rows share them out: 8 row tiles those of B, 4 columns of tiles
   // those of A, one instruction a wave and slot.  dx 4096 x 1280, K = 10240 in three parts: 124 -> 105 us.  Not for other tiles (deeper

@@ -895,7 +895,8 @@ def int8_quantize(x):
     """x [..., K] -> (q int8 [..., K], scale fp32 [...]): rows to 8-bit integers, scale = max|x| / 127 of the row, q = 127 x / max|x| rounded
     half to even (exactly: no element is off by a step).  Rows of activations are tokens, rows of a weight [N, K] its output channels.
 
-    q lies in rows of a 128-byte pitch, as int8_linear / int8_matmul read it without a copy.  A row of zeros has scale 0; a row that holds
+    q lies in rows of a 128-byte pitch, as int8_linear and int8_matmul read a weight without a copy; so does int8_matmul its first operand where K is a
+    multiple of 16 (else it makes one with zeros behind K, which it cannot take for granted).  A row of zeros has scale 0; a row that holds
     an infinity or a NaN has scale NaN (and q = 0), so that its products are NaN.  Not differentiable: the result carries no gradient."""
     x = x.detach()
     return _host.int8_quantize(x) if not x.is_cuda else _frozen_op("int8_quantize")(x)
@@ -913,8 +914,9 @@ def int8_linear(x, wq, w_scale, bias=None, base=None):
     """A frozen nn.Linear held in 8 bits: x [..., K] is quantised row by row, multiplied with wq [N, K] (int8) and scaled by both scales,
     plus bias [N] and `base` [..., N] (an adapter's output, same dtype as x), in one epilogue.
 
-    Differentiable in x and base.  The gradient is not quantised: dx = g (w_scale wq), the derivative of the layer with its weight as it is
-    held, with the rounding of x passed straight through.  The weight, its scale and the bias are frozen (a bias or scale that requires a
+    Differentiable in x and base, in reverse mode and once.  The gradient is not quantised: dx = g (w_scale wq), the derivative of the layer with
+    its weight as it is held, with the rounding of x passed straight through; its product keeps 11 bits of g w_scale in bf16, 22 in fp16, 24 in
+    fp32, and the integers as they are.  The weight, its scale and the bias are frozen (a bias or scale that requires a
     gradient is refused).  K is below 2^17, and x has at most 2^26 rows."""
     x = _amp(x)
     if base is not None and base.dtype != x.dtype:
@@ -930,8 +932,9 @@ def gated_linear(x, weight, bias=None, base=None, act="gelu", gate_first=False, 
     comes first (diffusion feed-forwards) unless `gate_first` (stacked gate / up projections).
 
     weight in x's dtype, trainable or frozen, or int8 with `weight_scale` [2 F] (int8_quantize of its rows): x is then quantised row by row
-    as in int8_linear.  Differentiable in x, base, bias and an unquantised weight.  The backward pass reads p in 24 bits (fp32: as it is),
-    3 M 2 F bytes kept from the forward; over an 8-bit weight dx is formed with the weight as it is held.  32-bit products run as sums of bf16 products
+    as in int8_linear.  Differentiable in x, base, bias and an unquantised weight, in reverse mode and once.  The backward pass reads p in 24 bits (fp32:
+    as it is), 3 M 2 F bytes kept from the forward, and multiplies the gradient of p in 11 bits (bf16), 22 (fp16) or 24 (fp32); over an 8-bit weight dx
+    is formed with the weight as it is held.  32-bit products run as sums of bf16 products
     (24 bits; of magnitudes below 2^-108 fewer, 2^-125 of the other factor a term; a row that holds an infinity comes out NaN)."""
     if act not in ACTIVATIONS:
         raise ValueError(f"gated_linear: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
