@@ -224,27 +224,30 @@ int launch_quant(const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, 
   return check_launch("int8_quantize");
 }
 
-// g [M, N] times col into NP fp16 planes, `plane` elements apart, rows of up(N, 8)
+FzPlane plane_job(const int8_t* q, int64_t ldq, void* out, int64_t O, int64_t I) { return FzPlane{q, out, ldq, (int)O, (int)I, (int)cdiv(O, FZ_PLANE_ROWS)}; }
+template <typename T>
+int launch_plane(const FzPlane& w, hipStream_t st) {
+  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)w.groups), dim3(256), 0, st, w);
+  return check_launch("weight plane");
+}
+
+// g [M, N] times col into NP fp16 planes, `plane` elements apart, rows of up(N, 8); and the weight's plane
 template <typename T, int NP>
-int launch_scale(const T* g, const float* col, _Float16* out, int64_t plane, float* scale, int64_t M, int64_t N, hipStream_t st) {
+int launch_scale(const T* g, const float* col, _Float16* out, int64_t plane, float* scale, int64_t M, int64_t N, FzPlane w, hipStream_t st) {
   if (M > ROW_SLAB) {
-    FZ_TRY((launch_scale<T, NP>(g, col, out, plane, scale, ROW_SLAB, N, st)));
-    return launch_scale<T, NP>(g + ROW_SLAB * N, col, out + ROW_SLAB * up(N, 8), plane, scale + ROW_SLAB, M - ROW_SLAB, N, st);
+    FZ_TRY((launch_scale<T, NP>(g, col, out, plane, scale, ROW_SLAB, N, w, st)));
+    w.groups = 0;
+    return launch_scale<T, NP>(g + ROW_SLAB * N, col, out + ROW_SLAB * up(N, 8), plane, scale + ROW_SLAB, M - ROW_SLAB, N, w, st);
   }
   const int vec = fz_al16(g) && N % 8 == 0, vcol = fz_al16(col) && N % 8 == 0;
   row_shape(cdiv(N, 8), [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-    hipLaunchKernelGGL((fz_scale_kernel<T, NP, TPR, NV>), dim3((unsigned)cdiv(M, 256 / TPR)), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec, vcol);
-  }, [&] { hipLaunchKernelGGL((fz_scale_long_kernel<T, NP>), dim3((unsigned)M), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec, vcol); });
+    hipLaunchKernelGGL((fz_scale_kernel<T, NP, TPR, NV>), dim3((unsigned)(w.groups + cdiv(M, 256 / TPR))), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec,
+                       vcol, w);
+  }, [&] { hipLaunchKernelGGL((fz_scale_long_kernel<T, NP>), dim3((unsigned)(w.groups + M)), dim3(256), 0, st, g, col, out, plane, scale, M, (int)N, vec, vcol, w); });
   return check_launch("scaled rows");
 }
 
-template <typename T>
-int launch_plane(const int8_t* q, int64_t ldq, T* out, int64_t O, int64_t I, hipStream_t st) {
-  const int rows = 4;
-  hipLaunchKernelGGL((fz_plane_kernel<T>), dim3((unsigned)cdiv(O, rows)), dim3(256), 0, st, q, ldq, out, up(I, 8), (int)O, (int)I, rows);
-  return check_launch("weight plane");
-}
 // The operands of a pass that have to be staged, and their one launch
 template <typename T>
 struct Stages {
@@ -344,13 +347,14 @@ int dx8(const T* g, const int8_t* wq, int64_t ldw, const float* sw, T* dx, Carve
     *bytes = ws.used;
     return LYC_OK;
   }
-  FZ_TRY(launch_plane<E>(wq, ldw, plane, N, K, st));
+  const FzPlane w = plane_job(wq, ldw, plane, N, K);
   if constexpr (F32) {
+    FZ_TRY(launch_plane<E>(w, st));
     Stages<T> stages;
     stages.add(g, sw, rows, M, N);
     FZ_TRY(stages.run(st));
   } else {
-    FZ_TRY((launch_scale<T, NP>(g, sw, rows, M * ld, scale, M, N, st)));
+    FZ_TRY((launch_scale<T, NP>(g, sw, rows, M * ld, scale, M, N, w, st)));
   }
   FzProb p = prob(rows, ld * 2, M * ld * 2, plane, up(K, 8) * 2, 0, M, K, N, 2);
   segments(p, NP);
@@ -513,7 +517,7 @@ int gated_bwd(const Gated& q, const T* g, const void* pre, const T* x, T* dp, T*
     }
   }
   if (want_dx) {
-    if (held) FZ_TRY(launch_plane<E>(static_cast<const int8_t*>(q.w), q.ldw, b, N, q.I, st));
+    if (held) FZ_TRY(launch_plane<E>(plane_job(static_cast<const int8_t*>(q.w), q.ldw, b, N, q.I), st));
     p = prob(a, ld * 2, q.M * ld * 2, b, ldi * 2, N * ldi * 2, q.M, q.I, N, 2);
     segments(p, gated_segments<T>(held));
     ep.out = dx;

@@ -109,6 +109,44 @@ __global__ __launch_bounds__(256) void fz_quant_long_kernel(const T* __restrict_
   }
 }
 
+// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): its integers, which 16 bits hold exactly; the scales go to the other
+// operand.  Columns I .. ldo are zeros.  A workgroup takes four rows: 10240 x 1280 in 11 us (39 MB), and 5 - 8 us, most of them the launch,
+// for 1280 x 1280 and 1280 x 5120
+// The bytes are taken out by bit-field extracts: written as shifts, the two words become one of 64 bits for the compiler, and its v_lshlrev_b64 by the last
+// register that the kernel has (v23 of 24) gave wrong results now and then on this card, a wave at a time.
+constexpr int FZ_PLANE_ROWS = 4;
+struct FzPlane {
+  const int8_t* q;
+  void* out;
+  int64_t ldq;
+  int O, I, groups;  // groups: workgroups that take rows of it
+};
+template <typename T>
+__device__ __forceinline__ void fz_plane_rows(const FzPlane& p, int group) {
+  const int chunks = (p.I + 7) >> 3;
+  for (int r = 0; r < FZ_PLANE_ROWS; ++r) {
+    const int o = group * FZ_PLANE_ROWS + r;
+    if (o >= p.O) return;
+    const int8_t* q = p.q + (int64_t)o * p.ldq;
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      T t[8];
+      if (8 * c + 8 <= p.I) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(q + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)(float)(int)__builtin_amdgcn_sbfe(w[e >> 2], 8 * (e & 3), 8);  // (the builtin is unsigned)
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)(8 * c + e < p.I ? (float)q[8 * c + e] : 0.f);
+      }
+      *reinterpret_cast<u32x4*>(static_cast<T*>(p.out) + ((int64_t)o * chunks + c) * 8) = *reinterpret_cast<u32x4*>(t);
+    }
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void fz_plane_kernel(FzPlane p) {
+  fz_plane_rows<T>(p, (int)blockIdx.x);
+}
+
 // ---- rows to fp16, scaled: out = 2^e g[m, n] col[n], scale[m] = 2^-e, the operand of dx over an 8-bit weight ------------------------------
 // The largest of a row comes to [2^14, 2^15), so that fp16 holds it with 11 bits down to 2^-28 of it and with a fixed step of 2^-38 below.
 // For bf16 gradients one plane is enough: g col in bf16 instead (8 bits), or col in the weight's plane, costs dx 1.4 times the error of its own
@@ -142,13 +180,15 @@ __device__ __forceinline__ void fz_store_planes(_Float16* out, int64_t plane, fl
     *reinterpret_cast<u32x4*>(out + p * plane) = *reinterpret_cast<u32x4*>(t);
   }
 }
-// the split over threads is fz_quant_kernel's
+// The split over threads is fz_quant_kernel's.  The weight's plane is made in the same launch, by the first w.groups workgroups: dx of a layer is short,
+// and a launch costs 4 us (4096 x 1280 x 1280, forward and dx: 60 -> 56 us).
 template <typename T, int NP, int TPR, int NV>
 __global__ __launch_bounds__(256) void fz_scale_kernel(const T* __restrict__ g, const float* __restrict__ col, _Float16* __restrict__ out, int64_t plane,
-                                                       float* __restrict__ scale, int64_t M, int N, int vec, int vcol) {
+                                                       float* __restrict__ scale, int64_t M, int N, int vec, int vcol, FzPlane w) {
   __shared__ unsigned red[4];
+  if ((int)blockIdx.x < w.groups) return fz_plane_rows<_Float16>(w, (int)blockIdx.x);
   const int t = threadIdx.x % TPR, ldo = (N + 7) & ~7;
-  const int64_t m = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int64_t m = ((int64_t)blockIdx.x - w.groups) * (256 / TPR) + threadIdx.x / TPR;
   float v[NV][8];
   unsigned bits = 0;
   if (m < M) {
@@ -172,9 +212,10 @@ __global__ __launch_bounds__(256) void fz_scale_kernel(const T* __restrict__ g, 
 }
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void fz_scale_long_kernel(const T* __restrict__ g, const float* __restrict__ col, _Float16* __restrict__ out, int64_t plane,
-                                                            float* __restrict__ scale, int64_t M, int N, int vec, int vcol) {
+                                                            float* __restrict__ scale, int64_t M, int N, int vec, int vcol, FzPlane w) {
   __shared__ unsigned red[4];
-  const int64_t m = blockIdx.x, ldo = (N + 7) & ~7;
+  if ((int)blockIdx.x < w.groups) return fz_plane_rows<_Float16>(w, (int)blockIdx.x);
+  const int64_t m = (int64_t)blockIdx.x - w.groups, ldo = (N + 7) & ~7;
   const T* row = g + m * N;
   unsigned bits = 0;
   float v[8];
@@ -190,31 +231,6 @@ __global__ __launch_bounds__(256) void fz_scale_long_kernel(const T* __restrict_
   for (int k = threadIdx.x * 8; k < N; k += 2048) {
     fz_scaled8<T>(row, col, k, N, vec, vcol, v);
     fz_store_planes<NP>(out + m * ldo + k, plane, v, up);
-  }
-}
-
-// ---- the 16-bit plane of an 8-bit weight (the backward pass's operand): its integers, which 16 bits hold exactly; the scales go to the other
-// operand.  Columns I .. ldo are zeros.  A workgroup takes four rows: 10240 x 1280 in 10 us (39 MB), and 5 - 8 us, most of them the launch,
-// for 1280 x 1280 and 1280 x 5120
-template <typename T>
-__global__ __launch_bounds__(256) void fz_plane_kernel(const int8_t* __restrict__ q, int64_t ldq, T* __restrict__ out, int64_t ldo, int O, int I,
-                                                       int rows_per_wg) {
-  const int chunks = (int)(ldo >> 3);
-  for (int r = 0; r < rows_per_wg; ++r) {
-    const int o = blockIdx.x * rows_per_wg + r;
-    if (o >= O) return;
-    for (int c = threadIdx.x; c < chunks; c += 256) {
-      T t[8];
-      if (8 * c + 8 <= I) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(q + (int64_t)o * ldq + 8 * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = (T)(float)(int8_t)(w[e >> 2] >> (8 * (e & 3)));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = (T)(8 * c + e < I ? (float)q[(int64_t)o * ldq + 8 * c + e] : 0.f);
-      }
-      *reinterpret_cast<u32x4*>(out + (int64_t)o * ldo + 8 * c) = *reinterpret_cast<u32x4*>(t);
-    }
   }
 }
 
