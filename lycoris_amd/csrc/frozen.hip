@@ -85,7 +85,7 @@ int launch_tile(const FzProb& p, const FzEpi& ep, hipStream_t st) {
 //   few and K is long, K in parts whose sums a second launch joins.
 // The tile of 160 columns is there for outputs of 320, 640 and 1280 channels, which it cuts into as many tiles as CUs (dx 8192 x 640, K = 5120: 64
 // us, against 83 with 128 x 128 and 127 with 256 x 256); with whole rounds of the larger tile that wins (dx 16384 x 5120, K = 1280: 190 us,
-// against 247 and 283), and in parts of a long K (dx 4096 x 1280, K = 10240, three parts: 106 + 12 us, against 157 with 128 x 128 and 127 with
+// against 247 and 283, on bf16 operands; 212 on fp16 ones), and in parts of a long K (dx 4096 x 1280, K = 10240, three parts: 106 + 12 us, against 157 with 128 x 128 and 127 with
 // 128 x 160).
 // The rule compares estimates in microseconds, from sweeps of 30 shapes with inputs out of HBM: a round costs what a step costs times the
 // steps, plus what a tile's beginning and end leave exposed -- of its epilogue's bytes, at a CU's share of HBM, less where a second
@@ -437,7 +437,7 @@ int dgate_rows(int64_t M, int64_t F) {
 }
 
 // The elementwise pass where products follow, 16 bits: rows of a slab.  512 slabs (of waves: 2048) are two workgroups a CU, whose rows follow each other
-// with the next one's loads in flight: 8192 x 2560 in 69 us, against 82 with 1024 slabs (and twice the partial column sums); 4096 x 5120 in 75, against 78.
+// with the next one's loads in flight: 8192 x 2560 in 69 us, against 82 in the same run with 1024 slabs (and twice the partial column sums); 4096 x 5120 in 75, against 78.
 int dgate_slab_rows(int64_t M, int64_t F) { return (int)cdiv(M, (F <= 512 ? 4 : 1) * 512); }
 template <typename T, int NP, bool SUMS>
 int launch_dgate_rows(const FzDgate& a, int64_t slabs, hipStream_t st) {
