@@ -292,6 +292,7 @@ def test_forward_mode_is_refused_and_not_dropped():
 def test_every_product_kernel_has_its_own_lds_limit_flags():
     """the limit of dynamic LDS is raised per kernel and device, and remembered: one set of flags for all kernels of a type would leave it at
     the default for all but the first one launched"""
+    N.load()
     nm = shutil.which("nm") or "/opt/rocm/llvm/bin/llvm-nm"
     names = subprocess.run([nm, N.lib_path()], check=True, capture_output=True, text=True).stdout.split()
     kernels = [n for n in names if re.search(r"__device_stub__fz_(gemm|skinny)_kernel", n)]

@@ -60,6 +60,7 @@ def test_the_scan_itself():
 
 @pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no llvm-objdump")
 def test_no_instruction_form_that_the_card_gets_wrong(tmp_path):
+    N.load()  # (built, if it is not)
     with open(N.lib_path(), "rb") as f:
         objects = list(code_objects(f.read()))
     assert len(objects) == 2
